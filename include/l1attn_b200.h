@@ -176,6 +176,44 @@ int l1attn_dense_softmax_v_bwd(const void *q, const void *k, const void *v, cons
  */
 int l1attn_test_softmax_v_form(int bs, int n_tok, int n_heads, int width, int v_width, int backward);
 
+/* ------------------------------------------------------------------ masked -------------- */
+
+/*
+ * Masks, cap and bias of masked attention (no counterpart in the reference, whose dense operator sees every pair).  With t a query's
+ * and s a key's position:
+ *   x[t][s] = (-1/sqrt(width)) * sum_w |q[t][w] - k[s][w]|;  x = softcap * tanh(x / softcap) where softcap > 0;  x -= slopes[head] * |t - s|
+ *   t sees s when (no doc, or doc[t] == doc[s] >= 0) and (s < prefix, or (s <= t where causal) and (|t - s| < window where window > 0))
+ * Weights as in l1attn_dense_softmax_v_fwd, over the keys that a query sees.  A query that sees none gets an output of zeros and no gradient;
+ * so does one whose keys are all infinitely far.  A key whose weight is zero contributes nothing, whatever its value row holds.
+ */
+typedef struct l1attn_mask {
+	int causal;            /* 0 or 1 */
+	int window;            /* 0: none */
+	int mode;              /* L1ATTN_SV_* */
+	float softcap;         /* 0: none */
+	const float *slopes;   /* device, [n_heads], or NULL: no bias */
+	const int32_t *doc;    /* device, [bs][n_tok] document of each token, negative: padding; or NULL: one document */
+	const int32_t *prefix; /* device, [bs] length of the prefix that every query sees, or NULL: none */
+} l1attn_mask;
+
+/*
+ * vo[b][t][h][:] = sum_s weight * v[b][s][h / (n_heads / n_kv_heads)][:], and the gradients.  q: [bs][n_tok][n_heads][width], k, v:
+ * [bs][n_tok][n_kv_heads][width / v_width] with n_heads a multiple of n_kv_heads; widths 1 .. 256; dtype L1ATTN_F32, L1ATTN_F16 or L1ATTN_BF16.
+ * strides: nine element strides (batch, token, head of q, then of k, then of v), in host memory; the width is contiguous, 0 repeats
+ * a tensor.  vo, dvo and the gradients are contiguous.  lse: float [bs][n_tok][n_heads], the rows' log-normalisers (NULL in the forward: not
+ * kept).  work: device memory of l1attn_masked_work_bytes() bytes, 256-byte aligned (the forward uses it only with documents and takes NULL
+ * without); nothing in it needs to be initialised or outlives the call, and calls that share it must not overlap on the GPU.
+ * Sums, weights and their normalisers are float32 in every case.  The backward is deterministic.
+ */
+size_t l1attn_masked_work_bytes(int bs, int n_tok, int n_heads, int backward);
+int l1attn_masked_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *vo, float *lse, void *work,
+		      int bs, int n_tok, int n_heads, int n_kv_heads, int width, int v_width,
+		      const l1attn_mask *mask, int dtype, void *stream);
+int l1attn_masked_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *vo, const void *dvo, const float *lse,
+		      void *dq, void *dk, void *dv, void *work,
+		      int bs, int n_tok, int n_heads, int n_kv_heads, int width, int v_width,
+		      const l1attn_mask *mask, int dtype, void *stream);
+
 /* ------------------------------------------------------------------ sparse -------------- */
 
 /*

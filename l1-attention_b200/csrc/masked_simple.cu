@@ -1,0 +1,394 @@
+// Masked L1 attention (mask.cuh), float32 arithmetic for every storage type and widths up to 256.
+//
+// Forward: a CTA owns 64 query rows of one head; keys and values stream in tiles of 64, all operands as floats in shared memory.  256
+// threads, a 4 x 4 tile of scores each (rows 4 ty + i, keys tx + 16 j); the 16 lanes of a half-warp own their four rows, so the running maximum
+// and sum (one pass over the keys) and the weights never leave the half-warp.  Bound: FP32 instructions, two per term of the distance.
+// Backward: two kernels without atomics.  One owns 64 query rows and makes dq, the other 64 key rows and makes dk and dv (summed
+// over the query heads that share them, in order); both recompute the weights from the log-normalisers and stream the other side in
+// tiles of 32.  sign(0) = 0.
+#include "mask.cuh"
+
+namespace l1b {
+
+namespace {
+
+constexpr int OWN = 64, KEYS = 64, STREAM = 32, THREADS = 256;
+
+// floats of a row of `w` values: whole float4s, an odd number of them so that 8 rows at one column lie in different banks
+__host__ __device__ inline int pitch(int w)
+{
+	const int p = (w + 3) / 4;
+	return 4 * (p % 2 ? p : p + 1);
+}
+
+// rows [first, first + rows) of one head as floats, zeros past n and past the width (to `cols` columns); true when a value is not finite
+template <typename T>
+__device__ bool load_rows(float *dst, int pitch_, int cols, const Strided &x, int b, int head, int first, int rows, int n, int width)
+{
+	const T *src = static_cast<const T *>(x.p) + b * x.batch + head * x.head;
+	bool odd = false;
+	for (int r = threadIdx.x / 32; r < rows; r += THREADS / 32)
+		for (int c = threadIdx.x % 32; c < cols; c += 32) {
+			const float f = first + r < n && c < width ? to_float(src[(first + r) * x.tok + c]) : 0.f;
+			odd |= !(fabsf(f) < INFINITY);
+			dst[r * pitch_ + c] = f;
+		}
+	return odd;
+}
+
+__device__ __forceinline__ float half_warp_max(float x)
+{
+#pragma unroll
+	for (int o = 8; o; o >>= 1)
+		x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+	return x;
+}
+__device__ __forceinline__ float half_warp_sum(float x)
+{
+#pragma unroll
+	for (int o = 8; o; o >>= 1)
+		x += __shfl_xor_sync(0xffffffffu, x, o);
+	return x;
+}
+
+// sum_w |a[row i] - b[key j]| of this thread's 4 x J pairs (columns past the width are zeros)
+template <int J> __device__ __forceinline__ void distances(const float *A, const float *B, int ap, int cols, int ty, int tx, float (&d)[4][J])
+{
+#pragma unroll
+	for (int i = 0; i < 4; i++)
+#pragma unroll
+		for (int j = 0; j < J; j++)
+			d[i][j] = 0.f;
+	for (int w = 0; w < cols; w += 4) {
+		float4 x[4], y[J];
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+			x[i] = *reinterpret_cast<const float4 *>(A + (4 * ty + i) * ap + w);
+#pragma unroll
+		for (int j = 0; j < J; j++)
+			y[j] = *reinterpret_cast<const float4 *>(B + (tx + 16 * j) * ap + w);
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+#pragma unroll
+			for (int j = 0; j < J; j++)
+				d[i][j] += (fabsf(x[i].x - y[j].x) + fabsf(x[i].y - y[j].y)) + (fabsf(x[i].z - y[j].z) + fabsf(x[i].w - y[j].w));
+	}
+}
+template <int J> __device__ __forceinline__ void products(const float *A, const float *B, int ap, int cols, int ty, int tx, float (&d)[4][J])
+{
+#pragma unroll
+	for (int i = 0; i < 4; i++)
+#pragma unroll
+		for (int j = 0; j < J; j++)
+			d[i][j] = 0.f;
+	for (int w = 0; w < cols; w += 4) {
+		float4 x[4], y[J];
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+			x[i] = *reinterpret_cast<const float4 *>(A + (4 * ty + i) * ap + w);
+#pragma unroll
+		for (int j = 0; j < J; j++)
+			y[j] = *reinterpret_cast<const float4 *>(B + (tx + 16 * j) * ap + w);
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+#pragma unroll
+			for (int j = 0; j < J; j++)
+				d[i][j] = fmaf(x[i].x, y[j].x, fmaf(x[i].y, y[j].y, fmaf(x[i].z, y[j].z, fmaf(x[i].w, y[j].w, d[i][j]))));
+	}
+}
+
+template <typename T, int NV> __global__ void __launch_bounds__(THREADS) masked_fwd_simple_kernel(MaskedArgs a, T *vo, float *lse, int tiles)
+{
+	extern __shared__ float4 smem4[];
+	const int wp = pitch(a.width), vp = 64 * NV, tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
+	float *Q = reinterpret_cast<float *>(smem4), *K = Q + OWN * wp, *V = K + KEYS * wp, *P = V + KEYS * vp;
+	constexpr int PP = KEYS + 4;
+	const int tile = tiles - 1 - int(blockIdx.x % tiles); // the longest rows of a causal mask first
+	const int head = (blockIdx.x / tiles) % a.heads, b = blockIdx.x / tiles / a.heads, kv = head / (a.heads / a.kv_heads);
+	const MaskView mask(a, b);
+	const int t0 = tile * OWN, t1 = min(a.n, t0 + OWN);
+	const float slope = a.slopes ? a.slopes[head] : 0.f, inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
+	load_rows<T>(Q, wp, wp, a.q, b, head, t0, OWN, a.n, a.width);
+	float m[4], l[4], acc[4][4 * NV];
+	int doc_t[4];
+#pragma unroll
+	for (int i = 0; i < 4; i++) {
+		m[i] = start_max(a.mode);
+		l[i] = start_sum(a.mode);
+		doc_t[i] = mask.doc && t0 + 4 * ty + i < a.n ? mask.doc[t0 + 4 * ty + i] : 0;
+#pragma unroll
+		for (int c = 0; c < 4 * NV; c++)
+			acc[i][c] = 0.f;
+	}
+	for (int s0 = 0; s0 < a.n; s0 += KEYS) {
+		const int s1 = min(a.n, s0 + KEYS);
+		if (!mask.any(t0, t1, s0, s1))
+			continue;
+		__syncthreads();
+		load_rows<T>(K, wp, wp, a.k, b, kv, s0, KEYS, a.n, a.width);
+		const bool odd = __syncthreads_or(load_rows<T>(V, vp, vp, a.v, b, kv, s0, KEYS, a.n, a.v_width));
+		float x[4][4];
+		distances<4>(Q, K, wp, a.width, ty, tx, x);
+#pragma unroll
+		for (int i = 0; i < 4; i++) {
+			const int t = t0 + 4 * ty + i;
+			float top = m[i];
+#pragma unroll
+			for (int j = 0; j < 4; j++) {
+				const int s = s0 + tx + 16 * j;
+				float y = -a.scale * x[i][j];
+				if (a.cap > 0.f)
+					y = a.cap * tanhf(y * inv_cap);
+				y -= slope * fabsf(float(t - s));
+				x[i][j] = mask.sees(t, s, doc_t[i], mask.doc && s < a.n ? mask.doc[s] : 0) ? y : -INFINITY;
+				top = fmaxf(top, x[i][j]);
+			}
+			top = half_warp_max(top);
+			const float ref = top == -INFINITY ? 0.f : top, keep = expf(m[i] - ref);
+			float sum = 0.f;
+#pragma unroll
+			for (int j = 0; j < 4; j++) {
+				const float p = expf(x[i][j] - ref);
+				sum += p;
+				P[(4 * ty + i) * PP + tx + 16 * j] = p;
+			}
+			l[i] = l[i] * keep + half_warp_sum(sum);
+			m[i] = top;
+#pragma unroll
+			for (int c = 0; c < 4 * NV; c++)
+				acc[i][c] *= keep;
+		}
+		__syncwarp();
+		for (int s = 0; s < s1 - s0; s++) {
+			float p[4];
+#pragma unroll
+			for (int i = 0; i < 4; i++)
+				p[i] = P[(4 * ty + i) * PP + s];
+#pragma unroll
+			for (int u = 0; u < NV; u++) {
+				const float4 v = *reinterpret_cast<const float4 *>(V + s * vp + 64 * u + 4 * tx);
+#pragma unroll
+				for (int i = 0; i < 4; i++) {
+					if (odd && p[i] == 0.f)
+						continue;
+					acc[i][4 * u] = fmaf(p[i], v.x, acc[i][4 * u]);
+					acc[i][4 * u + 1] = fmaf(p[i], v.y, acc[i][4 * u + 1]);
+					acc[i][4 * u + 2] = fmaf(p[i], v.z, acc[i][4 * u + 2]);
+					acc[i][4 * u + 3] = fmaf(p[i], v.w, acc[i][4 * u + 3]);
+				}
+			}
+		}
+	}
+#pragma unroll
+	for (int i = 0; i < 4; i++) {
+		const int t = t0 + 4 * ty + i;
+		if (t >= a.n)
+			continue;
+		const long long row = ((long long)b * a.n + t) * a.heads + head;
+		float ls;
+		const float f = finish_row(a.mode, m[i], l[i], &ls);
+		if (tx == 0 && lse)
+			lse[row] = ls;
+#pragma unroll
+		for (int c = 0; c < 4 * NV; c++) {
+			const int w = 64 * (c / 4) + 4 * tx + c % 4;
+			if (w < a.v_width)
+				vo[row * a.v_width + w] = from_float<T>(f == 0.f ? 0.f : acc[i][c] * f);
+		}
+	}
+}
+
+// OWN_KEYS: a CTA owns 64 keys of one key-value head and makes their dk and dv; else 64 queries of one head, dq.
+template <typename T, bool OWN_KEYS, int NW, int NV>
+__global__ void __launch_bounds__(THREADS) masked_bwd_simple_kernel(MaskedArgs a, const T *dvo, const float *lse, const float *delta, T *dq, T *dk, T *dv, int tiles)
+{
+	extern __shared__ float4 smem4[];
+	const int wp = pitch(64 * NW), vp = pitch(64 * NV), tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
+	constexpr int GP = STREAM + 4;
+	float *A = reinterpret_cast<float *>(smem4), *B = A + OWN * wp, *C = B + OWN * vp, *D = C + STREAM * wp, *G = D + STREAM * vp, *P = G + OWN * GP;
+	const int own_heads = OWN_KEYS ? a.kv_heads : a.heads, group = a.heads / a.kv_heads;
+	const int tile = OWN_KEYS ? int(blockIdx.x % tiles) : tiles - 1 - int(blockIdx.x % tiles);
+	const int own = (blockIdx.x / tiles) % own_heads, b = blockIdx.x / tiles / own_heads;
+	const MaskView mask(a, b);
+	const int o0 = tile * OWN, o1 = min(a.n, o0 + OWN);
+	const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
+	const Strided go = {dvo, (long long)a.n * a.heads * a.v_width, (long long)a.heads * a.v_width, a.v_width};
+	load_rows<T>(A, wp, wp, OWN_KEYS ? a.k : a.q, b, own, o0, OWN, a.n, a.width);
+	load_rows<T>(B, vp, vp, OWN_KEYS ? a.v : go, b, own, o0, OWN, a.n, a.v_width);
+	float acc[4][4 * NW], accv[4][OWN_KEYS ? 4 * NV : 1];
+#pragma unroll
+	for (int i = 0; i < 4; i++) {
+#pragma unroll
+		for (int c = 0; c < 4 * NW; c++)
+			acc[i][c] = 0.f;
+#pragma unroll
+		for (int c = 0; c < (OWN_KEYS ? 4 * NV : 1); c++)
+			accv[i][c] = 0.f;
+	}
+	for (int g = 0; g < (OWN_KEYS ? group : 1); g++) {
+		const int head = OWN_KEYS ? own * group + g : own;
+		const float slope = a.slopes ? a.slopes[head] : 0.f;
+		for (int r0 = 0; r0 < a.n; r0 += STREAM) {
+			const int r1 = min(a.n, r0 + STREAM);
+			if (OWN_KEYS ? !mask.any(r0, r1, o0, o1) : !mask.any(o0, o1, r0, r1))
+				continue;
+			__syncthreads();
+			load_rows<T>(C, wp, wp, OWN_KEYS ? a.q : a.k, b, OWN_KEYS ? head : own / group, r0, STREAM, a.n, a.width);
+			const bool odd = __syncthreads_or(load_rows<T>(D, vp, vp, OWN_KEYS ? go : a.v, b, OWN_KEYS ? head : own / group, r0, STREAM, a.n, a.v_width));
+			float x[4][2], dp[4][2];
+			distances<2>(A, C, wp, a.width, ty, tx, x);
+			products<2>(B, D, vp, a.v_width, ty, tx, dp);
+#pragma unroll
+			for (int i = 0; i < 4; i++)
+#pragma unroll
+				for (int j = 0; j < 2; j++) {
+					const int o = o0 + 4 * ty + i, r = r0 + tx + 16 * j, t = OWN_KEYS ? r : o, s = OWN_KEYS ? o : r;
+					float p = 0.f, e = 0.f;
+					if (t < a.n && s < a.n && mask.sees(t, s, mask.doc ? mask.doc[t] : 0, mask.doc ? mask.doc[s] : 0)) {
+						const long long row = ((long long)b * a.n + t) * a.heads + head;
+						float y = -a.scale * x[i][j], slant = 1.f;
+						if (a.cap > 0.f) {
+							const float th = tanhf(y * inv_cap);
+							slant = 1.f - th * th;
+							y = a.cap * th;
+						}
+						p = weight_of(y - slope * fabsf(float(t - s)), lse[row]);
+						if (p != 0.f)
+							e = -a.scale * slant * p * (dp[i][j] - delta[row]);
+					}
+					G[(4 * ty + i) * GP + tx + 16 * j] = e;
+					if (OWN_KEYS)
+						P[(4 * ty + i) * GP + tx + 16 * j] = p;
+				}
+			__syncwarp();
+			for (int r = 0; r < r1 - r0; r++) {
+				float e[4], p[4];
+#pragma unroll
+				for (int i = 0; i < 4; i++) {
+					e[i] = G[(4 * ty + i) * GP + r];
+					p[i] = OWN_KEYS ? P[(4 * ty + i) * GP + r] : 0.f;
+				}
+#pragma unroll
+				for (int u = 0; u < NW; u++) {
+					const float4 y = *reinterpret_cast<const float4 *>(C + r * wp + 64 * u + 4 * tx);
+#pragma unroll
+					for (int i = 0; i < 4; i++) {
+						const float4 z = *reinterpret_cast<const float4 *>(A + (4 * ty + i) * wp + 64 * u + 4 * tx);
+						acc[i][4 * u] += sign_apply(z.x - y.x, e[i]);
+						acc[i][4 * u + 1] += sign_apply(z.y - y.y, e[i]);
+						acc[i][4 * u + 2] += sign_apply(z.z - y.z, e[i]);
+						acc[i][4 * u + 3] += sign_apply(z.w - y.w, e[i]);
+					}
+				}
+				if (OWN_KEYS) {
+#pragma unroll
+					for (int u = 0; u < NV; u++) {
+						const float4 y = *reinterpret_cast<const float4 *>(D + r * vp + 64 * u + 4 * tx);
+#pragma unroll
+						for (int i = 0; i < 4; i++) {
+							if (odd && p[i] == 0.f)
+								continue;
+							accv[i][(4 * u) % (OWN_KEYS ? 4 * NV : 1)] += p[i] * y.x;
+							accv[i][(4 * u + 1) % (OWN_KEYS ? 4 * NV : 1)] += p[i] * y.y;
+							accv[i][(4 * u + 2) % (OWN_KEYS ? 4 * NV : 1)] += p[i] * y.z;
+							accv[i][(4 * u + 3) % (OWN_KEYS ? 4 * NV : 1)] += p[i] * y.w;
+						}
+					}
+				}
+			}
+		}
+	}
+#pragma unroll
+	for (int i = 0; i < 4; i++) {
+		const int o = o0 + 4 * ty + i;
+		if (o >= a.n)
+			continue;
+		const long long row = ((long long)b * a.n + o) * own_heads + own;
+#pragma unroll
+		for (int c = 0; c < 4 * NW; c++) {
+			const int w = 64 * (c / 4) + 4 * tx + c % 4;
+			if (w < a.width)
+				(OWN_KEYS ? dk : dq)[row * a.width + w] = from_float<T>(acc[i][c]);
+		}
+		if (OWN_KEYS)
+#pragma unroll
+			for (int c = 0; c < (OWN_KEYS ? 4 * NV : 1); c++) {
+				const int w = 64 * (c / 4) + 4 * tx + c % 4;
+				if (w < a.v_width)
+					dv[row * a.v_width + w] = from_float<T>(accv[i][c]);
+			}
+	}
+}
+
+int grid_of(long long n, unsigned *out)
+{
+	if (n > 0x7fffffffll)
+		return L1ATTN_ERR_SHAPE;
+	*out = unsigned(n);
+	return L1ATTN_OK;
+}
+
+template <typename T, int NV> int fwd(const MaskedArgs &a, void *vo, float *lse, cudaStream_t st)
+{
+	const int tiles = (a.n + OWN - 1) / OWN, bytes = 4 * (OWN * pitch(a.width) + KEYS * pitch(a.width) + KEYS * 64 * NV + OWN * (KEYS + 4));
+	unsigned grid = 0;
+	if (int rc = grid_of((long long)tiles * a.heads * a.bs, &grid))
+		return rc;
+	L1B_SHARED_MEMORY((masked_fwd_simple_kernel<T, NV>), bytes);
+	masked_fwd_simple_kernel<T, NV><<<grid, THREADS, bytes, st>>>(a, static_cast<T *>(vo), lse, tiles);
+	L1B_LAUNCH_CHECK();
+	return L1ATTN_OK;
+}
+
+template <typename T, bool OWN_KEYS, int NW, int NV>
+int bwd_one(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, cudaStream_t st)
+{
+	const int wp = pitch(64 * NW), vp = pitch(64 * NV);
+	const int tiles = (a.n + OWN - 1) / OWN, bytes = 4 * ((OWN + STREAM) * (wp + vp) + (OWN_KEYS ? 2 : 1) * OWN * (STREAM + 4));
+	unsigned grid = 0;
+	if (int rc = grid_of((long long)tiles * (OWN_KEYS ? a.kv_heads : a.heads) * a.bs, &grid))
+		return rc;
+	L1B_SHARED_MEMORY((masked_bwd_simple_kernel<T, OWN_KEYS, NW, NV>), bytes);
+	masked_bwd_simple_kernel<T, OWN_KEYS, NW, NV>
+	    <<<grid, THREADS, bytes, st>>>(a, static_cast<const T *>(dvo), lse, delta, static_cast<T *>(dq), static_cast<T *>(dk), static_cast<T *>(dv), tiles);
+	L1B_LAUNCH_CHECK();
+	return L1ATTN_OK;
+}
+
+template <typename T, int NW, int NV>
+int bwd(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, cudaStream_t st)
+{
+	if (int rc = bwd_one<T, false, NW, NV>(a, dvo, lse, delta, dq, dk, dv, st))
+		return rc;
+	return bwd_one<T, true, NW, NV>(a, dvo, lse, delta, dq, dk, dv, st);
+}
+
+template <typename T> int fwd_type(const MaskedArgs &a, void *vo, float *lse, cudaStream_t st)
+{
+	return a.v_width <= 64 ? fwd<T, 1>(a, vo, lse, st) : a.v_width <= 128 ? fwd<T, 2>(a, vo, lse, st) : fwd<T, 4>(a, vo, lse, st);
+}
+template <typename T>
+int bwd_type(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, cudaStream_t st)
+{
+	const int w = a.width > a.v_width ? a.width : a.v_width;
+	return w <= 64 ? bwd<T, 1, 1>(a, dvo, lse, delta, dq, dk, dv, st) : w <= 128 ? bwd<T, 2, 2>(a, dvo, lse, delta, dq, dk, dv, st) :
+											    bwd<T, 4, 4>(a, dvo, lse, delta, dq, dk, dv, st);
+}
+
+} // namespace
+
+int masked_simple_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st)
+{
+	return dtype == L1ATTN_F32 ? fwd_type<float>(a, vo, lse, st) : dtype == L1ATTN_F16 ? fwd_type<__half>(a, vo, lse, st) :
+											     fwd_type<__nv_bfloat16>(a, vo, lse, st);
+}
+
+int masked_simple_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, int dtype,
+			     cudaStream_t st)
+{
+	return dtype == L1ATTN_F32 ? bwd_type<float>(a, dvo, lse, delta, dq, dk, dv, st) :
+	       dtype == L1ATTN_F16 ? bwd_type<__half>(a, dvo, lse, delta, dq, dk, dv, st) :
+				     bwd_type<__nv_bfloat16>(a, dvo, lse, delta, dq, dk, dv, st);
+}
+
+} // namespace l1b

@@ -37,6 +37,9 @@ SIGNATURES = {
     "l1attn_dense_softmax_v_bwd_dx": (_i, [_vp] * 8 + [_i] * 6 + [_vp]),
     "l1attn_dense_bwd_scratch_bytes": (_sz, [_i] * 5),
     "l1attn_dense_bwd": (_i, [_vp] * 6 + [_i] * 5 + [_vp]),
+    "l1attn_masked_work_bytes": (_sz, [_i] * 4),
+    "l1attn_masked_fwd": (_i, [_vp] * 7 + [_i] * 6 + [_vp, _i, _vp]),
+    "l1attn_masked_bwd": (_i, [_vp] * 11 + [_i] * 6 + [_vp, _i, _vp]),
     "l1attn_sparse_index_bytes": (_sz, [_i] * 3),
     "l1attn_sparse_build_index": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
     "l1attn_sparse_fwd": (_i, [_vp] * 7 + [_i] * 10 + [_vp]),
@@ -290,6 +293,50 @@ def dense_softmax_v_bwd(q, k, v, dvo, lse, delta, dq, dk, dv, work):
     assert work.numel() * work.element_size() >= lib().l1attn_dense_softmax_v_bwd_bytes(bs, n, h, w, v.shape[3], _tdt(q))
     _check(lib().l1attn_dense_softmax_v_bwd(_dp(q), _dp(k), _dp(v), _dp(dvo), _dp(lse), _dp(delta), _dp(dq), _dp(dk), _dp(dv),
                                             _dp(work), bs, n, h, w, v.shape[3], _tdt(q), _stream()), "l1attn_dense_softmax_v_bwd")
+
+
+class Mask(ctypes.Structure):
+    """l1attn_mask; keeps the tensors whose addresses it holds."""
+    _fields_ = [("causal", _i), ("window", _i), ("mode", _i), ("softcap", _c.c_float), ("slopes", _vp), ("doc", _vp), ("prefix", _vp)]
+
+    def __init__(self, mode="softmax", causal=True, window=0, softcap=0.0, slopes=None, doc=None, prefix=None):
+        super().__init__(int(bool(causal)), int(window), SV_MODES[mode], float(softcap), _dp(slopes), _dp(doc), _dp(prefix))
+        self.tensors = (slopes, doc, prefix)
+
+
+def _strides(*tensors):
+    return (_c.c_int64 * 9)(*(s for t in tensors for s in t.stride()[:3]))
+
+
+def _masked_work(q, doc, backward):
+    import torch
+    if doc is None and not backward:
+        return None
+    bs, n, h, _ = q.shape
+    return torch.empty(lib().l1attn_masked_work_bytes(bs, n, h, int(backward)), dtype=torch.uint8, device=q.device)
+
+
+def masked_fwd(q, k, v, mask, lse=True):
+    """q [bs, n, h, w], k [bs, n, hk, w], v [bs, n, hk, wv] of any strides with contiguous widths -> (vo, lse [bs, n, h] or None)."""
+    import torch
+    (bs, n, h, w), (hk, wv) = q.shape, v.shape[2:]
+    vo = torch.empty((bs, n, h, wv), dtype=q.dtype, device=q.device)
+    ls = torch.empty((bs, n, h), dtype=torch.float32, device=q.device) if lse else None
+    work = _masked_work(q, mask.tensors[1], False)
+    _check(lib().l1attn_masked_fwd(_dp(q), _dp(k), _dp(v), _strides(q, k, v), _dp(vo), _dp(ls), _dp(work), bs, n, h, hk, w, wv, _c.byref(mask),
+                                   _tdt(q, allow16=True), _stream()), "l1attn_masked_fwd")
+    return vo, ls
+
+
+def masked_bwd(q, k, v, vo, dvo, lse, mask):
+    """-> (dq, dk, dv), contiguous; vo, dvo, lse contiguous."""
+    import torch
+    (bs, n, h, w), (hk, wv) = q.shape, v.shape[2:]
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    work = _masked_work(q, mask.tensors[1], True)
+    _check(lib().l1attn_masked_bwd(_dp(q), _dp(k), _dp(v), _strides(q, k, v), _dp(vo), _dp(dvo), _dp(lse), _dp(dq), _dp(dk), _dp(dv), _dp(work), bs, n, h,
+                                   hk, w, wv, _c.byref(mask), _tdt(q, allow16=True), _stream()), "l1attn_masked_bwd")
+    return dq, dk, dv
 
 
 def dense_bwd(d_attn, q, k, out=None, scratch="auto"):
