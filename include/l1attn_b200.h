@@ -214,6 +214,61 @@ int l1attn_masked_bwd(const void *q, const void *k, const void *v, const int64_t
 		      int bs, int n_tok, int n_heads, int n_kv_heads, int width, int v_width,
 		      const l1attn_mask *mask, int dtype, void *stream);
 
+/* ------------------------------------------------------------------ cache -------------- */
+
+/*
+ * A paged cache of keys and values in 8 bits (no counterpart in the reference).  A page holds `page` consecutive tokens of one sequence, for
+ * all heads; the tokens of a page share one float scale per head, for keys and for values: value = scale * code, codes -127 .. 127.
+ *   k_codes [n_pages][n_kv_heads][page][width], v_codes [n_pages][n_kv_heads][page][v_width], k_scale, v_scale [n_pages][n_kv_heads]
+ * page: 16, 32, 64, 128 or 256; widths 1 .. 256; codes 16-byte aligned.
+ * Calls take some sequences at once.  Sequence i's rows of the token tensors are [cu[i], cu[i+1]) and stand at its positions start[i],
+ * start[i] + 1, ...; its position p is in page table[i][p / page].  Rows behind cu[n_seqs] belong to no sequence: nothing reads or writes them.
+ * table, start and cu are device memory and may change between replays of a captured call.  Entries of table past a sequence's last page
+ * are not looked at.  A page id, a start or an offset out of range is never followed: its tokens are left out (keys: not seen; gathered rows: zeros) and
+ * *status, where given, is set to L1ATTN_ERR_INDEX.
+ */
+typedef struct l1attn_cache {
+	int8_t *k_codes, *v_codes;
+	float *k_scale, *v_scale;
+	int n_pages, page, n_kv_heads, width, v_width;
+	const int32_t *table; /* [n_seqs][max_pages] */
+	const int32_t *start; /* [n_seqs] */
+	const int32_t *cu;    /* [n_seqs + 1] */
+	int n_seqs, max_pages;
+	int32_t *status; /* device int32, or NULL */
+} l1attn_cache;
+
+/*
+ * Quantises new tokens into their pages.  k: [rows][n_kv_heads][width], v: [rows][n_kv_heads][v_width], dtype L1ATTN_F32, F16 or BF16;
+ * strides: row and head of k, then of v, in elements.  Per page and head: scale = max |x| / 127 over the new tokens of the page, or the page's scale where that
+ * is larger and the page holds earlier tokens of the sequence; code = x / scale to the nearest, ties to even, of the exact quotient;
+ * codes of earlier tokens follow a scale that grows (code * old / new, rounded alike).  NaN is stored as 0, infinities as +-127.  No two sequences of a call
+ * may write the same page.
+ */
+int l1attn_cache_append(const l1attn_cache *cache, const void *k, const void *v, const int64_t *strides, int rows, int dtype, void *stream);
+/* What the cache holds at the given positions: k [rows][n_kv_heads][width], v [rows][n_kv_heads][v_width], contiguous, rounded to dtype. */
+int l1attn_cache_gather(const l1attn_cache *cache, void *k, void *v, int rows, int dtype, void *stream);
+/*
+ * Page src[i] -> page dst[i], codes and scales, for n pairs (device memory) and `layers` caches that lie behind one another.  A page may be the
+ * source of several; no destination is another pair's source or destination.  Only the cache's tensors, sizes and status are looked at.
+ */
+int l1attn_cache_copy_pages(const l1attn_cache *cache, int layers, const int32_t *src, const int32_t *dst, int n, void *stream);
+/*
+ * Attention of q [rows][n_heads][width] (n_heads a multiple of n_kv_heads; strides: row and head) to the cache: each row sees the keys at its own and
+ * earlier positions of its sequence, scored, capped, biased, windowed and normalised as l1attn_mask says (causal must be 1, doc and prefix NULL);
+ * vo [rows][n_heads][v_width] contiguous.  max_len: the longest start + count that the caller knows of; it shapes the launch alone, any value gives
+ * right results.  work: device memory of l1attn_cache_attend_bytes() bytes for the same sizes, 256-byte aligned, as in l1attn_masked_fwd.
+ */
+size_t l1attn_cache_attend_bytes(const l1attn_cache *cache, int rows, int n_heads, int max_len, int dtype);
+int l1attn_cache_attend(const l1attn_cache *cache, const void *q, const int64_t *strides, void *vo, void *work, int rows, int n_heads, int max_len,
+			const l1attn_mask *mask, int dtype, void *stream);
+/*
+ * Test hook, not an operator, on the host alone: table, start, cu and status in HOST memory.  What the kernels make of work unit `unit` of a call whose
+ * sequences' units begin at cu[i] * num / den + i * extra: out = {sequence, first row, rows, start, the unit's number within the sequence, id of
+ * page `slot` (-1: out of range)}.
+ */
+int l1attn_test_cache_unit(const l1attn_cache *cache, int rows, long long unit, int num, int den, int extra, int slot, int32_t *out);
+
 /* ------------------------------------------------------------------ sparse -------------- */
 
 /*

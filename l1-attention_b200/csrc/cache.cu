@@ -1,0 +1,158 @@
+// The 8-bit cache: entry points, argument checks, and how attention to it is split over its long axis.
+#include <cmath>
+#include "cache.cuh"
+
+using namespace l1b;
+
+namespace {
+
+int check(const l1attn_cache *c, int rows, int dtype, bool tokens, CacheArgs *out)
+{
+	if (!c || rows < 0 || c->n_pages < 0 || c->n_kv_heads < 1 || c->width < 1 || c->v_width < 1)
+		return L1ATTN_ERR_ARG;
+	if (dtype != L1ATTN_F32 && dtype != L1ATTN_F16 && dtype != L1ATTN_BF16)
+		return L1ATTN_ERR_ARG;
+	if (c->page < 16 || c->page > 256 || (c->page & (c->page - 1)))
+		return L1ATTN_ERR_ARG;
+	if (c->width > 256 || c->v_width > 256 || c->n_kv_heads > 65535)
+		return L1ATTN_ERR_SHAPE;
+	if (!c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale)
+		return L1ATTN_ERR_ARG;
+	if (!aligned(c->k_codes, 16) || !aligned(c->v_codes, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4) || !aligned(c->status, 4))
+		return L1ATTN_ERR_ALIGN;
+	if (tokens) {
+		if (c->n_seqs < 0 || c->max_pages < 0)
+			return L1ATTN_ERR_ARG;
+		if ((long long)c->max_pages * c->page > 0x7fffffffll)
+			return L1ATTN_ERR_SHAPE;
+		if (rows == 0 || c->n_seqs == 0)
+			return 1; // nothing to do
+		if (!c->table || !c->start || !c->cu)
+			return L1ATTN_ERR_ARG;
+		if (!aligned(c->table, 4) || !aligned(c->start, 4) || !aligned(c->cu, 4))
+			return L1ATTN_ERR_ALIGN;
+	}
+	*out = {c->k_codes, c->v_codes, c->k_scale, c->v_scale, c->n_pages, c->page, c->n_kv_heads, c->width, c->v_width,
+		c->table, c->start, c->cu, c->n_seqs, c->max_pages, rows, c->status};
+	return L1ATTN_OK;
+}
+
+// Splits of the keys: enough CTAs for the GPU, at least 256 keys each.
+void plan(const CacheArgs &c, int rows, int heads, int max_len, int *splits, int *split_keys)
+{
+	const long long tiles = (long long)rows * (heads / c.kv_heads) / 16 + c.n_seqs, len = max_len < 1 ? 1 : max_len;
+	long long want = (1184 + tiles * c.kv_heads - 1) / (tiles * c.kv_heads), most = (len + 255) / 256;
+	want = want < most ? want : most;
+	*split_keys = int(((len + want - 1) / want + 63) / 64 * 64);
+	*splits = int((len + *split_keys - 1) / *split_keys);
+}
+
+} // namespace
+
+extern "C" int l1attn_cache_append(const l1attn_cache *cache, const void *k, const void *v, const int64_t *strides, int rows, int dtype, void *stream)
+{
+	CacheArgs c;
+	if (int rc = check(cache, rows, dtype, true, &c))
+		return rc > 0 ? L1ATTN_OK : rc;
+	if (!k || !v || !strides)
+		return L1ATTN_ERR_ARG;
+	const size_t es = dtype == L1ATTN_F32 ? 4 : 2;
+	if (!aligned(k, es) || !aligned(v, es))
+		return L1ATTN_ERR_ALIGN;
+	long long st[4];
+	for (int i = 0; i < 4; i++)
+		if ((st[i] = strides[i]) < 0)
+			return L1ATTN_ERR_ARG;
+	return append_launch(c, k, v, st, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int l1attn_cache_gather(const l1attn_cache *cache, void *k, void *v, int rows, int dtype, void *stream)
+{
+	CacheArgs c;
+	if (int rc = check(cache, rows, dtype, true, &c))
+		return rc > 0 ? L1ATTN_OK : rc;
+	if (!k || !v)
+		return L1ATTN_ERR_ARG;
+	const size_t es = dtype == L1ATTN_F32 ? 4 : 2;
+	if (!aligned(k, es) || !aligned(v, es))
+		return L1ATTN_ERR_ALIGN;
+	return gather_launch(c, k, v, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int l1attn_cache_copy_pages(const l1attn_cache *cache, int layers, const int32_t *src, const int32_t *dst, int n, void *stream)
+{
+	CacheArgs c;
+	if (int rc = check(cache, 0, L1ATTN_F32, false, &c))
+		return rc;
+	if (layers < 0 || n < 0)
+		return L1ATTN_ERR_ARG;
+	if (layers == 0 || n == 0)
+		return L1ATTN_OK;
+	if (!src || !dst)
+		return L1ATTN_ERR_ARG;
+	if (!aligned(src, 4) || !aligned(dst, 4))
+		return L1ATTN_ERR_ALIGN;
+	return copy_pages_launch(c, layers, src, dst, n, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t l1attn_cache_attend_bytes(const l1attn_cache *cache, int rows, int n_heads, int max_len, int dtype)
+{
+	CacheArgs c;
+	if (check(cache, rows, dtype, true, &c) || n_heads < 1 || n_heads % c.kv_heads)
+		return 0;
+	int splits, keys;
+	plan(c, rows, n_heads, max_len, &splits, &keys);
+	return splits > 1 ? size_t(splits) * rows * n_heads * (c.v_width + 2) * sizeof(float) : 0;
+}
+
+extern "C" int l1attn_cache_attend(const l1attn_cache *cache, const void *q, const int64_t *strides, void *vo, void *work, int rows, int n_heads, int max_len,
+				   const l1attn_mask *mask, int dtype, void *stream)
+{
+	AttendArgs a;
+	const int rc = check(cache, rows, dtype, true, &a.c);
+	if (rc < 0)
+		return rc;
+	if (!mask || !strides || n_heads < 1 || n_heads % cache->n_kv_heads || mask->mode < 0 || mask->mode > 2 || mask->window < 0 || !(mask->softcap >= 0.f) ||
+	    std::isinf(mask->softcap) || !mask->causal || mask->doc || mask->prefix || strides[0] < 0 || strides[1] < 0)
+		return L1ATTN_ERR_ARG;
+	if (rc > 0)
+		return L1ATTN_OK;
+	if (!q || !vo)
+		return L1ATTN_ERR_ARG;
+	const size_t es = dtype == L1ATTN_F32 ? 4 : 2;
+	if (!aligned(q, es) || !aligned(vo, es) || !aligned(work, 16) || !aligned(mask->slopes, 4))
+		return L1ATTN_ERR_ALIGN;
+	a.q = q;
+	a.vo = vo;
+	a.q_row = strides[0];
+	a.q_head = strides[1];
+	a.heads = n_heads;
+	a.group = n_heads / a.c.kv_heads;
+	a.window = mask->window;
+	a.mode = mask->mode;
+	a.cap = mask->softcap;
+	a.scale = float(1.0 / std::sqrt(double(a.c.width)));
+	a.slopes = mask->slopes;
+	plan(a.c, rows, n_heads, max_len, &a.splits, &a.split_keys);
+	if (a.splits > 1 && !work)
+		return L1ATTN_ERR_ARG;
+	a.part = a.splits > 1 ? static_cast<float *>(work) : nullptr;
+	const cudaStream_t st = static_cast<cudaStream_t>(stream);
+	if (const int e = attend_simple_launch(a, dtype, st))
+		return e;
+	return a.splits > 1 ? attend_merge_launch(a, dtype, st) : L1ATTN_OK;
+}
+
+extern "C" int l1attn_test_cache_unit(const l1attn_cache *cache, int rows, long long unit, int num, int den, int extra, int slot, int32_t *out)
+{
+	CacheArgs c;
+	if (int rc = check(cache, rows, L1ATTN_F32, true, &c))
+		return rc;
+	const int seq = cache_find(c, unit, num, den, extra);
+	const SeqView v = cache_seq(c, seq);
+	const long long mine = unit - cache_first_unit(c, seq, num, den, extra);
+	const int32_t got[] = {seq, v.row, v.count, v.start, int32_t(mine), slot >= 0 && slot < c.max_pages ? cache_page(c, seq, slot) : -2};
+	for (int i = 0; i < 6; i++)
+		out[i] = got[i];
+	return L1ATTN_OK;
+}

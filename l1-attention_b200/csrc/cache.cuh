@@ -1,0 +1,124 @@
+// A paged cache of keys and values in 8 bits (see l1attn_cache in l1attn_b200.h), as the kernels see it.
+//
+// Pages, starts and row offsets come from device memory that nobody has checked: a page id, a position or an offset out of range sets
+// the status word and what it names is left out, never dereferenced.
+#pragma once
+#include "mask.cuh"
+
+namespace l1b {
+
+struct CacheArgs {
+	int8_t *k_codes, *v_codes;
+	float *k_scale, *v_scale;
+	int n_pages, page, kv_heads, width, v_width;
+	const int32_t *table, *start, *cu;
+	int n_seqs, max_pages, rows; // rows: of the token tensors
+	int *status;
+};
+
+#define L1B_BOTH __host__ __device__ __forceinline__
+
+L1B_BOTH void cache_fault(const CacheArgs &c)
+{
+	if (c.status)
+		*reinterpret_cast<volatile int *>(c.status) = L1ATTN_ERR_INDEX;
+}
+
+// One sequence's part of a call: rows [row, row + count) of the token tensors are its positions [start, start + count).
+struct SeqView {
+	int row, count, start;
+};
+
+L1B_BOTH int cache_row(const CacheArgs &c, int seq)
+{
+	const int r = c.cu[seq];
+	return r < 0 ? 0 : r > c.rows ? c.rows : r;
+}
+
+L1B_BOTH SeqView cache_seq(const CacheArgs &c, int seq)
+{
+	const int a = c.cu[seq], b = c.cu[seq + 1], s = c.start[seq];
+	SeqView v = {cache_row(c, seq), 0, s};
+	if (a < 0 || b < a || b > c.rows || s < 0) {
+		cache_fault(c);
+		v.start = 0;
+		return v;
+	}
+	v.count = b - a;
+	const long long room = (long long)c.max_pages * c.page - s;
+	if (v.count > room) {
+		cache_fault(c);
+		v.count = room > 0 ? int(room) : 0;
+	}
+	return v;
+}
+
+// page that holds position pos of a sequence (pos / page < max_pages), or -1
+L1B_BOTH int cache_page(const CacheArgs &c, int seq, int slot)
+{
+	const int id = c.table[(long long)seq * c.max_pages + slot];
+	if (id < 0 || id >= c.n_pages) {
+		cache_fault(c);
+		return -1;
+	}
+	return id;
+}
+
+// Work units of a call lie behind one another: sequence i's begin at cu[i] * num / den + i * extra, which leaves room for at least
+// ceil(count * num / den) + extra - 1 of them.  The sequence that unit u belongs to (its own units are u - first; there may be fewer).
+L1B_BOTH long long cache_first_unit(const CacheArgs &c, int seq, int num, int den, int extra)
+{
+	return (long long)cache_row(c, seq) * num / den + (long long)seq * extra;
+}
+L1B_BOTH int cache_find(const CacheArgs &c, long long u, int num, int den, int extra)
+{
+	int lo = 0, hi = c.n_seqs - 1;
+	while (lo < hi) {
+		const int mid = (lo + hi + 1) / 2;
+		if (cache_first_unit(c, mid, num, den, extra) <= u)
+			lo = mid;
+		else
+			hi = mid - 1;
+	}
+	return lo;
+}
+
+// the sequence whose rows [cu[i], cu[i + 1]) hold `row`, if any does: the last one that begins at or before it
+L1B_BOTH int cache_find_row(const CacheArgs &c, long long row) { return cache_find(c, row, 1, 1, 0); }
+
+struct AttendArgs {
+	CacheArgs c;
+	const void *q;
+	void *vo;
+	long long q_row, q_head; // element strides of q
+	int heads, group;        // group: query heads that share a head of keys and values
+	int window, mode;
+	float cap, scale;
+	const float *slopes;
+	float *part; // [splits][rows][heads][v_width + 2], or null: one split
+	int splits, split_keys;
+};
+
+// joins the splits' running maxima, sums and accumulated values (a part: m, l, values)
+int attend_merge_launch(const AttendArgs &a, int dtype, cudaStream_t st);
+int append_launch(const CacheArgs &c, const void *k, const void *v, const long long *strides, int dtype, cudaStream_t st);
+int gather_launch(const CacheArgs &c, void *k, void *v, int dtype, cudaStream_t st);
+int copy_pages_launch(const CacheArgs &c, int layers, const int32_t *src, const int32_t *dst, int n, cudaStream_t st);
+int attend_simple_launch(const AttendArgs &a, int dtype, cudaStream_t st);
+
+// (m, l) of a row that has seen all its keys -> factor of its values; a row without weights gets 0.  The +1 form has one more key of
+// score 0, the exp form no normaliser.
+__device__ __forceinline__ float finish_softmax(int mode, float m, float l)
+{
+	if (mode == L1ATTN_SV_EXP)
+		return l == 0.f ? 0.f : expf(m);
+	if (mode == L1ATTN_SV_SOFTMAX_PLUS_ONE) {
+		if (l == 0.f)
+			return 0.f;
+		const float top = fmaxf(m, 0.f);
+		return expf(m - top) / (l * expf(m - top) + expf(-top));
+	}
+	return l == 0.f ? 0.f : 1.f / l;
+}
+
+} // namespace l1b

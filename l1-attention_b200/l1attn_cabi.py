@@ -40,6 +40,12 @@ SIGNATURES = {
     "l1attn_masked_work_bytes": (_sz, [_i] * 4),
     "l1attn_masked_fwd": (_i, [_vp] * 7 + [_i] * 6 + [_vp, _i, _vp]),
     "l1attn_masked_bwd": (_i, [_vp] * 11 + [_i] * 6 + [_vp, _i, _vp]),
+    "l1attn_cache_append": (_i, [_vp] * 4 + [_i] * 2 + [_vp]),
+    "l1attn_cache_gather": (_i, [_vp] * 3 + [_i] * 2 + [_vp]),
+    "l1attn_cache_copy_pages": (_i, [_vp, _i, _vp, _vp, _i, _vp]),
+    "l1attn_cache_attend_bytes": (_sz, [_vp] + [_i] * 4),
+    "l1attn_cache_attend": (_i, [_vp] * 5 + [_i] * 3 + [_vp, _i, _vp]),
+    "l1attn_test_cache_unit": (_i, [_vp, _i, _ll, _i, _i, _i, _i, _vp]),
     "l1attn_sparse_index_bytes": (_sz, [_i] * 3),
     "l1attn_sparse_build_index": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
     "l1attn_sparse_fwd": (_i, [_vp] * 7 + [_i] * 10 + [_vp]),
@@ -337,6 +343,42 @@ def masked_bwd(q, k, v, vo, dvo, lse, mask):
     _check(lib().l1attn_masked_bwd(_dp(q), _dp(k), _dp(v), _strides(q, k, v), _dp(vo), _dp(dvo), _dp(lse), _dp(dq), _dp(dk), _dp(dv), _dp(work), bs, n, h,
                                    hk, w, wv, _c.byref(mask), _tdt(q, allow16=True), _stream()), "l1attn_masked_bwd")
     return dq, dk, dv
+
+
+class Cache(ctypes.Structure):
+    """l1attn_cache; keeps the tensors whose addresses it holds."""
+    _fields_ = ([(x, _vp) for x in ("k_codes", "v_codes", "k_scale", "v_scale")] + [(x, _i) for x in ("n_pages", "page", "n_kv_heads", "width", "v_width")]
+                + [(x, _vp) for x in ("table", "start", "cu")] + [("n_seqs", _i), ("max_pages", _i), ("status", _vp)])
+
+    def __init__(self, k_codes, v_codes, k_scale, v_scale, table=None, start=None, cu=None, status=None):
+        n_pages, hk, page, w = k_codes.shape[-4:]
+        n_seqs, max_pages = (0, 0) if table is None else table.shape
+        super().__init__(_dp(k_codes), _dp(v_codes), _dp(k_scale), _dp(v_scale), n_pages, page, hk, w, v_codes.shape[-1], _dp(table), _dp(start), _dp(cu),
+                         n_seqs, max_pages, _dp(status))
+        self.tensors = (k_codes, v_codes, k_scale, v_scale, table, start, cu, status)
+
+
+def cache_append(cache, k, v):
+    st = (_c.c_int64 * 4)(*k.stride()[:2], *v.stride()[:2])
+    _check(lib().l1attn_cache_append(_c.byref(cache), _dp(k), _dp(v), st, k.shape[0], _tdt(k, allow16=True), _stream()), "l1attn_cache_append")
+
+
+def cache_gather(cache, k, v):
+    _check(lib().l1attn_cache_gather(_c.byref(cache), _dp(k), _dp(v), k.shape[0], _tdt(k, allow16=True), _stream()), "l1attn_cache_gather")
+
+
+def cache_copy_pages(cache, layers, src, dst):
+    _check(lib().l1attn_cache_copy_pages(_c.byref(cache), layers, _dp(src), _dp(dst), src.shape[0], _stream()), "l1attn_cache_copy_pages")
+
+
+def cache_attend(cache, q, mask, max_len, vo):
+    import torch
+    rows, h, _ = q.shape
+    dt = _tdt(q, allow16=True)
+    nb = lib().l1attn_cache_attend_bytes(_c.byref(cache), rows, h, max_len, dt)
+    work = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+    st = (_c.c_int64 * 2)(*q.stride()[:2])
+    _check(lib().l1attn_cache_attend(_c.byref(cache), _dp(q), st, _dp(vo), _dp(work), rows, h, max_len, _c.byref(mask), dt, _stream()), "l1attn_cache_attend")
 
 
 def dense_bwd(d_attn, q, k, out=None, scratch="auto"):
