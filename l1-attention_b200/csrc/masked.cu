@@ -135,7 +135,7 @@ extern "C" int l1attn_masked_fwd(const void *q, const void *k, const void *v, co
 	const cudaStream_t st = static_cast<cudaStream_t>(stream);
 	if ((rc = launch_ranges(a, work, st)))
 		return rc;
-	return masked_simple_fwd_launch(a, vo, lse, dtype, st);
+	return masked_mma_fits(a, dtype) ? masked_mma_fwd_launch(a, vo, lse, dtype, st) : masked_simple_fwd_launch(a, vo, lse, dtype, st);
 }
 
 extern "C" int l1attn_masked_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *vo, const void *dvo, const float *lse, void *dq,
