@@ -115,6 +115,7 @@ __device__ __forceinline__ float finish_row(int mode, float m, float l, float *l
 // 16-bit types, widths up to 128: distances and products on the tensor cores
 bool masked_mma_fits(const MaskedArgs &a, int dtype);
 int masked_mma_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st);
+int masked_mma_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, int dtype, cudaStream_t st);
 int masked_simple_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st);
 int masked_simple_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, int dtype,
 			     cudaStream_t st);

@@ -165,5 +165,7 @@ extern "C" int l1attn_masked_bwd(const void *q, const void *k, const void *v, co
 	else
 		launch_delta<__nv_bfloat16>(a, dvo, vo, delta, rows, st);
 	L1B_LAUNCH_CHECK();
+	if (masked_mma_fits(a, dtype))
+		return masked_mma_bwd_launch(a, dvo, lse, delta, dq, dk, dv, dtype, st);
 	return masked_simple_bwd_launch(a, dvo, lse, delta, dq, dk, dv, dtype, st);
 }

@@ -13,7 +13,7 @@ namespace l1b {
 
 namespace {
 
-constexpr int MB = 1, WARPS = 4, ROWS = 16 * MB * WARPS, KEYS = 64, THREADS = 32 * WARPS; // MB: blocks of 16 rows a warp
+constexpr int MB = 1, WARPS = 4, ROWS = 16 * MB * WARPS, KEYS = 64, STREAM = 32, THREADS = 32 * WARPS; // MB: blocks of 16 rows a warp
 constexpr float LOG2E = 1.4426950408889634f, LAG = 8.f;
 
 // One query row, by the definition: a warp, 32 keys at a time.  Rare, so simple.
@@ -375,6 +375,434 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 	}
 }
 
+// One row of dq (dk and dv), by the definition: a warp, 32 rows of the other side at a time.  Rare, so simple.
+template <typename T, bool OWN_KEYS>
+__device__ __noinline__ void exact_gradient_row(const MaskedArgs &a, const MaskView &mask, int b, int own, int o, const T *dvo, const float *lse, const float *delta, T *dx, T *dv)
+{
+	const int lane = threadIdx.x % 32, group = a.heads / a.kv_heads;
+	const Strided go = {dvo, (long long)a.n * a.heads * a.v_width, (long long)a.heads * a.v_width, a.v_width};
+	float acc[4] = {0.f, 0.f, 0.f, 0.f}, accv[4] = {0.f, 0.f, 0.f, 0.f};
+	for (int i = 0; i < (OWN_KEYS ? group : 1); i++) {
+		const int head = OWN_KEYS ? own * group + i : own, kv = OWN_KEYS ? own : own / group;
+		auto row_of = [&](const Strided &x, int h, int r) { return static_cast<const T *>(x.p) + b * x.batch + h * x.head + r * x.tok; };
+		for (int r0 = 0; r0 < a.n; r0 += 32) {
+			const int r = r0 + lane, t = OWN_KEYS ? r : o, s = OWN_KEYS ? o : r;
+			const bool seen = r < a.n && mask.sees(t, s, mask.doc ? mask.doc[t] : 0, mask.doc ? mask.doc[s] : 0);
+			if (!__any_sync(0xffffffffu, seen))
+				continue;
+			float p = 0.f, e = 0.f;
+			if (seen) {
+				const T *q = row_of(a.q, head, t), *k = row_of(a.k, kv, s), *v = row_of(a.v, kv, s), *g = row_of(go, head, t);
+				float x = 0.f, dp = 0.f, slant = 1.f;
+				for (int w = 0; w < a.width; w++)
+					x += fabsf(to_float(q[w]) - to_float(k[w]));
+				for (int w = 0; w < a.v_width; w++)
+					dp = fmaf(to_float(v[w]), to_float(g[w]), dp);
+				x *= -a.scale;
+				if (a.cap > 0.f) {
+					const float th = tanhf(x / a.cap);
+					slant = 1.f - th * th;
+					x = a.cap * th;
+				}
+				if (a.slopes)
+					x -= a.slopes[head] * fabsf(float(t - s));
+				const long long row = ((long long)b * a.n + t) * a.heads + head;
+				p = weight_of(x, lse[row]);
+				e = p == 0.f ? 0.f : -a.scale * slant * p * (dp - delta[row]);
+			}
+			for (int l = 0; l < 32; l++) {
+				const float pl = __shfl_sync(0xffffffffu, p, l), el = __shfl_sync(0xffffffffu, e, l);
+				if (pl == 0.f)
+					continue;
+				const T *mine = OWN_KEYS ? row_of(a.k, own, o) : row_of(a.q, own, o), *other = OWN_KEYS ? row_of(a.q, head, r0 + l) : row_of(a.k, kv, r0 + l);
+#pragma unroll
+				for (int c = 0; c < 4; c++) {
+					const int w = lane + 32 * c;
+					if (w < a.width)
+						acc[c] += sign_apply(to_float(mine[w]) - to_float(other[w]), el);
+					if (OWN_KEYS && w < a.v_width)
+						accv[c] = fmaf(pl, to_float(row_of(go, head, r0 + l)[w]), accv[c]);
+				}
+			}
+		}
+	}
+	const long long row = ((long long)b * a.n + o) * (OWN_KEYS ? a.kv_heads : a.heads) + own;
+#pragma unroll
+	for (int c = 0; c < 4; c++) {
+		const int w = lane + 32 * c;
+		if (w < a.width)
+			dx[row * a.width + w] = from_float<T>(acc[c]);
+		if (OWN_KEYS && w < a.v_width)
+			dv[row * a.v_width + w] = from_float<T>(accv[c]);
+	}
+}
+
+// Backward: a CTA owns 64 rows -- queries of a head (dq), or keys of a key-value head (dk, dv, over the query heads that share them, in order) -- and
+// streams the other side 32 rows at a time.  Both recompute the weights, 16 x 16 at a time:
+//   scores            rows own, columns streamed, as in the forward
+//   dP                own values (or dvo) times streamed dvo (values)
+//   e = -scale p (dP - delta) slant, the gradient of the distance; rounded to float16 relative to its row's largest so far (a power of two that follows)
+//   gradient          sum over the streamed rows of sign(own - streamed) e: for each own row a product with A = the signs [w][streamed], exact, two
+//                     instructions for two, and B = e in the column of that row: 16 own rows fill two 16 x 8 tiles per 16 columns
+//   dv                p^T dvo, weights rounded to the type (float16: times 2^12, so that small ones keep their bits)
+// No atomics, and the same sums in the same order every time.
+template <typename T, bool OWN_KEYS, int W, int V>
+__global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a, const T *dvo, const float *lse, const float *delta, T *dx, T *dv, int tiles, int vec)
+{
+	extern __shared__ uint4 smem16[];
+	__shared__ float sums[STREAM], stat_lse[STREAM], stat_delta[STREAM];
+	using H = Half2<T>;
+	constexpr int KP = W == 3 ? 16 : 4 * W, VP = 2 * V, WB = 2 * W; // 16-byte pieces of a row; 16-column blocks
+	constexpr uint32_t OWN_Y = ROWS * 64 * W * 2, STAGES = OWN_Y + ROWS * VP * 16, STAGE = STREAM * (KP + VP) * 16;
+	unsigned char *const smem = reinterpret_cast<unsigned char *>(smem16);
+	const uint32_t base = shared_address(smem16);
+	const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4, group = a.heads / a.kv_heads;
+	const int own_heads = OWN_KEYS ? a.kv_heads : a.heads;
+	const int bh = blockIdx.x % (a.bs * own_heads), rank = blockIdx.x / (a.bs * own_heads);
+	const int tile = OWN_KEYS ? rank : tiles - 1 - rank; // what a causal mask leaves most work first
+	const int own = bh % own_heads, b = bh / own_heads;
+	const MaskView mask(a, b);
+	const int o0 = tile * ROWS, o1 = min(a.n, o0 + ROWS), oa = o0 + 16 * warp + g; // this lane's rows: oa, oa + 8
+	const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
+	const Strided go = {dvo, (long long)a.n * a.heads * a.v_width, (long long)a.heads * a.v_width, a.v_width};
+
+	// own rows: in registers for the scores, every value twice in a word for the signs ([row][g][column block][w = g, g + 8]); own values stay in shared memory
+	const int32_t *own_doc = mask.doc && mask.ranges[o0 / DOC_TILE].others ? mask.doc : nullptr;
+	load_tile16<T, false, 4 * W, ROWS, THREADS>(base + STAGES, OWN_KEYS ? a.k : a.q, b, own, o0, a.n, a.width, own_doc, vec & (OWN_KEYS ? 2 : 1), tid);
+	load_tile16<T, true, VP, ROWS, THREADS>(base + OWN_Y, OWN_KEYS ? a.v : go, b, own, o0, a.n, a.v_width, own_doc, vec & (OWN_KEYS ? 4 : 8), tid);
+	cp_async_commit();
+	cp_async_wait<0>();
+	__syncthreads();
+	uint32_t x_own[WB][4];
+	float own_sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+	for (int u = 0; u < W; u++) {
+		const uint4 x = load_shared16(smem + STAGES, tile_offset<false>(4 * W, 16 * warp + g, 4 * u + j)),
+			    y = load_shared16(smem + STAGES, tile_offset<false>(4 * W, 16 * warp + g + 8, 4 * u + j));
+		x_own[2 * u][0] = x.x, x_own[2 * u][1] = y.x, x_own[2 * u][2] = x.y, x_own[2 * u][3] = y.y;
+		x_own[2 * u + 1][0] = x.z, x_own[2 * u + 1][1] = y.z, x_own[2 * u + 1][2] = x.w, x_own[2 * u + 1][3] = y.w;
+	}
+#pragma unroll
+	for (int u = 0; u < WB; u++)
+		H::mma(own_sum, x_own[u][0], x_own[u][1], x_own[u][2], x_own[u][3], H::ONES, H::ONES);
+	for (int i = tid; i < ROWS * 32 * W; i += THREADS) {
+		const int r = i / (32 * W), w = i % (32 * W);
+		const uint32_t bits = reinterpret_cast<const uint16_t *>(smem + STAGES)[r * 32 * W + w];
+		reinterpret_cast<uint32_t *>(smem)[(r * 8 + w % 8) * WB * 2 + w / 16 * 2 + w / 8 % 2] = bits | bits << 16;
+	}
+
+	float acc[WB][2][4], accv[OWN_KEYS ? 2 * V : 1][4]; // [column block][own rows 0-7, 8-15]: rows of the product are columns w, its columns own rows
+#pragma unroll
+	for (int i = 0; i < WB * 8; i++)
+		acc[i / 8][i / 4 % 2][i % 4] = 0.f;
+#pragma unroll
+	for (int i = 0; i < (OWN_KEYS ? 2 * V : 1) * 4; i++)
+		accv[i / 4][i % 4] = 0.f;
+	float unit[2] = {1.f, 1.f}, limit[2] = {0.f, 0.f}; // per row: a power of two times e is rounded to float16; e may come this far
+	const float p_unit = OWN_KEYS && sizeof(T) == 2 && H::ONES == Half2<__half>::ONES && a.mode != L1ATTN_SV_EXP ? 4096.f : 1.f;
+
+	// tiles of the other side
+	const int first_tile = [&] {
+		if (OWN_KEYS)
+			return mask.causal && o0 >= mask.prefix ? o0 / STREAM : 0;
+		return 0;
+	}();
+	const int prefix_tiles = OWN_KEYS ? 0 : (min(mask.prefix, a.n) + STREAM - 1) / STREAM;
+	const int lo = !OWN_KEYS && mask.window ? max(o0 - mask.window + 1, 0) / STREAM : 0;
+	const int all_tiles = (a.n + STREAM - 1) / STREAM;
+	const int end = OWN_KEYS ? (mask.causal && mask.window && o0 >= mask.prefix ? int(min((long long)all_tiles, ((long long)o1 + mask.window + STREAM - 1) / STREAM)) : all_tiles) :
+				   max(mask.causal ? (o1 + STREAM - 1) / STREAM : all_tiles, prefix_tiles);
+	const int heads_here = OWN_KEYS ? group : 1;
+	auto next = [&](int it) { // it: tile + head of the group * all_tiles
+		for (;; it++) {
+			int i = it % all_tiles, h = it / all_tiles;
+			if (h >= heads_here)
+				return heads_here * all_tiles;
+			if (i < first_tile)
+				it += first_tile - i, i = first_tile;
+			if (i >= prefix_tiles && i < lo)
+				it += lo - i, i = lo;
+			if (i >= end) {
+				it += all_tiles - i - 1;
+				continue;
+			}
+			const int r0 = i * STREAM, r1 = min(a.n, r0 + STREAM);
+			if (OWN_KEYS ? mask.any(r0, r1, o0, o1) : mask.any(o0, o1, r0, r1))
+				return it;
+		}
+	};
+	auto fetch = [&](int it, int stage) {
+		const int i = it % all_tiles, h = it / all_tiles, head = OWN_KEYS ? own * group + h : own / group;
+		const int32_t *doc = mask.doc && mask.ranges[i * STREAM / DOC_TILE].others ? mask.doc : nullptr;
+		const uint32_t at = base + STAGES + stage * STAGE;
+		load_tile16<T, true, 4 * W, STREAM, THREADS, KP>(at, OWN_KEYS ? a.q : a.k, b, head, i * STREAM, a.n, a.width, doc, vec & (OWN_KEYS ? 1 : 2), tid);
+		load_tile16<T, true, VP, STREAM, THREADS>(at + STREAM * KP * 16, OWN_KEYS ? go : a.v, b, head, i * STREAM, a.n, a.v_width, doc, vec & (OWN_KEYS ? 8 : 4), tid);
+	};
+	// a row's log-normaliser as the exponent takes it: a row without weights gets +inf, so that its weights are zero
+	auto exponent = [&](float x) { return x == -INFINITY ? INFINITY : x * LOG2E; };
+	float row_lse[2] = {0.f, 0.f}, row_delta[2] = {0.f, 0.f};
+	if (!OWN_KEYS)
+#pragma unroll
+		for (int r = 0; r < 2; r++) {
+			const long long row = ((long long)b * a.n + oa + 8 * r) * a.heads + own;
+			row_lse[r] = oa + 8 * r < a.n ? exponent(lse[row]) : INFINITY;
+			row_delta[r] = oa + 8 * r < a.n ? delta[row] : 0.f;
+		}
+	__syncthreads(); // (the stage that own rows came through is free)
+
+	const int stop = heads_here * all_tiles;
+	int it = next(0), stage = 0;
+	if (it < stop)
+		fetch(it, 0);
+	cp_async_commit();
+	while (it < stop) {
+		const int following = next(it + 1), i_tile = it % all_tiles, head = OWN_KEYS ? own * group + it / all_tiles : own;
+		const int r0 = i_tile * STREAM, r1 = min(a.n, r0 + STREAM);
+		cp_async_wait<0>();
+		__syncthreads(); // the tile is there; everyone is done with the other stage
+		if (following < stop)
+			fetch(following, stage ^ 1);
+		cp_async_commit();
+		const unsigned char *xt = smem + STAGES + stage * STAGE;
+		const uint32_t xs = base + STAGES + stage * STAGE, ys = xs + STREAM * KP * 16;
+		for (int r = 16 * warp; r < STREAM; r += 16 * WARPS) { // sums of the streamed rows
+			float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+			for (int u = 0; u < W; u++) {
+				const uint4 x = load_shared16(xt, tile_offset<true>(KP, r + g, 4 * u + j)), y = load_shared16(xt, tile_offset<true>(KP, r + g + 8, 4 * u + j));
+				H::mma(s, x.x, y.x, x.y, y.y, H::ONES, H::ONES);
+				H::mma(s, x.z, y.z, x.w, y.w, H::ONES, H::ONES);
+			}
+			if (j == 0) {
+				sums[r + g] = s[0];
+				sums[r + g + 8] = s[2];
+			}
+		}
+		if (OWN_KEYS && tid < STREAM) {
+			const long long row = ((long long)b * a.n + r0 + tid) * a.heads + head;
+			stat_lse[tid] = r0 + tid < a.n ? exponent(lse[row]) : INFINITY;
+			stat_delta[tid] = r0 + tid < a.n ? delta[row] : 0.f;
+		}
+		__syncthreads();
+		const bool whole = r1 == r0 + STREAM && o1 == o0 + ROWS && (OWN_KEYS ? mask.all(r0, r1, o0, o1) : mask.all(o0, o1, r0, r1));
+		const float slope = a.slopes ? a.slopes[head] : 0.f;
+#pragma unroll 1
+		for (int kb = 0; kb < STREAM / 16; kb++) {
+			float x[2][4] = {}, dp[2][4] = {};
+#pragma unroll
+			for (int n = 0; n < 8; n++) {
+				const uint32_t one = g == n ? H::ONES : 0u;
+#pragma unroll
+				for (int u = 0; u < W; u++)
+#pragma unroll
+					for (int h = 0; h < 2; h++) {
+						const uint4 k = load_shared16(xt, tile_offset<true>(KP, 16 * kb + 8 * h + n, 4 * u + j));
+						H::mma(x[h], H::min(x_own[2 * u][0], k.x), H::min(x_own[2 * u][1], k.x), H::min(x_own[2 * u][2], k.y), H::min(x_own[2 * u][3], k.y), one, one);
+						H::mma(x[h], H::min(x_own[2 * u + 1][0], k.z), H::min(x_own[2 * u + 1][1], k.z), H::min(x_own[2 * u + 1][2], k.w),
+						       H::min(x_own[2 * u + 1][3], k.w), one, one);
+					}
+			}
+#pragma unroll
+			for (int vb = 0; vb < V; vb++) {
+				uint32_t y[4], z[4];
+				ldmatrix4(y, base + OWN_Y + tile_offset<true>(VP, 16 * warp + lane % 16, 2 * vb + lane / 16));
+				ldmatrix4(z, ys + tile_offset<true>(VP, 16 * kb + lane % 8 + lane / 16 * 8, 2 * vb + lane / 8 % 2));
+				H::mma(dp[0], y[0], y[1], y[2], y[3], z[0], z[1]);
+				H::mma(dp[1], y[0], y[1], y[2], y[3], z[2], z[3]);
+			}
+			// weights and gradients of the distances
+			float slant[2][4];
+			float2 lse_c[2], delta_c[2];
+#pragma unroll
+			for (int h = 0; h < 2; h++) {
+				const int c0 = 16 * kb + 8 * h + 2 * j;
+				const float2 s = *reinterpret_cast<const float2 *>(&sums[c0]);
+				if (OWN_KEYS) {
+					lse_c[h] = *reinterpret_cast<const float2 *>(&stat_lse[c0]);
+					delta_c[h] = *reinterpret_cast<const float2 *>(&stat_delta[c0]);
+				} else
+					lse_c[h] = delta_c[h] = make_float2(0.f, 0.f);
+#pragma unroll
+				for (int c = 0; c < 4; c++) {
+					x[h][c] = a.scale * (fmaf(2.f, x[h][c], -own_sum[c & 2]) - (c & 1 ? s.y : s.x));
+					slant[h][c] = -a.scale;
+				}
+			}
+			if (!whole || a.cap > 0.f || a.slopes) {
+#pragma unroll
+				for (int h = 0; h < 2; h++)
+#pragma unroll
+					for (int c = 0; c < 4; c++) {
+						const int r = r0 + 16 * kb + 8 * h + 2 * j + (c & 1), o = oa + 8 * (c / 2), t = OWN_KEYS ? r : o, s = OWN_KEYS ? o : r;
+						float y = x[h][c];
+						if (a.cap > 0.f) {
+							const float th = tanhf(y * inv_cap);
+							slant[h][c] *= 1.f - th * th;
+							y = a.cap * th;
+						}
+						if (a.slopes)
+							y -= slope * fabsf(float(t - s));
+						if (!whole && !(t < a.n && s < a.n && mask.sees(t, s, mask.doc ? mask.doc[t] : 0, mask.doc ? mask.doc[s] : 0)))
+							y = -INFINITY;
+						x[h][c] = y;
+					}
+			}
+			float e[2][4];
+			bool grew = false;
+#pragma unroll
+			for (int h = 0; h < 2; h++)
+#pragma unroll
+				for (int c = 0; c < 4; c++) {
+					const float ls = OWN_KEYS ? (c & 1 ? lse_c[h].y : lse_c[h].x) : row_lse[c / 2], de = OWN_KEYS ? (c & 1 ? delta_c[h].y : delta_c[h].x) : row_delta[c / 2];
+					const float p = exp2_fast(fmaf(x[h][c], LOG2E, -ls));
+					e[h][c] = p == 0.f ? 0.f : p * slant[h][c] * (dp[h][c] - de);
+					x[h][c] = p;
+					grew |= fabsf(e[h][c]) > limit[c / 2];
+				}
+			if (__any_sync(0xffffffffu, grew)) { // a row's largest so far lies near 2^11 in float16: 25 binades below it keep 11 bits
+				float keep[2];
+#pragma unroll
+				for (int r = 0; r < 2; r++) {
+					float most = fmaxf(fmaxf(fabsf(e[0][2 * r]), fabsf(e[0][2 * r + 1])), fmaxf(fabsf(e[1][2 * r]), fabsf(e[1][2 * r + 1])));
+					most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+					most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+					keep[r] = 1.f;
+					if (most > limit[r]) {
+						// (powers of two from 2^-126 to 2^126; what is not finite stays so in its row)
+						const int top = min(max(int(__float_as_uint(most) >> 23), 13), 242);
+						const float now = __uint_as_float(uint32_t(254 + 11 - top) << 23);
+						keep[r] = limit[r] == 0.f ? 1.f : now / unit[r];
+						unit[r] = now;
+						limit[r] = __uint_as_float(uint32_t(top + 4) << 23);
+					}
+				}
+				// the product's columns are own rows: 2 j and 2 j + 1, and the same + 8
+				const float k0 = __shfl_sync(0xffffffffu, keep[0], 8 * j), k1 = __shfl_sync(0xffffffffu, keep[0], 8 * j + 4);
+				const float k2 = __shfl_sync(0xffffffffu, keep[1], 8 * j), k3 = __shfl_sync(0xffffffffu, keep[1], 8 * j + 4);
+#pragma unroll
+				for (int wb = 0; wb < WB; wb++) {
+					acc[wb][0][0] *= k0, acc[wb][0][1] *= k1, acc[wb][0][2] *= k0, acc[wb][0][3] *= k1;
+					acc[wb][1][0] *= k2, acc[wb][1][1] *= k3, acc[wb][1][2] *= k2, acc[wb][1][3] *= k3;
+				}
+			}
+			uint32_t eb[2][2]; // [own row g, g + 8][streamed 0-7, 8-15]
+#pragma unroll
+			for (int r = 0; r < 2; r++)
+#pragma unroll
+				for (int h = 0; h < 2; h++)
+					eb[r][h] = Half2<__half>::pack(e[h][2 * r] * unit[r], e[h][2 * r + 1] * unit[r]);
+			if (OWN_KEYS) {
+				uint32_t p[4];
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					p[2 * h] = H::pack(x[h][0] * p_unit, x[h][1] * p_unit);
+					p[2 * h + 1] = H::pack(x[h][2] * p_unit, x[h][3] * p_unit);
+				}
+#pragma unroll
+				for (int vb = 0; vb < V; vb++) {
+					uint32_t y[4];
+					ldmatrix4_trans(y, ys + tile_offset<true>(VP, 16 * kb + lane % 16, 2 * vb + lane / 16));
+					H::mma(accv[(2 * vb) % (OWN_KEYS ? 2 * V : 1)], p[0], p[1], p[2], p[3], y[0], y[1]);
+					H::mma(accv[(2 * vb + 1) % (OWN_KEYS ? 2 * V : 1)], p[0], p[1], p[2], p[3], y[2], y[3]);
+				}
+			}
+			// signs and gradients
+			uint32_t xT[WB][4]; // streamed rows, [w = g, g + 8][streamed pairs]
+#pragma unroll
+			for (int wb = 0; wb < WB; wb++)
+				ldmatrix4_trans(xT[wb], xs + tile_offset<true>(KP, 16 * kb + lane % 8 + lane / 16 * 8, 2 * wb + lane / 8 % 2));
+			const uint32_t *twice = reinterpret_cast<const uint32_t *>(smem) + (16 * warp * 8 + g) * WB * 2;
+#pragma unroll 1
+			for (int r = 0; r < 8; r++, twice += 8 * WB * 2) {
+				const bool mine = g == r;
+#pragma unroll
+				for (int half = 0; half < 2; half++) {
+					const uint32_t b0 = mine ? eb[half][0] : 0u, b1 = mine ? eb[half][1] : 0u;
+#pragma unroll
+					for (int wb = 0; wb < WB; wb += 2) {
+						const uint4 w = *reinterpret_cast<const uint4 *>(twice + half * 8 * 8 * WB * 2 + 2 * wb);
+						Half2<__half>::mma(acc[wb][half], H::sign(w.x, xT[wb][0]), H::sign(w.y, xT[wb][1]), H::sign(w.x, xT[wb][2]), H::sign(w.y, xT[wb][3]), b0, b1);
+						Half2<__half>::mma(acc[wb + 1][half], H::sign(w.z, xT[wb + 1][0]), H::sign(w.w, xT[wb + 1][1]), H::sign(w.z, xT[wb + 1][2]),
+								   H::sign(w.w, xT[wb + 1][3]), b0, b1);
+					}
+				}
+			}
+		}
+		it = following;
+		stage ^= 1;
+	}
+
+	// signs were 2^-24, e times unit
+	unsigned again = 0;
+	{
+		const float u0 = 0x1p24f / unit[0], u1 = 0x1p24f / unit[1];
+		const float f[4] = {__shfl_sync(0xffffffffu, u0, 8 * j), __shfl_sync(0xffffffffu, u0, 8 * j + 4), __shfl_sync(0xffffffffu, u1, 8 * j),
+				    __shfl_sync(0xffffffffu, u1, 8 * j + 4)};
+#pragma unroll
+		for (int i = 0; i < 4; i++) { // own rows 2 j, 2 j + 1, the same + 8
+			const int in_warp = 2 * j + (i & 1) + 8 * (i / 2), o = o0 + 16 * warp + in_warp;
+			bool odd = false;
+#pragma unroll
+			for (int wb = 0; wb < WB; wb++)
+#pragma unroll
+				for (int h = 0; h < 2; h++) {
+					const int w = 16 * wb + 8 * h + g;
+					const float y = acc[wb][i / 2][2 * h + (i & 1)] * f[i];
+					odd |= !(fabsf(y) < INFINITY);
+					if (o < a.n && w < a.width)
+						dx[(((long long)b * a.n + o) * own_heads + own) * a.width + w] = from_float<T>(y);
+				}
+			again |= odd ? 1u << in_warp : 0u;
+		}
+	}
+	if (OWN_KEYS) {
+#pragma unroll
+		for (int r = 0; r < 2; r++) {
+			const int o = oa + 8 * r;
+			bool odd = false;
+#pragma unroll
+			for (int i = 0; i < 2 * V; i++)
+#pragma unroll
+				for (int c = 0; c < 2; c++) {
+					const int w = 8 * i + 2 * j + c;
+					const float y = accv[i % (OWN_KEYS ? 2 * V : 1)][2 * r + c] * (1.f / p_unit);
+					odd |= !(fabsf(y) < INFINITY);
+					if (o < a.n && w < a.v_width)
+						dv[(((long long)b * a.n + o) * own_heads + own) * a.v_width + w] = from_float<T>(y);
+				}
+			again |= odd ? 1u << (g + 8 * r) : 0u;
+		}
+	}
+	again = __reduce_or_sync(0xffffffffu, again);
+	for (int r = 0; r < 16; r++)
+		if (again >> r & 1u && o0 + 16 * warp + r < a.n)
+			exact_gradient_row<T, OWN_KEYS>(a, mask, b, own, o0 + 16 * warp + r, dvo, lse, delta, dx, dv);
+}
+
+template <typename T, bool OWN_KEYS, int W, int V>
+int bwd_one(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dx, void *dv, int vec, cudaStream_t st)
+{
+	constexpr int KP = W == 3 ? 16 : 4 * W, VP = 2 * V, bytes = ROWS * 64 * W * 2 + ROWS * VP * 16 + 2 * STREAM * (KP + VP) * 16;
+	static_assert(2 * STREAM * (KP + VP) >= ROWS * 4 * W, "own rows pass through the stages");
+	const int tiles = (a.n + ROWS - 1) / ROWS;
+	const long long grid = (long long)tiles * (OWN_KEYS ? a.kv_heads : a.heads) * a.bs;
+	if (grid > 0x7fffffffll || (long long)(a.heads / a.kv_heads) * ((a.n + STREAM - 1) / STREAM) > 0x3fffffffll)
+		return L1ATTN_ERR_SHAPE;
+	L1B_SHARED_MEMORY((masked_bwd_mma_kernel<T, OWN_KEYS, W, V>), bytes);
+	masked_bwd_mma_kernel<T, OWN_KEYS, W, V>
+	    <<<unsigned(grid), THREADS, bytes, st>>>(a, static_cast<const T *>(dvo), lse, delta, static_cast<T *>(dx), static_cast<T *>(dv), tiles, vec);
+	L1B_LAUNCH_CHECK();
+	return L1ATTN_OK;
+}
+
+template <typename T, int W, int V>
+int bwd(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, int vec, cudaStream_t st)
+{
+	if (int rc = bwd_one<T, false, W, V>(a, dvo, lse, delta, dq, nullptr, vec, st))
+		return rc;
+	return bwd_one<T, true, W, V>(a, dvo, lse, delta, dk, dv, vec, st);
+}
+
 template <typename T, int W, int V> int fwd(const MaskedArgs &a, void *vo, float *lse, int vec, cudaStream_t st)
 {
 	constexpr int bytes = 2 * KEYS * (4 * W + 2 * V) * 16;
@@ -400,6 +828,17 @@ template <typename T> int fwd_type(const MaskedArgs &a, void *vo, float *lse, cu
 	return w == 1 ? fwd<T, 1, 8>(a, vo, lse, vec, st) : w == 2 ? fwd<T, 2, 8>(a, vo, lse, vec, st) : w == 3 ? fwd<T, 3, 8>(a, vo, lse, vec, st) : fwd<T, 4, 8>(a, vo, lse, vec, st);
 }
 
+template <typename T>
+int bwd_type(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, cudaStream_t st)
+{
+	const int vec = vectors(a.q) | vectors(a.k) << 1 | vectors(a.v) << 2 | (aligned(dvo, 16) && a.v_width % 8 == 0) << 3, w = (a.width + 31) / 32;
+	if (a.v_width <= 64)
+		return w == 1 ? bwd<T, 1, 4>(a, dvo, lse, delta, dq, dk, dv, vec, st) : w == 2 ? bwd<T, 2, 4>(a, dvo, lse, delta, dq, dk, dv, vec, st) :
+		       w == 3 ? bwd<T, 3, 4>(a, dvo, lse, delta, dq, dk, dv, vec, st) : bwd<T, 4, 4>(a, dvo, lse, delta, dq, dk, dv, vec, st);
+	return w == 1 ? bwd<T, 1, 8>(a, dvo, lse, delta, dq, dk, dv, vec, st) : w == 2 ? bwd<T, 2, 8>(a, dvo, lse, delta, dq, dk, dv, vec, st) :
+	       w == 3 ? bwd<T, 3, 8>(a, dvo, lse, delta, dq, dk, dv, vec, st) : bwd<T, 4, 8>(a, dvo, lse, delta, dq, dk, dv, vec, st);
+}
+
 } // namespace
 
 bool masked_mma_fits(const MaskedArgs &a, int dtype) { return dtype != L1ATTN_F32 && a.width <= 128 && a.v_width <= 128; }
@@ -407,6 +846,12 @@ bool masked_mma_fits(const MaskedArgs &a, int dtype) { return dtype != L1ATTN_F3
 int masked_mma_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st)
 {
 	return dtype == L1ATTN_F16 ? fwd_type<__half>(a, vo, lse, st) : fwd_type<__nv_bfloat16>(a, vo, lse, st);
+}
+
+
+int masked_mma_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, int dtype, cudaStream_t st)
+{
+	return dtype == L1ATTN_F16 ? bwd_type<__half>(a, dvo, lse, delta, dq, dk, dv, st) : bwd_type<__nv_bfloat16>(a, dvo, lse, delta, dq, dk, dv, st);
 }
 
 } // namespace l1b

@@ -35,6 +35,13 @@ template <> struct Half2<__half> {
 		asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
 		return d;
 	}
+	// sign(a - b) of both halves as the smallest float16, 2^-24, with its sign, or zero: differences do not vanish, subnormal results included
+	static __device__ __forceinline__ uint32_t sign(uint32_t a, uint32_t b)
+	{
+		uint32_t d;
+		asm("min.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(sub(a, b)), "r"(0x00010001u));
+		return d;
+	}
 	static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 	{
 		asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -60,6 +67,13 @@ template <> struct Half2<__nv_bfloat16> {
 	{
 		uint32_t d;
 		asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+		return d;
+	}
+	// (the smallest bfloat16's bits, read as a float16)
+	static __device__ __forceinline__ uint32_t sign(uint32_t a, uint32_t b)
+	{
+		uint32_t d;
+		asm("min.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(sub(a, b)), "r"(0x00010001u));
 		return d;
 	}
 	static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
@@ -95,31 +109,32 @@ __device__ __forceinline__ float exp2_fast(float x)
 	return y;
 }
 
-// Where 16-byte piece c of row r lies in a tile of rows of `pieces` pieces.  SWIZZLED: for ldmatrix, eight rows at one piece in eight places.
+// Where 16-byte piece c of row r lies in a tile of rows of `pieces` pieces (4, 8 or 16 where SWIZZLED).  SWIZZLED: for ldmatrix, eight rows at one piece
+// in eight different places of the banks.
 template <bool SWIZZLED> __device__ __forceinline__ uint32_t tile_offset(int pieces, int r, int c)
 {
-	return uint32_t(r * pieces + (SWIZZLED ? (c & ~7) | ((c ^ r) & (pieces < 8 ? pieces - 1 : 7)) : c)) * 16;
+	return uint32_t(r * pieces + (SWIZZLED ? (pieces < 8 ? c ^ (r / 2 & 3) : c ^ (r & 7)) : c)) * 16;
 }
 
 // Rows [first, first + ROWS) of one head into shared memory, asynchronously where rows are 16-byte vectors (`vec`); zeros past n and past the width, and
 // for rows of no document (`doc`: the batch item's documents, or null), whose contents are nobody's business.  A tile that is whole goes by the short
 // loop: a copy and an addition a piece (the general one took a tenth of the forward).
-template <typename T, bool SWIZZLED, int PIECES, int ROWS, int THREADS>
+template <typename T, bool SWIZZLED, int PIECES, int ROWS, int THREADS, int PITCH = PIECES>
 __device__ __forceinline__ void load_tile16(uint32_t dst, const Strided &x, int b, int head, int first, int n, int width, const int32_t *doc, bool vec, int tid)
 {
 	constexpr int STEP = THREADS / PIECES; // rows a pass
 	const T *src = static_cast<const T *>(x.p) + b * x.batch + head * x.head + first * x.tok;
-	static_assert(!SWIZZLED || STEP % 8 == 0, "rows of a thread lie at one place of the swizzle");
+	
 	if (vec && first + ROWS <= n && !doc) {
 		const int r0 = tid / PIECES, c = tid % PIECES, bytes = min(max(2 * width - 16 * c, 0), 16);
 		const T *from = src + (bytes ? r0 * x.tok + 8 * c : 0);
 		const long long step = bytes ? STEP * x.tok : 0;
-		const uint32_t at = dst + tile_offset<SWIZZLED>(PIECES, r0, c);
+		const uint32_t at = dst + tile_offset<SWIZZLED>(PITCH, r0, c);
 		if (THREADS % PIECES == 0 || r0 < STEP) {
 #pragma unroll
 			for (int i = 0; i < (ROWS + STEP - 1) / STEP; i++) {
-				if (ROWS % STEP == 0 || r0 + i * STEP < ROWS)
-					copy_async16(at + i * STEP * PIECES * 16, from, bytes);
+				if (ROWS % STEP == 0 || r0 + i * STEP < ROWS) // (rows of a thread lie at one place of the swizzle where they are multiples of eight apart)
+					copy_async16(!SWIZZLED || STEP % 8 == 0 ? at + i * STEP * PITCH * 16 : dst + tile_offset<SWIZZLED>(PITCH, r0 + i * STEP, c), from, bytes);
 				from += step;
 			}
 		}
@@ -130,7 +145,7 @@ __device__ __forceinline__ void load_tile16(uint32_t dst, const Strided &x, int 
 		const int r = i / PIECES, c = i % PIECES;
 		const bool there = first + r < n && (!doc || doc[first + r] >= 0);
 		const int left = there ? min(max(2 * width - 16 * c, 0), 16) : 0;
-		const uint32_t at = dst + tile_offset<SWIZZLED>(PIECES, r, c);
+		const uint32_t at = dst + tile_offset<SWIZZLED>(PITCH, r, c);
 		const T *from = src + (left ? r * x.tok + 8 * c : 0);
 		if (vec) {
 			copy_async16(at, left ? from : static_cast<const T *>(x.p), left);
