@@ -203,9 +203,10 @@ typedef struct l1attn_mask {
  * a tensor.  vo, dvo and the gradients are contiguous.  lse: float [bs][n_tok][n_heads], the rows' log-normalisers (NULL in the forward: not
  * kept).  work: device memory of l1attn_masked_work_bytes() bytes, 256-byte aligned (the forward uses it only with documents and takes NULL
  * without); nothing in it needs to be initialised or outlives the call, and calls that share it must not overlap on the GPU.
- * Sums, weights and their normalisers are float32 in every case.  The backward is deterministic.
+ * The backward in 16 bits with widths up to 128 keeps gradients of the distances there, up to a gigabyte at once (a float per pair and query head of a
+ * batch item; none beyond 16384 tokens).  Sums, weights and their normalisers are float32 in every case.  The backward is deterministic.
  */
-size_t l1attn_masked_work_bytes(int bs, int n_tok, int n_heads, int backward);
+size_t l1attn_masked_work_bytes(int bs, int n_tok, int n_heads, int n_kv_heads, int width, int v_width, int dtype, int backward);
 int l1attn_masked_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *vo, float *lse, void *work,
 		      int bs, int n_tok, int n_heads, int n_kv_heads, int width, int v_width,
 		      const l1attn_mask *mask, int dtype, void *stream);

@@ -113,9 +113,13 @@ __device__ __forceinline__ float finish_row(int mode, float m, float l, float *l
 }
 
 // 16-bit types, widths up to 128: distances and products on the tensor cores
-bool masked_mma_fits(const MaskedArgs &a, int dtype);
+bool masked_mma_fits(int width, int v_width, int dtype);
 int masked_mma_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st);
-int masked_mma_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, int dtype, cudaStream_t st);
+// shares: [bs][n][heads][width + v_width] floats where heads are shared; e: masked_units_at_once() * masked_unit_floats() floats, or null
+long long masked_unit_floats(int n);
+long long masked_units_at_once(int bs, int n, int heads);
+int masked_mma_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, float *e, int dtype,
+			  cudaStream_t st);
 int masked_simple_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st);
 int masked_simple_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, int dtype,
 			     cudaStream_t st);

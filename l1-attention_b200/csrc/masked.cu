@@ -115,11 +115,30 @@ template <typename T> void launch_delta(const MaskedArgs &a, const void *dvo, co
 
 using namespace l1b;
 
-extern "C" size_t l1attn_masked_work_bytes(int bs, int n_tok, int n_heads, int backward)
+namespace {
+// the backward's work: document ranges | delta | query heads' shares of dk and dv | gradients of the distances
+struct BackwardWork {
+	size_t delta, shares, e, bytes;
+	bool keeps_e;
+	BackwardWork(int bs, int n, int heads, int kv_heads, int width, int v_width, int dtype)
+	{
+		const size_t rows = size_t(bs) * n * heads;
+		const bool mma = masked_mma_fits(width, v_width, dtype);
+		const long long units = mma ? masked_units_at_once(bs, n, heads) : 0;
+		delta = ranges_bytes(bs, n);
+		shares = delta + pad256(rows * sizeof(float));
+		e = shares + (mma && heads != kv_heads ? pad256(rows * (width + v_width) * sizeof(float)) : 0);
+		keeps_e = units > 0;
+		bytes = e + size_t(units) * masked_unit_floats(n) * sizeof(float);
+	}
+};
+} // namespace
+
+extern "C" size_t l1attn_masked_work_bytes(int bs, int n_tok, int n_heads, int n_kv_heads, int width, int v_width, int dtype, int backward)
 {
-	if (bs < 1 || n_tok < 1 || n_heads < 1)
+	if (bs < 1 || n_tok < 1 || n_heads < 1 || n_kv_heads < 1 || width < 1 || v_width < 1)
 		return 256;
-	return ranges_bytes(bs, n_tok) + (backward ? pad256(size_t(bs) * n_tok * n_heads * sizeof(float)) : 0);
+	return backward ? BackwardWork(bs, n_tok, n_heads, n_kv_heads, width, v_width, dtype).bytes : ranges_bytes(bs, n_tok);
 }
 
 extern "C" int l1attn_masked_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *vo, float *lse, void *work, int bs, int n_tok,
@@ -135,7 +154,7 @@ extern "C" int l1attn_masked_fwd(const void *q, const void *k, const void *v, co
 	const cudaStream_t st = static_cast<cudaStream_t>(stream);
 	if ((rc = launch_ranges(a, work, st)))
 		return rc;
-	return masked_mma_fits(a, dtype) ? masked_mma_fwd_launch(a, vo, lse, dtype, st) : masked_simple_fwd_launch(a, vo, lse, dtype, st);
+	return masked_mma_fits(width, v_width, dtype) ? masked_mma_fwd_launch(a, vo, lse, dtype, st) : masked_simple_fwd_launch(a, vo, lse, dtype, st);
 }
 
 extern "C" int l1attn_masked_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *vo, const void *dvo, const float *lse, void *dq,
@@ -155,7 +174,10 @@ extern "C" int l1attn_masked_bwd(const void *q, const void *k, const void *v, co
 	const long long rows = (long long)bs * n_tok * n_heads;
 	if (rows / 8 >= 0x7fffffffll)
 		return L1ATTN_ERR_SHAPE;
-	float *delta = reinterpret_cast<float *>(static_cast<unsigned char *>(work) + ranges_bytes(bs, n_tok));
+	const BackwardWork layout(bs, n_tok, n_heads, n_kv_heads, width, v_width, dtype);
+	unsigned char *const base = static_cast<unsigned char *>(work);
+	float *const delta = reinterpret_cast<float *>(base + layout.delta), *const shares = reinterpret_cast<float *>(base + layout.shares);
+	float *const e = layout.keeps_e ? reinterpret_cast<float *>(base + layout.e) : nullptr;
 	if ((rc = launch_ranges(a, work, st)))
 		return rc;
 	if (dtype == L1ATTN_F32)
@@ -165,7 +187,7 @@ extern "C" int l1attn_masked_bwd(const void *q, const void *k, const void *v, co
 	else
 		launch_delta<__nv_bfloat16>(a, dvo, vo, delta, rows, st);
 	L1B_LAUNCH_CHECK();
-	if (masked_mma_fits(a, dtype))
-		return masked_mma_bwd_launch(a, dvo, lse, delta, dq, dk, dv, dtype, st);
+	if (masked_mma_fits(width, v_width, dtype))
+		return masked_mma_bwd_launch(a, dvo, lse, delta, dq, dk, dv, shares, e, dtype, st);
 	return masked_simple_bwd_launch(a, dvo, lse, delta, dq, dk, dv, dtype, st);
 }

@@ -375,92 +375,252 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 	}
 }
 
-// One row of dq (dk and dv), by the definition: a warp, 32 rows of the other side at a time.  Rare, so simple.
-template <typename T, bool OWN_KEYS>
-__device__ __noinline__ void exact_gradient_row(const MaskedArgs &a, const MaskView &mask, int b, int own, int o, const T *dvo, const float *lse, const float *delta, T *dx, T *dv)
+// One row of dq, or of one query head's share of dk and dv, by the definition: a warp, 32 rows of the other side at a time.  Rare, so simple.
+template <typename T, bool OWN_KEYS, typename OUT>
+__device__ __noinline__ void exact_gradient_row(const MaskedArgs &a, const MaskView &mask, int b, int head, int o, const T *dvo, const float *lse, const float *delta, OUT *dx, OUT *dv)
 {
-	const int lane = threadIdx.x % 32, group = a.heads / a.kv_heads;
+	const int lane = threadIdx.x % 32, kv = head / (a.heads / a.kv_heads);
 	const Strided go = {dvo, (long long)a.n * a.heads * a.v_width, (long long)a.heads * a.v_width, a.v_width};
+	auto row_of = [&](const Strided &x, int h, int r) { return static_cast<const T *>(x.p) + b * x.batch + h * x.head + r * x.tok; };
 	float acc[4] = {0.f, 0.f, 0.f, 0.f}, accv[4] = {0.f, 0.f, 0.f, 0.f};
-	for (int i = 0; i < (OWN_KEYS ? group : 1); i++) {
-		const int head = OWN_KEYS ? own * group + i : own, kv = OWN_KEYS ? own : own / group;
-		auto row_of = [&](const Strided &x, int h, int r) { return static_cast<const T *>(x.p) + b * x.batch + h * x.head + r * x.tok; };
-		for (int r0 = 0; r0 < a.n; r0 += 32) {
-			const int r = r0 + lane, t = OWN_KEYS ? r : o, s = OWN_KEYS ? o : r;
-			const bool seen = r < a.n && mask.sees(t, s, mask.doc ? mask.doc[t] : 0, mask.doc ? mask.doc[s] : 0);
-			if (!__any_sync(0xffffffffu, seen))
-				continue;
-			float p = 0.f, e = 0.f;
-			if (seen) {
-				const T *q = row_of(a.q, head, t), *k = row_of(a.k, kv, s), *v = row_of(a.v, kv, s), *g = row_of(go, head, t);
-				float x = 0.f, dp = 0.f, slant = 1.f;
-				for (int w = 0; w < a.width; w++)
-					x += fabsf(to_float(q[w]) - to_float(k[w]));
-				for (int w = 0; w < a.v_width; w++)
-					dp = fmaf(to_float(v[w]), to_float(g[w]), dp);
-				x *= -a.scale;
-				if (a.cap > 0.f) {
-					const float th = tanhf(x / a.cap);
-					slant = 1.f - th * th;
-					x = a.cap * th;
-				}
-				if (a.slopes)
-					x -= a.slopes[head] * fabsf(float(t - s));
-				const long long row = ((long long)b * a.n + t) * a.heads + head;
-				p = weight_of(x, lse[row]);
-				e = p == 0.f ? 0.f : -a.scale * slant * p * (dp - delta[row]);
+	for (int r0 = 0; r0 < a.n; r0 += 32) {
+		const int r = r0 + lane, t = OWN_KEYS ? r : o, s = OWN_KEYS ? o : r;
+		const bool seen = r < a.n && mask.sees(t, s, mask.doc ? mask.doc[t] : 0, mask.doc ? mask.doc[s] : 0);
+		if (!__any_sync(0xffffffffu, seen))
+			continue;
+		float p = 0.f, e = 0.f;
+		if (seen) {
+			const T *q = row_of(a.q, head, t), *k = row_of(a.k, kv, s), *v = row_of(a.v, kv, s), *g = row_of(go, head, t);
+			float x = 0.f, dp = 0.f, slant = 1.f;
+			for (int w = 0; w < a.width; w++)
+				x += fabsf(to_float(q[w]) - to_float(k[w]));
+			for (int w = 0; w < a.v_width; w++)
+				dp = fmaf(to_float(v[w]), to_float(g[w]), dp);
+			x *= -a.scale;
+			if (a.cap > 0.f) {
+				const float th = tanhf(x / a.cap);
+				slant = 1.f - th * th;
+				x = a.cap * th;
 			}
-			for (int l = 0; l < 32; l++) {
-				const float pl = __shfl_sync(0xffffffffu, p, l), el = __shfl_sync(0xffffffffu, e, l);
-				if (pl == 0.f)
-					continue;
-				const T *mine = OWN_KEYS ? row_of(a.k, own, o) : row_of(a.q, own, o), *other = OWN_KEYS ? row_of(a.q, head, r0 + l) : row_of(a.k, kv, r0 + l);
+			if (a.slopes)
+				x -= a.slopes[head] * fabsf(float(t - s));
+			const long long row = ((long long)b * a.n + t) * a.heads + head;
+			p = weight_of(x, lse[row]);
+			e = p == 0.f ? 0.f : -a.scale * slant * p * (dp - delta[row]);
+		}
+		for (int l = 0; l < 32; l++) {
+			const float pl = __shfl_sync(0xffffffffu, p, l), el = __shfl_sync(0xffffffffu, e, l);
+			if (pl == 0.f)
+				continue;
+			const T *mine = OWN_KEYS ? row_of(a.k, kv, o) : row_of(a.q, head, o), *other = OWN_KEYS ? row_of(a.q, head, r0 + l) : row_of(a.k, kv, r0 + l);
 #pragma unroll
-				for (int c = 0; c < 4; c++) {
-					const int w = lane + 32 * c;
-					if (w < a.width)
-						acc[c] += sign_apply(to_float(mine[w]) - to_float(other[w]), el);
-					if (OWN_KEYS && w < a.v_width)
-						accv[c] = fmaf(pl, to_float(row_of(go, head, r0 + l)[w]), accv[c]);
-				}
+			for (int c = 0; c < 4; c++) {
+				const int w = lane + 32 * c;
+				if (w < a.width)
+					acc[c] += sign_apply(to_float(mine[w]) - to_float(other[w]), el);
+				if (OWN_KEYS && w < a.v_width)
+					accv[c] = fmaf(pl, to_float(row_of(go, head, r0 + l)[w]), accv[c]);
 			}
 		}
 	}
-	const long long row = ((long long)b * a.n + o) * (OWN_KEYS ? a.kv_heads : a.heads) + own;
+	const long long row = ((long long)b * a.n + o) * a.heads + head;
 #pragma unroll
 	for (int c = 0; c < 4; c++) {
 		const int w = lane + 32 * c;
 		if (w < a.width)
-			dx[row * a.width + w] = from_float<T>(acc[c]);
+			dx[row * a.width + w] = from_float<OUT>(acc[c]);
 		if (OWN_KEYS && w < a.v_width)
-			dv[row * a.v_width + w] = from_float<T>(accv[c]);
+			dv[row * a.v_width + w] = from_float<OUT>(accv[c]);
 	}
 }
 
-// Backward: a CTA owns 64 rows -- queries of a head (dq), or keys of a key-value head (dk, dv, over the query heads that share them, in order) -- and
-// streams the other side 32 rows at a time.  Both recompute the weights, 16 x 16 at a time:
+// What a backward kernel of some units -- query heads of batch items, [first, first + units) in order -- leaves beside the gradients.
+struct BackwardParts {
+	int first, units;
+	float *e;               // gradients of the distances, [unit][t][pitch s], for the queries' kernel; or null
+	long long unit_floats;
+	int pitch;
+	float *dk, *dv;         // [bs][n][heads][width]: each query head's share of shared heads' gradients; or null
+};
+
+// Own rows for the signs: every value twice in a word, as it is or as its code, [row][g][column block][w = g, g + 8] in pieces of 16 bytes that lie so that
+// the eight g of one piece are in different banks.  Returns whether codes do not hold a value.
+template <int W> __device__ __forceinline__ int own_word(int row, int g, int word) // word: column block * 2 + half
+{
+	const int piece = word / 4;
+	return (row * 8 + g) * 4 * W + (W == 4 ? piece ^ (g / 2) : W == 2 ? piece ^ (g / 4) : piece) * 4 + word % 4;
+}
+template <typename T, int W> __device__ __forceinline__ uint32_t own_table(unsigned char *table, const unsigned char *rows, int tid)
+{
+	uint32_t off = 0;
+	for (int i = tid; i < ROWS * 32 * W; i += THREADS) {
+		const int r = i / (32 * W), w = i % (32 * W);
+		const uint32_t twice = reinterpret_cast<const uint16_t *>(rows)[i] * 0x10001u;
+		reinterpret_cast<uint32_t *>(table)[own_word<W>(r, w % 8, w / 16 * 2 + w / 8 % 2)] = Half2<T>::ONES == Half2<__half>::ONES ? twice : codes_of_bf16(twice, &off);
+	}
+	return off;
+}
+
+// 1 - codes of a streamed tile, in the same places
+template <int W, int KP> __device__ __forceinline__ void encode_tile(unsigned char *to, const unsigned char *from, uint32_t *off, int tid)
+{
+#pragma unroll
+	for (int i = tid; i < STREAM * 4 * W; i += THREADS) {
+		const uint32_t at = tile_offset<true>(KP, i / (4 * W), i % (4 * W));
+		uint4 v = *reinterpret_cast<const uint4 *>(from + at);
+		v.x = __vsub2(0x10001u, codes_of_bf16(v.x, off));
+		v.y = __vsub2(0x10001u, codes_of_bf16(v.y, off));
+		v.z = __vsub2(0x10001u, codes_of_bf16(v.z, off));
+		v.w = __vsub2(0x10001u, codes_of_bf16(v.w, off));
+		*reinterpret_cast<uint4 *>(to + at) = v;
+	}
+}
+
+// acc[column block][own rows 0-7, 8-15] += signs(own - streamed) e of 16 own rows and 16 streamed ones (rows `first` of the tile at xs); the products' rows
+// are columns w, their columns own rows.  coded: both sides are codes, and signs one too large; else streamed values, and own ones of `plain` for bfloat16.
+template <typename T, int W>
+__device__ __forceinline__ void add_signed(float (&acc)[2 * W][2][4], const uint32_t (&eb)[2][2], bool coded, uint32_t xs, int first, const unsigned char *table,
+					   const uint16_t *plain, int warp, int lane)
+{
+	using H = Half2<T>;
+	constexpr int KP = W == 3 ? 16 : 4 * W, WB = 2 * W;
+	constexpr bool CODES = H::ONES == Half2<__nv_bfloat16>::ONES;
+	const int g = lane / 4;
+	uint32_t x[WB][4]; // streamed rows, [w = g, g + 8][streamed pairs]
+#pragma unroll
+	for (int wb = 0; wb < WB; wb++)
+		ldmatrix4_trans(x[wb], xs + tile_offset<true>(KP, first + lane % 8 + lane / 16 * 8, 2 * wb + lane / 8 % 2));
+	const uint32_t *twice = reinterpret_cast<const uint32_t *>(table);
+	if (coded) {
+#pragma unroll 1
+		for (int r = 0; r < 8; r++)
+#pragma unroll
+			for (int half = 0; half < 2; half++) {
+				const uint32_t b0 = g == r ? eb[half][0] : 0u, b1 = g == r ? eb[half][1] : 0u;
+#pragma unroll
+				for (int wb = 0; wb < WB; wb += 2) {
+					const uint4 w = *reinterpret_cast<const uint4 *>(twice + own_word<W>(16 * warp + r + 8 * half, g, 2 * wb));
+					Half2<__half>::mma(acc[wb][half], signs_of_codes(w.x, x[wb][0]), signs_of_codes(w.y, x[wb][1]), signs_of_codes(w.x, x[wb][2]),
+							   signs_of_codes(w.y, x[wb][3]), b0, b1);
+					Half2<__half>::mma(acc[wb + 1][half], signs_of_codes(w.z, x[wb + 1][0]), signs_of_codes(w.w, x[wb + 1][1]),
+							   signs_of_codes(w.z, x[wb + 1][2]), signs_of_codes(w.w, x[wb + 1][3]), b0, b1);
+				}
+			}
+		return;
+	}
+#pragma unroll 1
+	for (int r = 0; r < 8; r++)
+#pragma unroll
+		for (int half = 0; half < 2; half++) {
+			const uint32_t b0 = g == r ? eb[half][0] : 0u, b1 = g == r ? eb[half][1] : 0u;
+			const uint16_t *row = plain + (16 * warp + r + 8 * half) * 32 * W + g;
+#pragma unroll
+			for (int wb = 0; wb < WB; wb += 2) {
+				uint4 w;
+				if (CODES)
+					w = make_uint4(row[16 * wb] * 0x10001u, row[16 * wb + 8] * 0x10001u, row[16 * wb + 16] * 0x10001u, row[16 * wb + 24] * 0x10001u);
+				else
+					w = *reinterpret_cast<const uint4 *>(twice + own_word<W>(16 * warp + r + 8 * half, g, 2 * wb));
+				Half2<__half>::mma(acc[wb][half], H::sign(w.x, x[wb][0]), H::sign(w.y, x[wb][1]), H::sign(w.x, x[wb][2]), H::sign(w.y, x[wb][3]), b0, b1);
+				Half2<__half>::mma(acc[wb + 1][half], H::sign(w.z, x[wb + 1][0]), H::sign(w.w, x[wb + 1][1]), H::sign(w.z, x[wb + 1][2]),
+						   H::sign(w.w, x[wb + 1][3]), b0, b1);
+			}
+		}
+}
+
+// e is rounded to float16 times a power of two per own row (`unit`; rows g, g + 8 of this lane's quad), which puts the row's largest so far near 2^11: 25
+// binades below it keep 11 bits.  Called when an e is beyond a row's limit (2^15 by the present unit); what was added up follows.
+template <int W> __device__ __forceinline__ void follow_largest(const float (&e)[2][4], float (&unit)[2], float (&limit)[2], float (&e_sum)[4], float (&acc)[2 * W][2][4], int j)
+{
+	float keep[2];
+#pragma unroll
+	for (int r = 0; r < 2; r++) {
+		float most = fmaxf(fmaxf(fabsf(e[0][2 * r]), fabsf(e[0][2 * r + 1])), fmaxf(fabsf(e[1][2 * r]), fabsf(e[1][2 * r + 1])));
+		most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+		most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+		keep[r] = 1.f;
+		if (most > limit[r]) {
+			// (exponents cut so that both powers are normal; what is not finite stays so, in its row)
+			const int top = min(max(int(__float_as_uint(most) >> 23), 13), 242);
+			const float now = __uint_as_float(uint32_t(254 + 11 - top) << 23);
+			keep[r] = limit[r] == 0.f ? 1.f : now / unit[r];
+			unit[r] = now;
+			limit[r] = __uint_as_float(uint32_t(top + 4) << 23);
+		}
+	}
+	e_sum[0] *= keep[0];
+	e_sum[2] *= keep[1];
+	// the products' columns are own rows: 2 j and 2 j + 1, and the same + 8
+	const float k0 = __shfl_sync(0xffffffffu, keep[0], 8 * j), k1 = __shfl_sync(0xffffffffu, keep[0], 8 * j + 4);
+	const float k2 = __shfl_sync(0xffffffffu, keep[1], 8 * j), k3 = __shfl_sync(0xffffffffu, keep[1], 8 * j + 4);
+#pragma unroll
+	for (int wb = 0; wb < 2 * W; wb++) {
+		acc[wb][0][0] *= k0, acc[wb][0][1] *= k1, acc[wb][0][2] *= k0, acc[wb][0][3] *= k1;
+		acc[wb][1][0] *= k2, acc[wb][1][1] *= k3, acc[wb][1][2] *= k2, acc[wb][1][3] *= k3;
+	}
+}
+
+// Signs were 2^-24 (and one too large where e_sum counts them), e times unit: a warp's 16 rows of the gradient, to `part` or `dx`.  Returns the rows whose
+// values are not finite, by this lane.
+template <typename T, int W>
+__device__ __forceinline__ unsigned store_signed(const float (&acc)[2 * W][2][4], const float (&unit)[2], const float (&e_sum)[4], const MaskedArgs &a, int b, int head,
+						 int first, int lane, float *part, T *dx)
+{
+	const int g = lane / 4, j = lane % 4;
+	const float u0 = 0x1p24f / unit[0], u1 = 0x1p24f / unit[1], s0 = e_sum[0] * 0x1p-24f, s1 = e_sum[2] * 0x1p-24f;
+	unsigned again = 0;
+#pragma unroll
+	for (int i = 0; i < 4; i++) { // rows 2 j, 2 j + 1, the same + 8
+		const int in_warp = 2 * j + (i & 1) + 8 * (i / 2), o = first + in_warp, from = 8 * j + 4 * (i & 1);
+		const float f = __shfl_sync(0xffffffffu, i < 2 ? u0 : u1, from), less = __shfl_sync(0xffffffffu, i < 2 ? s0 : s1, from);
+		bool odd = false;
+#pragma unroll
+		for (int wb = 0; wb < 2 * W; wb++)
+#pragma unroll
+			for (int h = 0; h < 2; h++) {
+				const int w = 16 * wb + 8 * h + g;
+				const float y = (acc[wb][i / 2][2 * h + (i & 1)] - less) * f;
+				odd |= !(fabsf(y) < INFINITY);
+				if (o < a.n && w < a.width) {
+					const long long at = (((long long)b * a.n + o) * a.heads + head) * a.width + w;
+					if (part)
+						part[at] = y;
+					else
+						dx[at] = from_float<T>(y);
+				}
+			}
+		again |= odd ? 1u << in_warp : 0u;
+	}
+	return again;
+}
+
+// Backward: a CTA owns 64 rows of one query head -- its keys (dk, dv: its share of them, where heads are shared), or its queries (dq) -- and streams the
+// other side 32 rows at a time.  The keys' kernel leaves the gradients of the distances for the queries' (masked_dq_mma_kernel), whose own form here, with
+// the weights formed again, serves where they would take too much memory.  16 x 16 at a time:
 //   scores            rows own, columns streamed, as in the forward
 //   dP                own values (or dvo) times streamed dvo (values)
 //   e = -scale p (dP - delta) slant, the gradient of the distance; rounded to float16 relative to its row's largest so far (a power of two that follows)
-//   gradient          sum over the streamed rows of sign(own - streamed) e: for each own row a product with A = the signs [w][streamed], exact, two
-//                     instructions for two, and B = e in the column of that row: 16 own rows fill two 16 x 8 tiles per 16 columns
+//   gradient          sum over the streamed rows of sign(own - streamed) e: for each own row a product with A = the signs [w][streamed], exact, and
+//                     B = e in the column of that row: 16 own rows fill two 16 x 8 tiles per 16 columns.  Signs take two instructions for two values
+//                     (a subtraction, which mma.sync does not overlap, and a minimum), or one for bfloat16 as codes of 15 bits; a tile with values
+//                     that these do not hold takes the two
 //   dv                p^T dvo, weights rounded to the type (float16: times 2^12, so that small ones keep their bits)
 // No atomics, and the same sums in the same order every time.
 template <typename T, bool OWN_KEYS, int W, int V>
-__global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a, const T *dvo, const float *lse, const float *delta, T *dx, T *dv, int tiles, int vec)
+__global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a, const T *dvo, const float *lse, const float *delta, T *dx, T *dv, BackwardParts parts, int tiles, int vec)
 {
 	extern __shared__ uint4 smem16[];
 	__shared__ float sums[STREAM], stat_lse[STREAM], stat_delta[STREAM];
 	using H = Half2<T>;
 	constexpr int KP = W == 3 ? 16 : 4 * W, VP = 2 * V, WB = 2 * W; // 16-byte pieces of a row; 16-column blocks
-	constexpr uint32_t OWN_Y = ROWS * 64 * W * 2, STAGES = OWN_Y + ROWS * VP * 16, STAGE = STREAM * (KP + VP) * 16;
+	constexpr bool CODES = H::ONES == Half2<__nv_bfloat16>::ONES;
+	constexpr uint32_t OWN_Y = ROWS * 64 * W * 2, STAGES = OWN_Y + ROWS * VP * 16, STAGE = STREAM * (KP + VP) * 16, OWN_X = STAGES + 2 * STAGE, CODED = OWN_X + ROWS * 64 * W;
 	unsigned char *const smem = reinterpret_cast<unsigned char *>(smem16);
 	const uint32_t base = shared_address(smem16);
-	const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4, group = a.heads / a.kv_heads;
-	const int own_heads = OWN_KEYS ? a.kv_heads : a.heads;
-	const int bh = blockIdx.x % (a.bs * own_heads), rank = blockIdx.x / (a.bs * own_heads);
+	const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4;
+	const int unit_bh = blockIdx.x % parts.units, rank = blockIdx.x / parts.units, bh = parts.first + unit_bh; // (a unit: a query head of a batch item)
 	const int tile = OWN_KEYS ? rank : tiles - 1 - rank; // what a causal mask leaves most work first
-	const int own = bh % own_heads, b = bh / own_heads;
+	const int head = bh % a.heads, b = bh / a.heads, kv = head / (a.heads / a.kv_heads);
 	const MaskView mask(a, b);
 	const int o0 = tile * ROWS, o1 = min(a.n, o0 + ROWS), oa = o0 + 16 * warp + g; // this lane's rows: oa, oa + 8
 	const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
@@ -468,8 +628,9 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 
 	// own rows: in registers for the scores, every value twice in a word for the signs ([row][g][column block][w = g, g + 8]); own values stay in shared memory
 	const int32_t *own_doc = mask.doc && mask.ranges[o0 / DOC_TILE].others ? mask.doc : nullptr;
-	load_tile16<T, false, 4 * W, ROWS, THREADS>(base + STAGES, OWN_KEYS ? a.k : a.q, b, own, o0, a.n, a.width, own_doc, vec & (OWN_KEYS ? 2 : 1), tid);
-	load_tile16<T, true, VP, ROWS, THREADS>(base + OWN_Y, OWN_KEYS ? a.v : go, b, own, o0, a.n, a.v_width, own_doc, vec & (OWN_KEYS ? 4 : 8), tid);
+	constexpr uint32_t FROM = CODES ? OWN_X : STAGES; // (kept where tiles that codes do not fit may need it)
+	load_tile16<T, false, 4 * W, ROWS, THREADS>(base + FROM, OWN_KEYS ? a.k : a.q, b, OWN_KEYS ? kv : head, o0, a.n, a.width, own_doc, vec & (OWN_KEYS ? 2 : 1), tid);
+	load_tile16<T, true, VP, ROWS, THREADS>(base + OWN_Y, OWN_KEYS ? a.v : go, b, OWN_KEYS ? kv : head, o0, a.n, a.v_width, own_doc, vec & (OWN_KEYS ? 4 : 8), tid);
 	cp_async_commit();
 	cp_async_wait<0>();
 	__syncthreads();
@@ -477,19 +638,15 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 	float own_sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
 	for (int u = 0; u < W; u++) {
-		const uint4 x = load_shared16(smem + STAGES, tile_offset<false>(4 * W, 16 * warp + g, 4 * u + j)),
-			    y = load_shared16(smem + STAGES, tile_offset<false>(4 * W, 16 * warp + g + 8, 4 * u + j));
+		const uint4 x = load_shared16(smem + FROM, tile_offset<false>(4 * W, 16 * warp + g, 4 * u + j)),
+			    y = load_shared16(smem + FROM, tile_offset<false>(4 * W, 16 * warp + g + 8, 4 * u + j));
 		x_own[2 * u][0] = x.x, x_own[2 * u][1] = y.x, x_own[2 * u][2] = x.y, x_own[2 * u][3] = y.y;
 		x_own[2 * u + 1][0] = x.z, x_own[2 * u + 1][1] = y.z, x_own[2 * u + 1][2] = x.w, x_own[2 * u + 1][3] = y.w;
 	}
 #pragma unroll
 	for (int u = 0; u < WB; u++)
 		H::mma(own_sum, x_own[u][0], x_own[u][1], x_own[u][2], x_own[u][3], H::ONES, H::ONES);
-	for (int i = tid; i < ROWS * 32 * W; i += THREADS) {
-		const int r = i / (32 * W), w = i % (32 * W);
-		const uint32_t bits = reinterpret_cast<const uint16_t *>(smem + STAGES)[r * 32 * W + w];
-		reinterpret_cast<uint32_t *>(smem)[(r * 8 + w % 8) * WB * 2 + w / 16 * 2 + w / 8 % 2] = bits | bits << 16;
-	}
+	uint32_t own_off = own_table<T, W>(smem, smem + FROM, tid);
 
 	float acc[WB][2][4], accv[OWN_KEYS ? 2 * V : 1][4]; // [column block][own rows 0-7, 8-15]: rows of the product are columns w, its columns own rows
 #pragma unroll
@@ -498,6 +655,7 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 #pragma unroll
 	for (int i = 0; i < (OWN_KEYS ? 2 * V : 1) * 4; i++)
 		accv[i / 4][i % 4] = 0.f;
+	float e_sum[4] = {0.f, 0.f, 0.f, 0.f}; // CODES: of the rounded e, by own row: signs there are one too large
 	float unit[2] = {1.f, 1.f}, limit[2] = {0.f, 0.f}; // per row: a power of two times e is rounded to float16; e may come this far
 	const float p_unit = OWN_KEYS && sizeof(T) == 2 && H::ONES == Half2<__half>::ONES && a.mode != L1ATTN_SV_EXP ? 4096.f : 1.f;
 
@@ -512,31 +670,23 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 	const int all_tiles = (a.n + STREAM - 1) / STREAM;
 	const int end = OWN_KEYS ? (mask.causal && mask.window && o0 >= mask.prefix ? int(min((long long)all_tiles, ((long long)o1 + mask.window + STREAM - 1) / STREAM)) : all_tiles) :
 				   max(mask.causal ? (o1 + STREAM - 1) / STREAM : all_tiles, prefix_tiles);
-	const int heads_here = OWN_KEYS ? group : 1;
-	auto next = [&](int it) { // it: tile + head of the group * all_tiles
-		for (;; it++) {
-			int i = it % all_tiles, h = it / all_tiles;
-			if (h >= heads_here)
-				return heads_here * all_tiles;
-			if (i < first_tile)
-				it += first_tile - i, i = first_tile;
+	auto next = [&](int i) {
+		for (;; i++) {
 			if (i >= prefix_tiles && i < lo)
-				it += lo - i, i = lo;
-			if (i >= end) {
-				it += all_tiles - i - 1;
-				continue;
-			}
+				i = lo;
+			if (i >= end)
+				return end;
 			const int r0 = i * STREAM, r1 = min(a.n, r0 + STREAM);
 			if (OWN_KEYS ? mask.any(r0, r1, o0, o1) : mask.any(o0, o1, r0, r1))
-				return it;
+				return i;
 		}
 	};
-	auto fetch = [&](int it, int stage) {
-		const int i = it % all_tiles, h = it / all_tiles, head = OWN_KEYS ? own * group + h : own / group;
+	auto fetch = [&](int i, int stage) {
+		const int other = OWN_KEYS ? head : kv;
 		const int32_t *doc = mask.doc && mask.ranges[i * STREAM / DOC_TILE].others ? mask.doc : nullptr;
 		const uint32_t at = base + STAGES + stage * STAGE;
-		load_tile16<T, true, 4 * W, STREAM, THREADS, KP>(at, OWN_KEYS ? a.q : a.k, b, head, i * STREAM, a.n, a.width, doc, vec & (OWN_KEYS ? 1 : 2), tid);
-		load_tile16<T, true, VP, STREAM, THREADS>(at + STREAM * KP * 16, OWN_KEYS ? go : a.v, b, head, i * STREAM, a.n, a.v_width, doc, vec & (OWN_KEYS ? 8 : 4), tid);
+		load_tile16<T, true, 4 * W, STREAM, THREADS, KP>(at, OWN_KEYS ? a.q : a.k, b, other, i * STREAM, a.n, a.width, doc, vec & (OWN_KEYS ? 1 : 2), tid);
+		load_tile16<T, true, VP, STREAM, THREADS>(at + STREAM * KP * 16, OWN_KEYS ? go : a.v, b, other, i * STREAM, a.n, a.v_width, doc, vec & (OWN_KEYS ? 8 : 4), tid);
 	};
 	// a row's log-normaliser as the exponent takes it: a row without weights gets +inf, so that its weights are zero
 	auto exponent = [&](float x) { return x == -INFINITY ? INFINITY : x * LOG2E; };
@@ -544,23 +694,22 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 	if (!OWN_KEYS)
 #pragma unroll
 		for (int r = 0; r < 2; r++) {
-			const long long row = ((long long)b * a.n + oa + 8 * r) * a.heads + own;
+			const long long row = ((long long)b * a.n + oa + 8 * r) * a.heads + head;
 			row_lse[r] = oa + 8 * r < a.n ? exponent(lse[row]) : INFINITY;
 			row_delta[r] = oa + 8 * r < a.n ? delta[row] : 0.f;
 		}
-	__syncthreads(); // (the stage that own rows came through is free)
+	own_off = __syncthreads_or(own_off != 0); // (and the stage that own rows came through is free)
 
-	const int stop = heads_here * all_tiles;
-	int it = next(0), stage = 0;
-	if (it < stop)
+	const float slope = a.slopes ? a.slopes[head] : 0.f;
+	int it = next(first_tile), stage = 0;
+	if (it < end)
 		fetch(it, 0);
 	cp_async_commit();
-	while (it < stop) {
-		const int following = next(it + 1), i_tile = it % all_tiles, head = OWN_KEYS ? own * group + it / all_tiles : own;
-		const int r0 = i_tile * STREAM, r1 = min(a.n, r0 + STREAM);
+	while (it < end) {
+		const int following = next(it + 1), r0 = it * STREAM, r1 = min(a.n, r0 + STREAM);
 		cp_async_wait<0>();
 		__syncthreads(); // the tile is there; everyone is done with the other stage
-		if (following < stop)
+		if (following < end)
 			fetch(following, stage ^ 1);
 		cp_async_commit();
 		const unsigned char *xt = smem + STAGES + stage * STAGE;
@@ -583,9 +732,11 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 			stat_lse[tid] = r0 + tid < a.n ? exponent(lse[row]) : INFINITY;
 			stat_delta[tid] = r0 + tid < a.n ? delta[row] : 0.f;
 		}
-		__syncthreads();
+		uint32_t off = own_off;
+		if (CODES)
+			encode_tile<W, KP>(smem + CODED, xt, &off, tid);
+		off = __syncthreads_or(off != 0);
 		const bool whole = r1 == r0 + STREAM && o1 == o0 + ROWS && (OWN_KEYS ? mask.all(r0, r1, o0, o1) : mask.all(o0, o1, r0, r1));
-		const float slope = a.slopes ? a.slopes[head] : 0.f;
 #pragma unroll 1
 		for (int kb = 0; kb < STREAM / 16; kb++) {
 			float x[2][4] = {}, dp[2][4] = {};
@@ -659,38 +810,20 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 					x[h][c] = p;
 					grew |= fabsf(e[h][c]) > limit[c / 2];
 				}
-			if (__any_sync(0xffffffffu, grew)) { // a row's largest so far lies near 2^11 in float16: 25 binades below it keep 11 bits
-				float keep[2];
-#pragma unroll
-				for (int r = 0; r < 2; r++) {
-					float most = fmaxf(fmaxf(fabsf(e[0][2 * r]), fabsf(e[0][2 * r + 1])), fmaxf(fabsf(e[1][2 * r]), fabsf(e[1][2 * r + 1])));
-					most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-					most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-					keep[r] = 1.f;
-					if (most > limit[r]) {
-						// (powers of two from 2^-126 to 2^126; what is not finite stays so in its row)
-						const int top = min(max(int(__float_as_uint(most) >> 23), 13), 242);
-						const float now = __uint_as_float(uint32_t(254 + 11 - top) << 23);
-						keep[r] = limit[r] == 0.f ? 1.f : now / unit[r];
-						unit[r] = now;
-						limit[r] = __uint_as_float(uint32_t(top + 4) << 23);
-					}
-				}
-				// the product's columns are own rows: 2 j and 2 j + 1, and the same + 8
-				const float k0 = __shfl_sync(0xffffffffu, keep[0], 8 * j), k1 = __shfl_sync(0xffffffffu, keep[0], 8 * j + 4);
-				const float k2 = __shfl_sync(0xffffffffu, keep[1], 8 * j), k3 = __shfl_sync(0xffffffffu, keep[1], 8 * j + 4);
-#pragma unroll
-				for (int wb = 0; wb < WB; wb++) {
-					acc[wb][0][0] *= k0, acc[wb][0][1] *= k1, acc[wb][0][2] *= k0, acc[wb][0][3] *= k1;
-					acc[wb][1][0] *= k2, acc[wb][1][1] *= k3, acc[wb][1][2] *= k2, acc[wb][1][3] *= k3;
-				}
-			}
+			if (__any_sync(0xffffffffu, grew))
+				follow_largest<W>(e, unit, limit, e_sum, acc, j);
 			uint32_t eb[2][2]; // [own row g, g + 8][streamed 0-7, 8-15]
 #pragma unroll
-			for (int r = 0; r < 2; r++)
+			for (int i = 0; i < 4; i++)
+				eb[i / 2][i % 2] = Half2<__half>::pack(e[i % 2][i / 2 * 2] * unit[i / 2], e[i % 2][i / 2 * 2 + 1] * unit[i / 2]);
+			if (OWN_KEYS && parts.e) { // for the queries' kernel: [unit][t][s]
+				float *const to = parts.e + unit_bh * parts.unit_floats + (long long)(r0 + 16 * kb + 2 * j) * parts.pitch + oa;
 #pragma unroll
 				for (int h = 0; h < 2; h++)
-					eb[r][h] = Half2<__half>::pack(e[h][2 * r] * unit[r], e[h][2 * r + 1] * unit[r]);
+#pragma unroll
+					for (int c = 0; c < 4; c++)
+						to[(8 * h + (c & 1)) * parts.pitch + 8 * (c / 2)] = e[h][c];
+			}
 			if (OWN_KEYS) {
 				uint32_t p[4];
 #pragma unroll
@@ -706,55 +839,16 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 					H::mma(accv[(2 * vb + 1) % (OWN_KEYS ? 2 * V : 1)], p[0], p[1], p[2], p[3], y[2], y[3]);
 				}
 			}
-			// signs and gradients
-			uint32_t xT[WB][4]; // streamed rows, [w = g, g + 8][streamed pairs]
-#pragma unroll
-			for (int wb = 0; wb < WB; wb++)
-				ldmatrix4_trans(xT[wb], xs + tile_offset<true>(KP, 16 * kb + lane % 8 + lane / 16 * 8, 2 * wb + lane / 8 % 2));
-			const uint32_t *twice = reinterpret_cast<const uint32_t *>(smem) + (16 * warp * 8 + g) * WB * 2;
-#pragma unroll 1
-			for (int r = 0; r < 8; r++, twice += 8 * WB * 2) {
-				const bool mine = g == r;
-#pragma unroll
-				for (int half = 0; half < 2; half++) {
-					const uint32_t b0 = mine ? eb[half][0] : 0u, b1 = mine ? eb[half][1] : 0u;
-#pragma unroll
-					for (int wb = 0; wb < WB; wb += 2) {
-						const uint4 w = *reinterpret_cast<const uint4 *>(twice + half * 8 * 8 * WB * 2 + 2 * wb);
-						Half2<__half>::mma(acc[wb][half], H::sign(w.x, xT[wb][0]), H::sign(w.y, xT[wb][1]), H::sign(w.x, xT[wb][2]), H::sign(w.y, xT[wb][3]), b0, b1);
-						Half2<__half>::mma(acc[wb + 1][half], H::sign(w.z, xT[wb + 1][0]), H::sign(w.w, xT[wb + 1][1]), H::sign(w.z, xT[wb + 1][2]),
-								   H::sign(w.w, xT[wb + 1][3]), b0, b1);
-					}
-				}
-			}
+			const bool coded = CODES && !off;
+			if (coded) // (one product: e as A, ones as B)
+				Half2<__half>::mma(e_sum, eb[0][0], eb[1][0], eb[0][1], eb[1][1], Half2<__half>::ONES, Half2<__half>::ONES);
+			add_signed<T, W>(acc, eb, coded, coded ? base + CODED : xs, 16 * kb, smem, reinterpret_cast<const uint16_t *>(smem + OWN_X), warp, lane);
 		}
 		it = following;
 		stage ^= 1;
 	}
 
-	// signs were 2^-24, e times unit
-	unsigned again = 0;
-	{
-		const float u0 = 0x1p24f / unit[0], u1 = 0x1p24f / unit[1];
-		const float f[4] = {__shfl_sync(0xffffffffu, u0, 8 * j), __shfl_sync(0xffffffffu, u0, 8 * j + 4), __shfl_sync(0xffffffffu, u1, 8 * j),
-				    __shfl_sync(0xffffffffu, u1, 8 * j + 4)};
-#pragma unroll
-		for (int i = 0; i < 4; i++) { // own rows 2 j, 2 j + 1, the same + 8
-			const int in_warp = 2 * j + (i & 1) + 8 * (i / 2), o = o0 + 16 * warp + in_warp;
-			bool odd = false;
-#pragma unroll
-			for (int wb = 0; wb < WB; wb++)
-#pragma unroll
-				for (int h = 0; h < 2; h++) {
-					const int w = 16 * wb + 8 * h + g;
-					const float y = acc[wb][i / 2][2 * h + (i & 1)] * f[i];
-					odd |= !(fabsf(y) < INFINITY);
-					if (o < a.n && w < a.width)
-						dx[(((long long)b * a.n + o) * own_heads + own) * a.width + w] = from_float<T>(y);
-				}
-			again |= odd ? 1u << in_warp : 0u;
-		}
-	}
+	unsigned again = store_signed<T, W>(acc, unit, e_sum, a, b, head, o0 + 16 * warp, lane, OWN_KEYS ? parts.dk : nullptr, dx);
 	if (OWN_KEYS) {
 #pragma unroll
 		for (int r = 0; r < 2; r++) {
@@ -767,40 +861,176 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 					const int w = 8 * i + 2 * j + c;
 					const float y = accv[i % (OWN_KEYS ? 2 * V : 1)][2 * r + c] * (1.f / p_unit);
 					odd |= !(fabsf(y) < INFINITY);
-					if (o < a.n && w < a.v_width)
-						dv[(((long long)b * a.n + o) * own_heads + own) * a.v_width + w] = from_float<T>(y);
+					if (o < a.n && w < a.v_width) {
+						const long long at = (((long long)b * a.n + o) * a.heads + head) * a.v_width + w;
+						if (parts.dv)
+							parts.dv[at] = y;
+						else
+							dv[at] = from_float<T>(y);
+					}
 				}
 			again |= odd ? 1u << (g + 8 * r) : 0u;
 		}
 	}
 	again = __reduce_or_sync(0xffffffffu, again);
 	for (int r = 0; r < 16; r++)
-		if (again >> r & 1u && o0 + 16 * warp + r < a.n)
-			exact_gradient_row<T, OWN_KEYS>(a, mask, b, own, o0 + 16 * warp + r, dvo, lse, delta, dx, dv);
+		if (again >> r & 1u && o0 + 16 * warp + r < a.n) {
+			if (OWN_KEYS && parts.dk)
+				exact_gradient_row<T, OWN_KEYS>(a, mask, b, head, o0 + 16 * warp + r, dvo, lse, delta, parts.dk, parts.dv);
+			else
+				exact_gradient_row<T, OWN_KEYS>(a, mask, b, head, o0 + 16 * warp + r, dvo, lse, delta, dx, dv);
+		}
 }
 
-template <typename T, bool OWN_KEYS, int W, int V>
-int bwd_one(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dx, void *dv, int vec, cudaStream_t st)
+// The queries' gradients from stored gradients of the distances (parts.e, by the keys' kernel): signs alone.  64 query rows a CTA, keys in tiles of 32.
+template <typename T, int W>
+__global__ void __launch_bounds__(THREADS, 3) masked_dq_mma_kernel(MaskedArgs a, const T *dvo, const float *lse, const float *delta, T *dq, BackwardParts parts, int tiles, int vec)
 {
-	constexpr int KP = W == 3 ? 16 : 4 * W, VP = 2 * V, bytes = ROWS * 64 * W * 2 + ROWS * VP * 16 + 2 * STREAM * (KP + VP) * 16;
-	static_assert(2 * STREAM * (KP + VP) >= ROWS * 4 * W, "own rows pass through the stages");
-	const int tiles = (a.n + ROWS - 1) / ROWS;
-	const long long grid = (long long)tiles * (OWN_KEYS ? a.kv_heads : a.heads) * a.bs;
-	if (grid > 0x7fffffffll || (long long)(a.heads / a.kv_heads) * ((a.n + STREAM - 1) / STREAM) > 0x3fffffffll)
-		return L1ATTN_ERR_SHAPE;
-	L1B_SHARED_MEMORY((masked_bwd_mma_kernel<T, OWN_KEYS, W, V>), bytes);
-	masked_bwd_mma_kernel<T, OWN_KEYS, W, V>
-	    <<<unsigned(grid), THREADS, bytes, st>>>(a, static_cast<const T *>(dvo), lse, delta, static_cast<T *>(dx), static_cast<T *>(dv), tiles, vec);
-	L1B_LAUNCH_CHECK();
-	return L1ATTN_OK;
+	extern __shared__ uint4 smem16[];
+	constexpr int KP = W == 3 ? 16 : 4 * W, WB = 2 * W;
+	constexpr bool CODES = Half2<T>::ONES == Half2<__nv_bfloat16>::ONES;
+	constexpr uint32_t STAGES = ROWS * 128 * W, STAGE = STREAM * KP * 16, OWN_X = STAGES + 2 * STAGE, CODED = OWN_X + ROWS * 64 * W, FROM = CODES ? OWN_X : STAGES;
+	unsigned char *const smem = reinterpret_cast<unsigned char *>(smem16);
+	const uint32_t base = shared_address(smem16);
+	const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4;
+	const int unit_bh = blockIdx.x % parts.units, bh = parts.first + unit_bh, tile = tiles - 1 - int(blockIdx.x / parts.units);
+	const int head = bh % a.heads, b = bh / a.heads, kv = head / (a.heads / a.kv_heads);
+	const MaskView mask(a, b);
+	const int o0 = tile * ROWS, o1 = min(a.n, o0 + ROWS), oa = o0 + 16 * warp + g;
+	load_tile16<T, false, 4 * W, ROWS, THREADS>(base + FROM, a.q, b, head, o0, a.n, a.width, mask.doc && mask.ranges[o0 / DOC_TILE].others ? mask.doc : nullptr, vec & 1, tid);
+	cp_async_commit();
+	cp_async_wait<0>();
+	__syncthreads();
+	uint32_t own_off = own_table<T, W>(smem, smem + FROM, tid);
+	float acc[WB][2][4];
+#pragma unroll
+	for (int i = 0; i < WB * 8; i++)
+		acc[i / 8][i / 4 % 2][i % 4] = 0.f;
+	float e_sum[4] = {0.f, 0.f, 0.f, 0.f}, unit[2] = {1.f, 1.f}, limit[2] = {0.f, 0.f};
+	const int all_tiles = (a.n + STREAM - 1) / STREAM, prefix_tiles = (min(mask.prefix, a.n) + STREAM - 1) / STREAM;
+	const int lo = mask.window ? max(o0 - mask.window + 1, 0) / STREAM : 0, end = max(mask.causal ? (o1 + STREAM - 1) / STREAM : all_tiles, prefix_tiles);
+	auto next = [&](int i) {
+		for (;; i++) {
+			if (i >= prefix_tiles && i < lo)
+				i = lo;
+			if (i >= end || mask.any(o0, o1, i * STREAM, min(a.n, i * STREAM + STREAM)))
+				return i;
+		}
+	};
+	auto fetch = [&](int i, int stage) {
+		load_tile16<T, true, 4 * W, STREAM, THREADS, KP>(base + STAGES + stage * STAGE, a.k, b, kv, i * STREAM, a.n, a.width,
+								 mask.doc && mask.ranges[i * STREAM / DOC_TILE].others ? mask.doc : nullptr, vec & 2, tid);
+	};
+	own_off = __syncthreads_or(own_off != 0);
+	int it = next(0), stage = 0;
+	if (it < end)
+		fetch(it, 0);
+	cp_async_commit();
+	while (it < end) {
+		const int following = next(it + 1), r0 = it * STREAM;
+		// what the keys' kernel has gone over: blocks of 32 queries and 64 keys that may see each other
+		const int t32 = (o0 + 16 * warp) / 32 * 32, s64 = r0 / 64 * 64;
+		const bool there = t32 < a.n && mask.any(t32, min(a.n, t32 + 32), s64, min(a.n, s64 + 64));
+		const float *const from = parts.e + unit_bh * parts.unit_floats + (long long)oa * parts.pitch + r0 + 2 * j;
+		float2 e_all[2][4]; // [step][streamed 0-7, 8-15][own row g, g + 8]
+#pragma unroll
+		for (int i = 0; i < 8; i++)
+			e_all[i / 4][i % 4] = there ? *reinterpret_cast<const float2 *>(from + (i % 2) * 8 * (long long)parts.pitch + 16 * (i / 4) + 8 * (i / 2 % 2)) : make_float2(0.f, 0.f);
+		cp_async_wait<0>();
+		__syncthreads(); // the tile is there; everyone is done with the other stage, and with the codes
+		if (following < end)
+			fetch(following, stage ^ 1);
+		cp_async_commit();
+		uint32_t off = own_off;
+		if (CODES)
+			encode_tile<W, KP>(smem + CODED, smem + STAGES + stage * STAGE, &off, tid);
+		off = CODES ? __syncthreads_or(off != 0) : 0;
+		if (there)
+#pragma unroll
+			for (int kb = 0; kb < STREAM / 16; kb++) {
+				float e[2][4];
+				bool grew = false;
+#pragma unroll
+				for (int i = 0; i < 4; i++) {
+					e[i / 2][2 * (i % 2)] = e_all[kb][i].x;
+					e[i / 2][2 * (i % 2) + 1] = e_all[kb][i].y;
+					grew |= fabsf(e_all[kb][i].x) > limit[i % 2] || fabsf(e_all[kb][i].y) > limit[i % 2];
+				}
+				if (__any_sync(0xffffffffu, grew))
+					follow_largest<W>(e, unit, limit, e_sum, acc, j);
+				uint32_t eb[2][2];
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					eb[i / 2][i % 2] = Half2<__half>::pack(e[i % 2][i / 2 * 2] * unit[i / 2], e[i % 2][i / 2 * 2 + 1] * unit[i / 2]);
+				const bool coded = CODES && !off;
+				if (coded)
+					Half2<__half>::mma(e_sum, eb[0][0], eb[1][0], eb[0][1], eb[1][1], Half2<__half>::ONES, Half2<__half>::ONES);
+				add_signed<T, W>(acc, eb, coded, coded ? base + CODED : base + STAGES + stage * STAGE, 16 * kb, smem, reinterpret_cast<const uint16_t *>(smem + OWN_X), warp, lane);
+			}
+		it = following;
+		stage ^= 1;
+	}
+	const unsigned again = __reduce_or_sync(0xffffffffu, store_signed<T, W>(acc, unit, e_sum, a, b, head, o0 + 16 * warp, lane, nullptr, dq));
+	for (int r = 0; r < 16; r++)
+		if (again >> r & 1u && o0 + 16 * warp + r < a.n)
+			exact_gradient_row<T, false>(a, mask, b, head, o0 + 16 * warp + r, dvo, lse, delta, dq, dq);
+}
+
+// dk and dv of shared heads: the query heads' shares, in order
+template <typename T> __global__ void __launch_bounds__(256) sum_shares_kernel(const float *part, T *out, long long rows, int group, int width)
+{
+	const long long i = blockIdx.x * 256ll + threadIdx.x; // [bs][n][kv_heads][width]
+	if (i >= rows * width)
+		return;
+	const long long row = i / width;
+	const float *from = part + row * group * width + i % width;
+	float sum = 0.f;
+	for (int g = 0; g < group; g++)
+		sum += from[(long long)g * width];
+	out[i] = from_float<T>(sum);
 }
 
 template <typename T, int W, int V>
-int bwd(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, int vec, cudaStream_t st)
+int bwd(const MaskedArgs &a, const void *dvo_, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, float *e, int vec, cudaStream_t st)
 {
-	if (int rc = bwd_one<T, false, W, V>(a, dvo, lse, delta, dq, nullptr, vec, st))
-		return rc;
-	return bwd_one<T, true, W, V>(a, dvo, lse, delta, dk, dv, vec, st);
+	constexpr int KP = W == 3 ? 16 : 4 * W, VP = 2 * V;
+	constexpr bool CODES = Half2<T>::ONES == Half2<__nv_bfloat16>::ONES;
+	constexpr int dq_bytes = ROWS * 128 * W + 2 * STREAM * KP * 16 + (CODES ? ROWS * 64 * W + STREAM * KP * 16 : 0), bytes = dq_bytes + ROWS * VP * 16 + 2 * STREAM * VP * 16;
+	static_assert(2 * STREAM * KP >= ROWS * 4 * W, "own rows pass through the stages");
+	const T *dvo = static_cast<const T *>(dvo_);
+	const int tiles = (a.n + ROWS - 1) / ROWS, group = a.heads / a.kv_heads;
+	const long long all = (long long)a.bs * a.heads, rows = (long long)a.bs * a.n * a.kv_heads;
+	if (all * tiles > 0x7fffffffll || rows * (a.width > a.v_width ? a.width : a.v_width) / 256 >= 0x7fffffffll)
+		return L1ATTN_ERR_SHAPE;
+	BackwardParts parts = {0, int(all), e, masked_unit_floats(a.n), int((a.n + 63ll) / 64 * 64), nullptr, nullptr};
+	if (group > 1) {
+		parts.dk = shares;
+		parts.dv = shares + (long long)a.bs * a.n * a.heads * a.width;
+	}
+	const long long step = e ? masked_units_at_once(a.bs, a.n, a.heads) : all;
+	for (long long first = 0; first < all; first += step) {
+		parts.first = int(first);
+		parts.units = int(all - first < step ? all - first : step);
+		const unsigned grid = unsigned(parts.units) * unsigned(tiles);
+		L1B_SHARED_MEMORY((masked_bwd_mma_kernel<T, true, W, V>), bytes);
+		masked_bwd_mma_kernel<T, true, W, V><<<grid, THREADS, bytes, st>>>(a, dvo, lse, delta, static_cast<T *>(dk), static_cast<T *>(dv), parts, tiles, vec);
+		L1B_LAUNCH_CHECK();
+		if (e) {
+			L1B_SHARED_MEMORY((masked_dq_mma_kernel<T, W>), dq_bytes);
+			masked_dq_mma_kernel<T, W><<<grid, THREADS, dq_bytes, st>>>(a, dvo, lse, delta, static_cast<T *>(dq), parts, tiles, vec);
+		} else {
+			L1B_SHARED_MEMORY((masked_bwd_mma_kernel<T, false, W, V>), bytes);
+			masked_bwd_mma_kernel<T, false, W, V><<<grid, THREADS, bytes, st>>>(a, dvo, lse, delta, static_cast<T *>(dq), nullptr, parts, tiles, vec);
+		}
+		L1B_LAUNCH_CHECK();
+	}
+	if (group > 1) {
+		sum_shares_kernel<<<unsigned((rows * a.width + 255) / 256), 256, 0, st>>>(parts.dk, static_cast<T *>(dk), rows, group, a.width);
+		L1B_LAUNCH_CHECK();
+		sum_shares_kernel<<<unsigned((rows * a.v_width + 255) / 256), 256, 0, st>>>(parts.dv, static_cast<T *>(dv), rows, group, a.v_width);
+		L1B_LAUNCH_CHECK();
+	}
+	return L1ATTN_OK;
 }
 
 template <typename T, int W, int V> int fwd(const MaskedArgs &a, void *vo, float *lse, int vec, cudaStream_t st)
@@ -829,19 +1059,19 @@ template <typename T> int fwd_type(const MaskedArgs &a, void *vo, float *lse, cu
 }
 
 template <typename T>
-int bwd_type(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, cudaStream_t st)
+int bwd_type(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, float *e, cudaStream_t st)
 {
 	const int vec = vectors(a.q) | vectors(a.k) << 1 | vectors(a.v) << 2 | (aligned(dvo, 16) && a.v_width % 8 == 0) << 3, w = (a.width + 31) / 32;
 	if (a.v_width <= 64)
-		return w == 1 ? bwd<T, 1, 4>(a, dvo, lse, delta, dq, dk, dv, vec, st) : w == 2 ? bwd<T, 2, 4>(a, dvo, lse, delta, dq, dk, dv, vec, st) :
-		       w == 3 ? bwd<T, 3, 4>(a, dvo, lse, delta, dq, dk, dv, vec, st) : bwd<T, 4, 4>(a, dvo, lse, delta, dq, dk, dv, vec, st);
-	return w == 1 ? bwd<T, 1, 8>(a, dvo, lse, delta, dq, dk, dv, vec, st) : w == 2 ? bwd<T, 2, 8>(a, dvo, lse, delta, dq, dk, dv, vec, st) :
-	       w == 3 ? bwd<T, 3, 8>(a, dvo, lse, delta, dq, dk, dv, vec, st) : bwd<T, 4, 8>(a, dvo, lse, delta, dq, dk, dv, vec, st);
+		return w == 1 ? bwd<T, 1, 4>(a, dvo, lse, delta, dq, dk, dv, shares, e, vec, st) : w == 2 ? bwd<T, 2, 4>(a, dvo, lse, delta, dq, dk, dv, shares, e, vec, st) :
+		       w == 3 ? bwd<T, 3, 4>(a, dvo, lse, delta, dq, dk, dv, shares, e, vec, st) : bwd<T, 4, 4>(a, dvo, lse, delta, dq, dk, dv, shares, e, vec, st);
+	return w == 1 ? bwd<T, 1, 8>(a, dvo, lse, delta, dq, dk, dv, shares, e, vec, st) : w == 2 ? bwd<T, 2, 8>(a, dvo, lse, delta, dq, dk, dv, shares, e, vec, st) :
+	       w == 3 ? bwd<T, 3, 8>(a, dvo, lse, delta, dq, dk, dv, shares, e, vec, st) : bwd<T, 4, 8>(a, dvo, lse, delta, dq, dk, dv, shares, e, vec, st);
 }
 
 } // namespace
 
-bool masked_mma_fits(const MaskedArgs &a, int dtype) { return dtype != L1ATTN_F32 && a.width <= 128 && a.v_width <= 128; }
+bool masked_mma_fits(int width, int v_width, int dtype) { return dtype != L1ATTN_F32 && width <= 128 && v_width <= 128; }
 
 int masked_mma_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st)
 {
@@ -849,9 +1079,23 @@ int masked_mma_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, 
 }
 
 
-int masked_mma_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, int dtype, cudaStream_t st)
+// Floats that hold a unit's e (rows and columns to whole tiles), and units whose e are alive at once: up to a gigabyte of them; none when one unit is
+// larger (more than 16384 tokens): the queries' kernel then forms the weights again.
+long long masked_unit_floats(int n)
 {
-	return dtype == L1ATTN_F16 ? bwd_type<__half>(a, dvo, lse, delta, dq, dk, dv, st) : bwd_type<__nv_bfloat16>(a, dvo, lse, delta, dq, dk, dv, st);
+	const long long side = (n + 63ll) / 64 * 64;
+	return side * side;
+}
+long long masked_units_at_once(int bs, int n, int heads)
+{
+	const long long all = (long long)bs * heads, fit = (1ll << 28) / masked_unit_floats(n);
+	return fit < all ? fit : all;
+}
+
+int masked_mma_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, float *e, int dtype,
+			  cudaStream_t st)
+{
+	return dtype == L1ATTN_F16 ? bwd_type<__half>(a, dvo, lse, delta, dq, dk, dv, shares, e, st) : bwd_type<__nv_bfloat16>(a, dvo, lse, delta, dq, dk, dv, shares, e, st);
 }
 
 } // namespace l1b

@@ -109,6 +109,20 @@ __device__ __forceinline__ float exp2_fast(float x)
 	return y;
 }
 
+// bfloat16 values as codes of 15 bits in their order: signs of differences then take one instruction for two (signs_of_codes).  A code is the value's
+// magnitude, less CODE_BASE and not below 0, with its sign: exact from 2^-63 to 2^64, and for zero.
+constexpr int CODE_BASE = 8063, CODE_MOST = 16383;
+// two codes; *off: not zero once a value is not zero and outside
+__device__ __forceinline__ uint32_t codes_of_bf16(uint32_t x, uint32_t *off)
+{
+	const uint32_t size = x & 0x7fff7fffu, above = __viaddmax_s16x2(size, uint32_t(-CODE_BASE & 0xffff) * 0x10001u, 0u);
+	const uint32_t m = __vmins2(above, CODE_MOST * 0x10001u), minus = (x >> 15 & 0x10001u) * 0xffffu;
+	*off |= (m ^ above) | (__vminu2(m, 0x10001u) ^ __vminu2(size, 0x10001u)); // cut at the top; at the bottom without being zero
+	return __vsub2(m ^ minus, minus);
+}
+// sign(a - b) + 1 as float16: 0, 2^-24 or 2^-23; takes 1 - b
+__device__ __forceinline__ uint32_t signs_of_codes(uint32_t a, uint32_t one_less_b) { return __viaddmin_s16x2_relu(a, one_less_b, 0x00020002u); }
+
 // Where 16-byte piece c of row r lies in a tile of rows of `pieces` pieces (4, 8 or 16 where SWIZZLED).  SWIZZLED: for ldmatrix, eight rows at one piece
 // in eight different places of the banks.
 template <bool SWIZZLED> __device__ __forceinline__ uint32_t tile_offset(int pieces, int r, int c)

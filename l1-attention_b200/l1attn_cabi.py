@@ -37,7 +37,7 @@ SIGNATURES = {
     "l1attn_dense_softmax_v_bwd_dx": (_i, [_vp] * 8 + [_i] * 6 + [_vp]),
     "l1attn_dense_bwd_scratch_bytes": (_sz, [_i] * 5),
     "l1attn_dense_bwd": (_i, [_vp] * 6 + [_i] * 5 + [_vp]),
-    "l1attn_masked_work_bytes": (_sz, [_i] * 4),
+    "l1attn_masked_work_bytes": (_sz, [_i] * 8),
     "l1attn_masked_fwd": (_i, [_vp] * 7 + [_i] * 6 + [_vp, _i, _vp]),
     "l1attn_masked_bwd": (_i, [_vp] * 11 + [_i] * 6 + [_vp, _i, _vp]),
     "l1attn_cache_append": (_i, [_vp] * 4 + [_i] * 2 + [_vp]),
@@ -314,12 +314,12 @@ def _strides(*tensors):
     return (_c.c_int64 * 9)(*(s for t in tensors for s in t.stride()[:3]))
 
 
-def _masked_work(q, doc, backward):
+def _masked_work(q, v, doc, backward):
     import torch
     if doc is None and not backward:
         return None
-    bs, n, h, _ = q.shape
-    return torch.empty(lib().l1attn_masked_work_bytes(bs, n, h, int(backward)), dtype=torch.uint8, device=q.device)
+    (bs, n, h, w), (hk, wv) = q.shape, v.shape[2:]
+    return torch.empty(lib().l1attn_masked_work_bytes(bs, n, h, hk, w, wv, _tdt(q, allow16=True), int(backward)), dtype=torch.uint8, device=q.device)
 
 
 def masked_fwd(q, k, v, mask, lse=True):
@@ -328,7 +328,7 @@ def masked_fwd(q, k, v, mask, lse=True):
     (bs, n, h, w), (hk, wv) = q.shape, v.shape[2:]
     vo = torch.empty((bs, n, h, wv), dtype=q.dtype, device=q.device)
     ls = torch.empty((bs, n, h), dtype=torch.float32, device=q.device) if lse else None
-    work = _masked_work(q, mask.tensors[1], False)
+    work = _masked_work(q, v, mask.tensors[1], False)
     _check(lib().l1attn_masked_fwd(_dp(q), _dp(k), _dp(v), _strides(q, k, v), _dp(vo), _dp(ls), _dp(work), bs, n, h, hk, w, wv, _c.byref(mask),
                                    _tdt(q, allow16=True), _stream()), "l1attn_masked_fwd")
     return vo, ls
@@ -339,7 +339,7 @@ def masked_bwd(q, k, v, vo, dvo, lse, mask):
     import torch
     (bs, n, h, w), (hk, wv) = q.shape, v.shape[2:]
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    work = _masked_work(q, mask.tensors[1], True)
+    work = _masked_work(q, v, mask.tensors[1], True)
     _check(lib().l1attn_masked_bwd(_dp(q), _dp(k), _dp(v), _strides(q, k, v), _dp(vo), _dp(dvo), _dp(lse), _dp(dq), _dp(dk), _dp(dv), _dp(work), bs, n, h,
                                    hk, w, wv, _c.byref(mask), _tdt(q, allow16=True), _stream()), "l1attn_masked_bwd")
     return dq, dk, dv

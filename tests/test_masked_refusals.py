@@ -48,7 +48,14 @@ def test_abi_alignment_and_empty():
 
 def test_work_bytes():
     f = l1attn_cabi.lib().l1attn_masked_work_bytes
-    assert f(2, 65, 3, 0) == 256 and f(2, 1024, 3, 0) == 2 * 16 * 16 and f(2, 1024, 3, 1) == 512 + 2 * 1024 * 3 * 4 and f(0, 0, 0, 1) == 256
+    f32, bf16 = l1attn_cabi.F32, l1attn_cabi.BF16
+    assert f(2, 65, 3, 3, 64, 64, bf16, 0) == 256 and f(2, 1024, 3, 3, 64, 64, bf16, 0) == 2 * 16 * 16 and f(0, 0, 0, 0, 0, 0, bf16, 1) == 256
+    rows = 2 * 1024 * 4 * 4
+    assert f(2, 1024, 4, 4, 64, 64, f32, 1) == f(2, 1024, 4, 2, 129, 64, bf16, 1) == 512 + rows  # ranges, delta
+    assert f(2, 1024, 4, 4, 64, 32, bf16, 1) == 512 + rows + 8 * 1024 * 1024 * 4  # and a float per pair
+    assert f(2, 1024, 4, 2, 64, 32, bf16, 1) == 512 + rows + rows * 96 + 8 * 1024 * 1024 * 4  # and shares of shared heads
+    assert f(8, 8192, 8, 8, 64, 64, bf16, 1) == 8 * 128 * 16 + 8 * 8192 * 8 * 4 + (1 << 30)  # never more than a gigabyte of pairs
+    assert f(1, 16385, 2, 2, 64, 64, bf16, 1) == 257 * 16 // 256 * 256 + 256 + (16385 * 2 * 4 + 255) // 256 * 256
 
 
 def test_module_refusals():
