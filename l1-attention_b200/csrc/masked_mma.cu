@@ -610,7 +610,7 @@ template <typename T, bool OWN_KEYS, int W, int V>
 __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a, const T *dvo, const float *lse, const float *delta, T *dx, T *dv, BackwardParts parts, int tiles, int vec)
 {
 	extern __shared__ uint4 smem16[];
-	__shared__ float sums[STREAM], stat_lse[STREAM], stat_delta[STREAM];
+	__shared__ float sums[STREAM], stats[2][2][STREAM]; // [stage][log-normaliser, delta] of streamed queries
 	using H = Half2<T>;
 	constexpr int KP = W == 3 ? 16 : 4 * W, VP = 2 * V, WB = 2 * W; // 16-byte pieces of a row; 16-column blocks
 	constexpr bool CODES = H::ONES == Half2<__nv_bfloat16>::ONES;
@@ -626,27 +626,22 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 	const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
 	const Strided go = {dvo, (long long)a.n * a.heads * a.v_width, (long long)a.heads * a.v_width, a.v_width};
 
-	// own rows: in registers for the scores, every value twice in a word for the signs ([row][g][column block][w = g, g + 8]); own values stay in shared memory
+	// own rows stay in shared memory: as they are for the scores (registers that held them were missing beside the sums), as a table for the signs
 	const int32_t *own_doc = mask.doc && mask.ranges[o0 / DOC_TILE].others ? mask.doc : nullptr;
-	constexpr uint32_t FROM = CODES ? OWN_X : STAGES; // (kept where tiles that codes do not fit may need it)
-	load_tile16<T, false, 4 * W, ROWS, THREADS>(base + FROM, OWN_KEYS ? a.k : a.q, b, OWN_KEYS ? kv : head, o0, a.n, a.width, own_doc, vec & (OWN_KEYS ? 2 : 1), tid);
+	load_tile16<T, false, 4 * W, ROWS, THREADS>(base + OWN_X, OWN_KEYS ? a.k : a.q, b, OWN_KEYS ? kv : head, o0, a.n, a.width, own_doc, vec & (OWN_KEYS ? 2 : 1), tid);
 	load_tile16<T, true, VP, ROWS, THREADS>(base + OWN_Y, OWN_KEYS ? a.v : go, b, OWN_KEYS ? kv : head, o0, a.n, a.v_width, own_doc, vec & (OWN_KEYS ? 4 : 8), tid);
 	cp_async_commit();
 	cp_async_wait<0>();
 	__syncthreads();
-	uint32_t x_own[WB][4];
+	const unsigned char *const own_rows = smem + OWN_X;
 	float own_sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
 	for (int u = 0; u < W; u++) {
-		const uint4 x = load_shared16(smem + FROM, tile_offset<false>(4 * W, 16 * warp + g, 4 * u + j)),
-			    y = load_shared16(smem + FROM, tile_offset<false>(4 * W, 16 * warp + g + 8, 4 * u + j));
-		x_own[2 * u][0] = x.x, x_own[2 * u][1] = y.x, x_own[2 * u][2] = x.y, x_own[2 * u][3] = y.y;
-		x_own[2 * u + 1][0] = x.z, x_own[2 * u + 1][1] = y.z, x_own[2 * u + 1][2] = x.w, x_own[2 * u + 1][3] = y.w;
+		const uint4 x = load_shared16(own_rows, tile_offset<false>(4 * W, 16 * warp + g, 4 * u + j)), y = load_shared16(own_rows, tile_offset<false>(4 * W, 16 * warp + g + 8, 4 * u + j));
+		H::mma(own_sum, x.x, y.x, x.y, y.y, H::ONES, H::ONES);
+		H::mma(own_sum, x.z, y.z, x.w, y.w, H::ONES, H::ONES);
 	}
-#pragma unroll
-	for (int u = 0; u < WB; u++)
-		H::mma(own_sum, x_own[u][0], x_own[u][1], x_own[u][2], x_own[u][3], H::ONES, H::ONES);
-	uint32_t own_off = own_table<T, W>(smem, smem + FROM, tid);
+	uint32_t own_off = own_table<T, W>(smem, own_rows, tid);
 
 	float acc[WB][2][4], accv[OWN_KEYS ? 2 * V : 1][4]; // [column block][own rows 0-7, 8-15]: rows of the product are columns w, its columns own rows
 #pragma unroll
@@ -687,6 +682,11 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 		const uint32_t at = base + STAGES + stage * STAGE;
 		load_tile16<T, true, 4 * W, STREAM, THREADS, KP>(at, OWN_KEYS ? a.q : a.k, b, other, i * STREAM, a.n, a.width, doc, vec & (OWN_KEYS ? 1 : 2), tid);
 		load_tile16<T, true, VP, STREAM, THREADS>(at + STREAM * KP * 16, OWN_KEYS ? go : a.v, b, other, i * STREAM, a.n, a.v_width, doc, vec & (OWN_KEYS ? 8 : 4), tid);
+		if (OWN_KEYS && tid < 2 * STREAM) {
+			const int t = i * STREAM + tid % STREAM;
+			const float *from = (tid < STREAM ? lse : delta) + ((long long)b * a.n + min(t, a.n - 1)) * a.heads + head;
+			asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_address(&stats[stage][tid / STREAM][tid % STREAM])), "l"(from) : "memory");
+		}
 	};
 	// a row's log-normaliser as the exponent takes it: a row without weights gets +inf, so that its weights are zero
 	auto exponent = [&](float x) { return x == -INFINITY ? INFINITY : x * LOG2E; };
@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 			row_lse[r] = oa + 8 * r < a.n ? exponent(lse[row]) : INFINITY;
 			row_delta[r] = oa + 8 * r < a.n ? delta[row] : 0.f;
 		}
-	own_off = __syncthreads_or(own_off != 0); // (and the stage that own rows came through is free)
+	own_off = __syncthreads_or(own_off != 0);
 
 	const float slope = a.slopes ? a.slopes[head] : 0.f;
 	int it = next(first_tile), stage = 0;
@@ -727,11 +727,6 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 				sums[r + g + 8] = s[2];
 			}
 		}
-		if (OWN_KEYS && tid < STREAM) {
-			const long long row = ((long long)b * a.n + r0 + tid) * a.heads + head;
-			stat_lse[tid] = r0 + tid < a.n ? exponent(lse[row]) : INFINITY;
-			stat_delta[tid] = r0 + tid < a.n ? delta[row] : 0.f;
-		}
 		uint32_t off = own_off;
 		if (CODES)
 			encode_tile<W, KP>(smem + CODED, xt, &off, tid);
@@ -740,6 +735,13 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 #pragma unroll 1
 		for (int kb = 0; kb < STREAM / 16; kb++) {
 			float x[2][4] = {}, dp[2][4] = {};
+			uint32_t x_own[WB][4];
+#pragma unroll
+			for (int u = 0; u < W; u++) {
+				const uint4 v = load_shared16(own_rows, tile_offset<false>(4 * W, 16 * warp + g, 4 * u + j)), w = load_shared16(own_rows, tile_offset<false>(4 * W, 16 * warp + g + 8, 4 * u + j));
+				x_own[2 * u][0] = v.x, x_own[2 * u][1] = w.x, x_own[2 * u][2] = v.y, x_own[2 * u][3] = w.y;
+				x_own[2 * u + 1][0] = v.z, x_own[2 * u + 1][1] = w.z, x_own[2 * u + 1][2] = v.w, x_own[2 * u + 1][3] = w.w;
+			}
 #pragma unroll
 			for (int n = 0; n < 8; n++) {
 				const uint32_t one = g == n ? H::ONES : 0u;
@@ -769,8 +771,9 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 				const int c0 = 16 * kb + 8 * h + 2 * j;
 				const float2 s = *reinterpret_cast<const float2 *>(&sums[c0]);
 				if (OWN_KEYS) {
-					lse_c[h] = *reinterpret_cast<const float2 *>(&stat_lse[c0]);
-					delta_c[h] = *reinterpret_cast<const float2 *>(&stat_delta[c0]);
+					const float2 l = *reinterpret_cast<const float2 *>(&stats[stage][0][c0]);
+					lse_c[h] = make_float2(exponent(l.x), exponent(l.y));
+					delta_c[h] = *reinterpret_cast<const float2 *>(&stats[stage][1][c0]);
 				} else
 					lse_c[h] = delta_c[h] = make_float2(0.f, 0.f);
 #pragma unroll
@@ -995,7 +998,8 @@ int bwd(const MaskedArgs &a, const void *dvo_, const float *lse, const float *de
 {
 	constexpr int KP = W == 3 ? 16 : 4 * W, VP = 2 * V;
 	constexpr bool CODES = Half2<T>::ONES == Half2<__nv_bfloat16>::ONES;
-	constexpr int dq_bytes = ROWS * 128 * W + 2 * STREAM * KP * 16 + (CODES ? ROWS * 64 * W + STREAM * KP * 16 : 0), bytes = dq_bytes + ROWS * VP * 16 + 2 * STREAM * VP * 16;
+	constexpr int bytes = ROWS * 128 * W + ROWS * VP * 16 + 2 * STREAM * (KP + VP) * 16 + ROWS * 64 * W + (CODES ? STREAM * KP * 16 : 0);
+	constexpr int dq_bytes = ROWS * 128 * W + 2 * STREAM * KP * 16 + (CODES ? ROWS * 64 * W + STREAM * KP * 16 : 0);
 	static_assert(2 * STREAM * KP >= ROWS * 4 * W, "own rows pass through the stages");
 	const T *dvo = static_cast<const T *>(dvo_);
 	const int tiles = (a.n + ROWS - 1) / ROWS, group = a.heads / a.kv_heads;
