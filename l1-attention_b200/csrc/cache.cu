@@ -37,14 +37,19 @@ int check(const l1attn_cache *c, int rows, int dtype, bool tokens, CacheArgs *ou
 	return L1ATTN_OK;
 }
 
-// Splits of the keys: enough CTAs for the GPU, at least 256 keys each.
-void plan(const CacheArgs &c, int rows, int heads, int max_len, int *splits, int *split_keys)
+// Rows of a CTA and splits of the keys: enough CTAs for the GPU, at least 256 keys each.
+void plan(AttendArgs *a, int rows, int heads, int max_len, int dtype)
 {
-	const long long tiles = (long long)rows * (heads / c.kv_heads) / 16 + c.n_seqs, len = max_len < 1 ? 1 : max_len;
-	long long want = (1184 + tiles * c.kv_heads - 1) / (tiles * c.kv_heads), most = (len + 255) / 256;
+	a->heads = heads;
+	a->group = heads / a->c.kv_heads;
+	// eight rows cost half of sixteen on the tensor cores; sequences of one token have as many rows as a group has heads
+	const long long per_seq = (long long)rows * a->group / a->c.n_seqs;
+	a->tile_rows = attend_mma_fits(a->c.width, a->c.v_width, dtype) && per_seq <= 8 ? 8 : 16;
+	const long long tiles = (long long)rows * a->group / a->tile_rows + a->c.n_seqs, len = max_len < 1 ? 1 : max_len;
+	long long want = (1184 + tiles * a->c.kv_heads - 1) / (tiles * a->c.kv_heads), most = (len + 255) / 256;
 	want = want < most ? want : most;
-	*split_keys = int(((len + want - 1) / want + 63) / 64 * 64);
-	*splits = int((len + *split_keys - 1) / *split_keys);
+	a->split_keys = int(((len + want - 1) / want + 63) / 64 * 64);
+	a->splits = int((len + a->split_keys - 1) / a->split_keys);
 }
 
 } // namespace
@@ -97,12 +102,11 @@ extern "C" int l1attn_cache_copy_pages(const l1attn_cache *cache, int layers, co
 
 extern "C" size_t l1attn_cache_attend_bytes(const l1attn_cache *cache, int rows, int n_heads, int max_len, int dtype)
 {
-	CacheArgs c;
-	if (check(cache, rows, dtype, true, &c) || n_heads < 1 || n_heads % c.kv_heads)
+	AttendArgs a;
+	if (check(cache, rows, dtype, true, &a.c) || n_heads < 1 || n_heads % a.c.kv_heads)
 		return 0;
-	int splits, keys;
-	plan(c, rows, n_heads, max_len, &splits, &keys);
-	return splits > 1 ? size_t(splits) * rows * n_heads * (c.v_width + 2) * sizeof(float) : 0;
+	plan(&a, rows, n_heads, max_len, dtype);
+	return a.splits > 1 ? size_t(a.splits) * rows * n_heads * (a.c.v_width + 2) * sizeof(float) : 0;
 }
 
 extern "C" int l1attn_cache_attend(const l1attn_cache *cache, const void *q, const int64_t *strides, void *vo, void *work, int rows, int n_heads, int max_len,
@@ -126,19 +130,17 @@ extern "C" int l1attn_cache_attend(const l1attn_cache *cache, const void *q, con
 	a.vo = vo;
 	a.q_row = strides[0];
 	a.q_head = strides[1];
-	a.heads = n_heads;
-	a.group = n_heads / a.c.kv_heads;
 	a.window = mask->window;
 	a.mode = mask->mode;
 	a.cap = mask->softcap;
 	a.scale = float(1.0 / std::sqrt(double(a.c.width)));
 	a.slopes = mask->slopes;
-	plan(a.c, rows, n_heads, max_len, &a.splits, &a.split_keys);
+	plan(&a, rows, n_heads, max_len, dtype);
 	if (a.splits > 1 && !work)
 		return L1ATTN_ERR_ARG;
 	a.part = a.splits > 1 ? static_cast<float *>(work) : nullptr;
 	const cudaStream_t st = static_cast<cudaStream_t>(stream);
-	if (const int e = attend_simple_launch(a, dtype, st))
+	if (const int e = attend_mma_fits(a.c.width, a.c.v_width, dtype) ? attend_mma_launch(a, dtype, st) : attend_simple_launch(a, dtype, st))
 		return e;
 	return a.splits > 1 ? attend_merge_launch(a, dtype, st) : L1ATTN_OK;
 }

@@ -97,6 +97,7 @@ struct AttendArgs {
 	const float *slopes;
 	float *part; // [splits][rows][heads][v_width + 2], or null: one split
 	int splits, split_keys;
+	int tile_rows; // rows -- (token, head of the group) pairs of one sequence -- of a CTA: 8 or 16
 };
 
 // joins the splits' running maxima, sums and accumulated values (a part: m, l, values)
@@ -104,6 +105,9 @@ int attend_merge_launch(const AttendArgs &a, int dtype, cudaStream_t st);
 int append_launch(const CacheArgs &c, const void *k, const void *v, const long long *strides, int dtype, cudaStream_t st);
 int gather_launch(const CacheArgs &c, void *k, void *v, int dtype, cudaStream_t st);
 int copy_pages_launch(const CacheArgs &c, int layers, const int32_t *src, const int32_t *dst, int n, cudaStream_t st);
+// 16-bit types, widths up to 128: on the tensor cores
+bool attend_mma_fits(int width, int v_width, int dtype);
+int attend_mma_launch(const AttendArgs &a, int dtype, cudaStream_t st);
 int attend_simple_launch(const AttendArgs &a, int dtype, cudaStream_t st);
 
 // (m, l) of a row that has seen all its keys -> factor of its values; a row without weights gets 0.  The +1 form has one more key of
