@@ -30,6 +30,12 @@ __device__ __forceinline__ uint32_t permute(uint32_t a, uint32_t b, uint32_t how
 __device__ __forceinline__ uint32_t half_codes(uint32_t u, uint32_t how) { return H::sub(permute(u, 0x64646464u, how), 0x64806480u); }
 constexpr uint32_t LOW = 0x4140, HIGH = 0x4342;
 
+template <typename T> __device__ __forceinline__ T half_of(uint32_t x, int which)
+{
+	const uint16_t bits = uint16_t(x >> 16 * which);
+	return *reinterpret_cast<const T *>(&bits);
+}
+
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
 {
 	uint32_t y;
@@ -88,6 +94,8 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 	const uint32_t stages = shared_address(mine) + L::Q_TABLE;
 	if (lane < 16 * TILES)
 		rest[lane % (16 * TILES)] = 0.f;
+	for (int i = lane; i < ROWS * W / 2; i += 32)
+		q_table[i] = __floats2half2_rn(0.f, 0.f); // (rows past the last stay zeros)
 	__syncthreads();
 
 	// this lane's columns: query rows 8 tile + 2 j, + 1
@@ -113,12 +121,14 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 	for (int s = 16; s; s >>= 1)
 		q_max = fmaxf(q_max, __shfl_xor_sync(0xffffffffu, q_max, s));
 
-	// chunk number k of this warp begins at position (chunk0 + WARPS k) CHUNK; pages of 32 chunks at a time, one a lane, two such sets
-	const int chunk0 = lo / CHUNK + warp, chunks = hi > lo ? max(0, ((hi + CHUNK - 1) / CHUNK - chunk0 + WARPS - 1) / WARPS) : 0;
+	// The range's chunks are dealt out to the warps in runs (a run has each page's q' formed once); this warp's number k begins at position
+	// (chunk0 + k) CHUNK.  Pages are looked up for 32 chunks at a time, one a lane, two such sets.
+	const int in_range = hi > lo ? (hi + CHUNK - 1) / CHUNK - lo / CHUNK : 0;
+	const int chunk0 = lo / CHUNK + in_range * warp / WARPS, chunks = lo / CHUNK + in_range * (warp + 1) / WARPS - chunk0;
 	int page_id[2];
 	float page_k[2], page_v[2];
 	auto look_up = [&](int block) {
-		const int k = block * 32 + lane, pos = (chunk0 + WARPS * k) * CHUNK;
+		const int k = block * 32 + lane, pos = (chunk0 + k) * CHUNK;
 		int id = -1;
 		float ks = 0.f, vs = 0.f;
 		if (k < chunks) {
@@ -132,24 +142,32 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 		page_k[block & 1] = ks;
 		page_v[block & 1] = vs;
 	};
+	// this lane's pieces of a chunk: rows lane / pieces + i K_ROWS; where they go differs by whole rows, for values also in the bit that i's parity flips
+	constexpr int K_ROWS = 8 / WG, V_ROWS = 16 / VG;
+	const int k_row = lane / (4 * WG), k_piece = lane % (4 * WG), v_row = lane / (2 * VG), v_piece = lane % (2 * VG);
+	const int k_bytes = min(max(c.width - 16 * k_piece, 0), 16), v_bytes = min(max(c.v_width - 16 * v_piece, 0), 16);
+	const int k_from = k_row * c.width + 16 * k_piece, v_from = v_row * c.v_width + 16 * v_piece;
+	const uint32_t k_at = key_place<WG>(k_row, k_piece);
+	const uint32_t v_at[2] = {L::KEY_BYTES + value_place<VG>(v_row, v_piece / 2) + v_piece % 2 * 16,
+				  L::KEY_BYTES + value_place<VG>(v_row + V_ROWS, v_piece / 2) + v_piece % 2 * 16 - V_ROWS * 32 * VG};
 	auto of_chunk = [&](auto &set, int k) { return __shfl_sync(0xffffffffu, k & 32 ? set[1] : set[0], k & 31); };
 	auto fetch = [&](int k) {
 		if (k < chunks) {
-			const int pos = (chunk0 + WARPS * k) * CHUNK, id = of_chunk(page_id, k);
+			const int pos = (chunk0 + k) * CHUNK, id = of_chunk(page_id, k);
 			const uint32_t at = stages + k % L::STAGES * L::STAGE;
 			const long long row = ((long long)max(id, 0) * c.kv_heads + kv) * c.page + pos % c.page;
 			const int8_t *from_k = c.k_codes + row * c.width, *from_v = c.v_codes + row * c.v_width;
-			if (vec) {
+			if (vec) { // a lane copies one column of pieces
+				const int kb = id < 0 ? 0 : k_bytes, vb = id < 0 ? 0 : v_bytes;
+				from_k += kb ? k_from : 0;
+				from_v += vb ? v_from : 0;
+				const int k_step = kb ? K_ROWS * c.width : 0, v_step = vb ? V_ROWS * c.v_width : 0;
 #pragma unroll
-				for (int i = lane; i < CHUNK * 4 * WG; i += 32) {
-					const int r = i / (4 * WG), p = i % (4 * WG), bytes = id < 0 ? 0 : min(max(c.width - 16 * p, 0), 16);
-					copy_async16(at + key_place<WG>(r, p), bytes ? from_k + r * c.width + 16 * p : from_k, bytes);
-				}
+				for (int i = 0; i < CHUNK / K_ROWS; i++, from_k += k_step)
+					copy_async16(at + k_at + i * K_ROWS * 64 * WG, from_k, kb);
 #pragma unroll
-				for (int i = lane; i < CHUNK * 2 * VG; i += 32) {
-					const int r = i / (2 * VG), p = i % (2 * VG), bytes = id < 0 ? 0 : min(max(c.v_width - 16 * p, 0), 16);
-					copy_async16(at + L::KEY_BYTES + value_place<VG>(r, p / 2) + p % 2 * 16, bytes ? from_v + r * c.v_width + 16 * p : from_v, bytes);
-				}
+				for (int i = 0; i < CHUNK / V_ROWS; i++, from_v += v_step)
+					copy_async16(at + v_at[i & 1] + i * V_ROWS * 32 * VG, from_v, vb);
 			} else { // rows that are no 16-byte vectors
 				unsigned char *const to = mine + L::Q_TABLE + k % L::STAGES * L::STAGE;
 				for (int i = lane; i < CHUNK * W; i += 32) {
@@ -177,7 +195,7 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 			look_up(k / 32 + 1);
 		__syncwarp(); // (everyone is done with the stage that is filled next)
 		fetch(k + L::STAGES - 1);
-		const int id = of_chunk(page_id, k), s0 = (chunk0 + WARPS * k) * CHUNK;
+		const int id = of_chunk(page_id, k), s0 = (chunk0 + k) * CHUNK;
 		const float ks = of_chunk(page_k, k), vs = of_chunk(page_v, k);
 		if (id != page_before) { // q' of this page
 			page_before = id;
@@ -186,8 +204,13 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 			const float inv = none ? 0.f : 1.f / ks, s = none ? 0.f : ks;
 			const bool clips = none || !(q_max * inv <= 128.f);
 			if (!clips) {
-				for (int i = lane; i < ROWS * W / 2; i += 32)
-					q_table[i] = __floats2half2_rn(to_float(q_rows[2 * i]) * inv, to_float(q_rows[2 * i + 1]) * inv);
+				for (int i = lane; i < rows * (W / 4); i += 32) {
+					const uint2 x = reinterpret_cast<const uint2 *>(q_rows)[i];
+					uint2 y;
+					y.x = H::pack(to_float(half_of<T>(x.x, 0)) * inv, to_float(half_of<T>(x.x, 1)) * inv);
+					y.y = H::pack(to_float(half_of<T>(x.y, 0)) * inv, to_float(half_of<T>(x.y, 1)) * inv);
+					reinterpret_cast<uint2 *>(q_table)[i] = y;
+				}
 			} else {
 				for (int r = 0; r < rows; r++) {
 					float off = 0.f;
