@@ -83,6 +83,17 @@ L1B_BOTH int cache_find(const CacheArgs &c, long long u, int num, int den, int e
 	return lo;
 }
 
+#ifdef __CUDACC__
+// cache_find by a whole warp: a lane per sequence, so that the reads do not wait for one another (a CTA's first steps are many such waits)
+__device__ __forceinline__ int cache_find_warp(const CacheArgs &c, long long u, int num, int den, int extra)
+{
+	int before = 0;
+	for (int i = threadIdx.x % 32; i < (c.n_seqs + 31) / 32 * 32; i += 32)
+		before += __popc(__ballot_sync(0xffffffffu, i < c.n_seqs && cache_first_unit(c, min(i, c.n_seqs - 1), num, den, extra) <= u));
+	return max(before - 1, 0);
+}
+#endif
+
 // the sequence whose rows [cu[i], cu[i + 1]) hold `row`, if any does: the last one that begins at or before it
 L1B_BOTH int cache_find_row(const CacheArgs &c, long long row) { return cache_find(c, row, 1, 1, 0); }
 

@@ -38,7 +38,7 @@ template <typename T, int NV> __global__ void __launch_bounds__(THREADS) attend_
 	const int wp = pitch(c.width), vp = 64 * NV, tid = threadIdx.x, tx = tid % 16, ty = tid / 16, kv = blockIdx.y;
 	constexpr int PP = KEYS + 4;
 	float *Q = reinterpret_cast<float *>(smem4), *K = Q + ROWS * wp, *V = K + KEYS * wp, *P = V + KEYS * vp;
-	const int seq = cache_find(c, blockIdx.x, a.group, a.tile_rows, 1);
+	const int seq = cache_find_warp(c, blockIdx.x, a.group, a.tile_rows, 1);
 	const SeqView sv = cache_seq(c, seq);
 	const long long first = (blockIdx.x - cache_first_unit(c, seq, a.group, a.tile_rows, 1)) * ROWS, all = (long long)sv.count * a.group;
 	if (first < 0 || first >= all)

@@ -54,13 +54,13 @@ template <int VG> __device__ __forceinline__ uint32_t value_place(int row, int g
 // WG: 64-column groups of the width (1, 2); VG: 32-channel groups of the values (2, 4); TILES: of eight query rows; NG: groups of 16 keys a chunk (1 where pages
 // are of 16 tokens, so that a chunk has one scale)
 template <typename T, int WG, int VG, int TILES, int NG> struct Layout {
-	static constexpr int CHUNK = 16 * NG, KEY_BYTES = CHUNK * 64 * WG, STAGE = CHUNK * (64 * WG + 32 * VG), STAGES = TILES == 1 ? 3 : 2;
+	static constexpr int CHUNK = 16 * NG, KEY_BYTES = CHUNK * 64 * WG, STAGE = CHUNK * (64 * WG + 32 * VG), STAGES = 2;
 	static constexpr int Q_TABLE = 8 * TILES * 64 * WG * 2, WARP = Q_TABLE + STAGES * STAGE + 64 * TILES; // q' | stages | clipped rests
 	static constexpr int Q_ROWS = 8 * TILES * 64 * WG * 2, JOIN = WARPS * 8 * TILES * (32 * VG + 2) * 4;
 	static constexpr int BYTES = Q_ROWS + (WARPS * WARP > JOIN ? WARPS * WARP : JOIN);
 };
 
-template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launch_bounds__(THREADS, 2) attend_mma_kernel(AttendArgs a, int vec)
+template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launch_bounds__(THREADS, TILES == 1 ? 3 : 2) attend_mma_kernel(AttendArgs a, int vec)
 {
 	extern __shared__ uint4 smem16[];
 	using L = Layout<T, WG, VG, TILES, NG>;
@@ -68,7 +68,7 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 	const CacheArgs &c = a.c;
 	unsigned char *const smem = reinterpret_cast<unsigned char *>(smem16);
 	const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4, kv = blockIdx.y;
-	const int seq = cache_find(c, blockIdx.x, a.group, a.tile_rows, 1);
+	const int seq = cache_find_warp(c, blockIdx.x, a.group, a.tile_rows, 1);
 	const SeqView sv = cache_seq(c, seq);
 	const long long first = (blockIdx.x - cache_first_unit(c, seq, a.group, a.tile_rows, 1)) * a.tile_rows, all = (long long)sv.count * a.group;
 	if (first < 0 || first >= all)

@@ -29,7 +29,7 @@ __device__ __forceinline__ int quantise(float x, float s, float inv)
 template <typename T>
 __global__ void __launch_bounds__(THREADS) append_kernel(CacheArgs c, const T *k, const T *v, long long k_row, long long k_head, long long v_row, long long v_head)
 {
-	const int seq = cache_find(c, blockIdx.x, 1, c.page, 2), head = blockIdx.y, tid = threadIdx.x;
+	const int seq = cache_find_warp(c, blockIdx.x, 1, c.page, 2), head = blockIdx.y, tid = threadIdx.x;
 	const SeqView sv = cache_seq(c, seq);
 	const long long unit = blockIdx.x - cache_first_unit(c, seq, 1, c.page, 2), slot = sv.start / c.page + unit;
 	if (unit < 0 || sv.count == 0 || slot * c.page >= (long long)sv.start + sv.count)
