@@ -37,19 +37,35 @@ int check(const l1attn_cache *c, int rows, int dtype, bool tokens, CacheArgs *ou
 	return L1ATTN_OK;
 }
 
-// Rows of a CTA and splits of the keys: enough CTAs for the GPU, at least 256 keys each.
-void plan(AttendArgs *a, int rows, int heads, int max_len, int dtype)
+// How a call is divided, and the bytes of work that takes.
+int plan(AttendArgs *a, int rows, int heads, int max_len, int dtype, size_t *bytes)
 {
 	a->heads = heads;
 	a->group = heads / a->c.kv_heads;
-	// eight rows cost half of sixteen on the tensor cores; sequences of one token have as many rows as a group has heads
-	const long long per_seq = (long long)rows * a->group / a->c.n_seqs;
-	a->tile_rows = attend_mma_fits(a->c.width, a->c.v_width, dtype) && per_seq <= 8 ? 8 : 16;
+	const size_t part = (a->c.v_width + 2) * sizeof(float);
+	if (attend_mma_fits(a->c.width, a->c.v_width, dtype)) { // one wave of CTAs that share the chunks; at least 16 chunks each
+		// eight rows cost half of sixteen; sequences of one token have as many rows as a group has heads
+		a->tile_rows = (long long)rows * a->group / a->c.n_seqs <= 8 ? 8 : 16;
+		int sms = 0;
+		if (int rc = multiprocessors(&sms))
+			return rc;
+		a->ctas = attend_mma_ctas(a->tile_rows, sms);
+		a->least = 16;
+		if ((long long)rows * a->group > 0x7fffffffll - 16)
+			return L1ATTN_ERR_SHAPE;
+		a->splits = 1;
+		*bytes = (2ull * a->ctas * a->tile_rows * part + 255) / 256 * 256 + a->ctas * sizeof(AttendSplit);
+		return L1ATTN_OK;
+	}
+	// splits of the keys: enough CTAs for the GPU, at least 256 keys each
+	a->tile_rows = 16;
 	const long long tiles = (long long)rows * a->group / a->tile_rows + a->c.n_seqs, len = max_len < 1 ? 1 : max_len;
 	long long want = (1184 + tiles * a->c.kv_heads - 1) / (tiles * a->c.kv_heads), most = (len + 255) / 256;
 	want = want < most ? want : most;
 	a->split_keys = int(((len + want - 1) / want + 63) / 64 * 64);
 	a->splits = int((len + a->split_keys - 1) / a->split_keys);
+	*bytes = a->splits > 1 ? size_t(a->splits) * rows * heads * part : 0;
+	return L1ATTN_OK;
 }
 
 } // namespace
@@ -105,8 +121,8 @@ extern "C" size_t l1attn_cache_attend_bytes(const l1attn_cache *cache, int rows,
 	AttendArgs a;
 	if (check(cache, rows, dtype, true, &a.c) || n_heads < 1 || n_heads % a.c.kv_heads)
 		return 0;
-	plan(&a, rows, n_heads, max_len, dtype);
-	return a.splits > 1 ? size_t(a.splits) * rows * n_heads * (a.c.v_width + 2) * sizeof(float) : 0;
+	size_t bytes = 0;
+	return plan(&a, rows, n_heads, max_len, dtype, &bytes) ? 0 : bytes;
 }
 
 extern "C" int l1attn_cache_attend(const l1attn_cache *cache, const void *q, const int64_t *strides, void *vo, void *work, int rows, int n_heads, int max_len,
@@ -135,12 +151,18 @@ extern "C" int l1attn_cache_attend(const l1attn_cache *cache, const void *q, con
 	a.cap = mask->softcap;
 	a.scale = float(1.0 / std::sqrt(double(a.c.width)));
 	a.slopes = mask->slopes;
-	plan(&a, rows, n_heads, max_len, dtype);
-	if (a.splits > 1 && !work)
+	size_t bytes = 0;
+	if (const int e = plan(&a, rows, n_heads, max_len, dtype, &bytes))
+		return e;
+	if (bytes && !work)
 		return L1ATTN_ERR_ARG;
-	a.part = a.splits > 1 ? static_cast<float *>(work) : nullptr;
+	a.part = bytes ? static_cast<float *>(work) : nullptr;
 	const cudaStream_t st = static_cast<cudaStream_t>(stream);
-	if (const int e = attend_mma_fits(a.c.width, a.c.v_width, dtype) ? attend_mma_launch(a, dtype, st) : attend_simple_launch(a, dtype, st))
+	if (attend_mma_fits(a.c.width, a.c.v_width, dtype)) {
+		a.splits_of = reinterpret_cast<AttendSplit *>(static_cast<unsigned char *>(work) + bytes - a.ctas * sizeof(AttendSplit));
+		return attend_mma_launch(a, dtype, st);
+	}
+	if (const int e = attend_simple_launch(a, dtype, st))
 		return e;
 	return a.splits > 1 ? attend_merge_launch(a, dtype, st) : L1ATTN_OK;
 }

@@ -97,6 +97,8 @@ __device__ __forceinline__ int cache_find_warp(const CacheArgs &c, long long u, 
 // the sequence whose rows [cu[i], cu[i + 1]) hold `row`, if any does: the last one that begins at or before it
 L1B_BOTH int cache_find_row(const CacheArgs &c, long long row) { return cache_find(c, row, 1, 1, 0); }
 
+struct AttendSplit;
+
 struct AttendArgs {
 	CacheArgs c;
 	const void *q;
@@ -109,6 +111,15 @@ struct AttendArgs {
 	float *part; // [splits][rows][heads][v_width + 2], or null: one split
 	int splits, split_keys;
 	int tile_rows; // rows -- (token, head of the group) pairs of one sequence -- of a CTA: 8 or 16
+	// attend_mma: CTAs that share the work equally, the least share in chunks, and what they leave for each other (work: part, then a record a CTA)
+	int ctas, least;
+	AttendSplit *splits_of;
+};
+
+// A unit -- a tile of rows and a head of keys and values -- that begins in a CTA's share and ends in a later one's (last); kv < 0: none
+struct AttendSplit {
+	int kv, rows, last, pad;
+	long long pair; // first (token, head of the group) pair: token row * group + head of the group
 };
 
 // joins the splits' running maxima, sums and accumulated values (a part: m, l, values)
@@ -118,6 +129,7 @@ int gather_launch(const CacheArgs &c, void *k, void *v, int dtype, cudaStream_t 
 int copy_pages_launch(const CacheArgs &c, int layers, const int32_t *src, const int32_t *dst, int n, cudaStream_t st);
 // 16-bit types, widths up to 128: on the tensor cores
 bool attend_mma_fits(int width, int v_width, int dtype);
+int attend_mma_ctas(int tile_rows, int sms);
 int attend_mma_launch(const AttendArgs &a, int dtype, cudaStream_t st);
 int attend_simple_launch(const AttendArgs &a, int dtype, cudaStream_t st);
 
