@@ -4,6 +4,8 @@
   l1attn_cuda_drv.so                pybind/torch drivers with the reference's module names
   l1attn_sparse_cuda_drv.so         (cuda/setup.py:13-33 of the reference builds the same three
   l1attn_sparse_bidi_cuda_drv.so     modules), each a thin layer that calls the C ABI
+  l1attn_masked_cuda_drv.so         the same for masked attention and the 8-bit cache
+  l1attn_cache_cuda_drv.so
 
 Usage:  python build.py [--force] [--no-drivers]
 nvcc cross-compiles, so no GPU is needed to build.  The objects stay beside the sources
@@ -22,7 +24,7 @@ CSRC = os.path.join(HERE, "csrc")
 INC = os.path.join(ROOT, "include")
 LIB = os.path.join(HERE, "libl1attn_b200.so")
 CU_SOURCES = ["dense_fwd.cu", "dense_fwd_tma.cu", "dense_bwd.cu", "dense_bwd_tma.cu", "dense_bwd_sv.cu", "dense_bwd_small.cu", "dense_bwd_svr.cu", "dense_ties.cu", "dense_softmax_v.cu", "masked.cu", "masked_simple.cu", "masked_mma.cu", "cache.cu", "cache_pages.cu", "cache_attend.cu", "cache_attend_mma.cu", "sparse.cu", "coo.cu", "capi.cu", "tma.cu"]
-DRIVERS = ["l1attn_cuda_drv", "l1attn_sparse_cuda_drv", "l1attn_sparse_bidi_cuda_drv"]
+DRIVERS = ["l1attn_cuda_drv", "l1attn_sparse_cuda_drv", "l1attn_sparse_bidi_cuda_drv", "l1attn_masked_cuda_drv", "l1attn_cache_cuda_drv"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 

@@ -38,6 +38,16 @@ inline void l1b_same(const torch::Tensor &a, const torch::Tensor &b, const char 
 		TORCH_CHECK(a.sizes() == b.sizes(), an, " and ", bn, " must have the same shape");
 }
 
+// Numbers of a message as text.  (They are not streamed: a driver may carry its own copy of the C++ library, whose streams then look for
+// number formats in the locale of the process's other copy.)
+inline std::string l1b_shape(at::IntArrayRef sizes)
+{
+	std::string s = "[";
+	for (size_t i = 0; i < sizes.size(); i++)
+		s += (i ? ", " : "") + std::to_string(sizes[i]);
+	return s + "]";
+}
+
 inline void l1b_status(int rc, const char *fn)
 {
 	if (rc == L1ATTN_OK)

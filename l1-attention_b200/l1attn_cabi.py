@@ -302,7 +302,7 @@ def dense_softmax_v_bwd(q, k, v, dvo, lse, delta, dq, dk, dv, work):
 
 
 class Mask(ctypes.Structure):
-    """l1attn_mask; keeps the tensors whose addresses it holds."""
+    """l1attn_mask, for callers of l1attn_masked_* and l1attn_cache_attend without torch; keeps the tensors whose addresses it holds."""
     _fields_ = [("causal", _i), ("window", _i), ("mode", _i), ("softcap", _c.c_float), ("slopes", _vp), ("doc", _vp), ("prefix", _vp)]
 
     def __init__(self, mode="softmax", causal=True, window=0, softcap=0.0, slopes=None, doc=None, prefix=None):
@@ -310,43 +310,8 @@ class Mask(ctypes.Structure):
         self.tensors = (slopes, doc, prefix)
 
 
-def _strides(*tensors):
-    return (_c.c_int64 * 9)(*(s for t in tensors for s in t.stride()[:3]))
-
-
-def _masked_work(q, v, doc, backward):
-    import torch
-    if doc is None and not backward:
-        return None
-    (bs, n, h, w), (hk, wv) = q.shape, v.shape[2:]
-    return torch.empty(lib().l1attn_masked_work_bytes(bs, n, h, hk, w, wv, _tdt(q, allow16=True), int(backward)), dtype=torch.uint8, device=q.device)
-
-
-def masked_fwd(q, k, v, mask, lse=True):
-    """q [bs, n, h, w], k [bs, n, hk, w], v [bs, n, hk, wv] of any strides with contiguous widths -> (vo, lse [bs, n, h] or None)."""
-    import torch
-    (bs, n, h, w), (hk, wv) = q.shape, v.shape[2:]
-    vo = torch.empty((bs, n, h, wv), dtype=q.dtype, device=q.device)
-    ls = torch.empty((bs, n, h), dtype=torch.float32, device=q.device) if lse else None
-    work = _masked_work(q, v, mask.tensors[1], False)
-    _check(lib().l1attn_masked_fwd(_dp(q), _dp(k), _dp(v), _strides(q, k, v), _dp(vo), _dp(ls), _dp(work), bs, n, h, hk, w, wv, _c.byref(mask),
-                                   _tdt(q, allow16=True), _stream()), "l1attn_masked_fwd")
-    return vo, ls
-
-
-def masked_bwd(q, k, v, vo, dvo, lse, mask):
-    """-> (dq, dk, dv), contiguous; vo, dvo, lse contiguous."""
-    import torch
-    (bs, n, h, w), (hk, wv) = q.shape, v.shape[2:]
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    work = _masked_work(q, v, mask.tensors[1], True)
-    _check(lib().l1attn_masked_bwd(_dp(q), _dp(k), _dp(v), _strides(q, k, v), _dp(vo), _dp(dvo), _dp(lse), _dp(dq), _dp(dk), _dp(dv), _dp(work), bs, n, h,
-                                   hk, w, wv, _c.byref(mask), _tdt(q, allow16=True), _stream()), "l1attn_masked_bwd")
-    return dq, dk, dv
-
-
 class Cache(ctypes.Structure):
-    """l1attn_cache; keeps the tensors whose addresses it holds."""
+    """l1attn_cache, for callers of l1attn_cache_* without torch; keeps the tensors whose addresses it holds."""
     _fields_ = ([(x, _vp) for x in ("k_codes", "v_codes", "k_scale", "v_scale")] + [(x, _i) for x in ("n_pages", "page", "n_kv_heads", "width", "v_width")]
                 + [(x, _vp) for x in ("table", "start", "cu")] + [("n_seqs", _i), ("max_pages", _i), ("status", _vp)])
 
@@ -356,29 +321,6 @@ class Cache(ctypes.Structure):
         super().__init__(_dp(k_codes), _dp(v_codes), _dp(k_scale), _dp(v_scale), n_pages, page, hk, w, v_codes.shape[-1], _dp(table), _dp(start), _dp(cu),
                          n_seqs, max_pages, _dp(status))
         self.tensors = (k_codes, v_codes, k_scale, v_scale, table, start, cu, status)
-
-
-def cache_append(cache, k, v):
-    st = (_c.c_int64 * 4)(*k.stride()[:2], *v.stride()[:2])
-    _check(lib().l1attn_cache_append(_c.byref(cache), _dp(k), _dp(v), st, k.shape[0], _tdt(k, allow16=True), _stream()), "l1attn_cache_append")
-
-
-def cache_gather(cache, k, v):
-    _check(lib().l1attn_cache_gather(_c.byref(cache), _dp(k), _dp(v), k.shape[0], _tdt(k, allow16=True), _stream()), "l1attn_cache_gather")
-
-
-def cache_copy_pages(cache, layers, src, dst):
-    _check(lib().l1attn_cache_copy_pages(_c.byref(cache), layers, _dp(src), _dp(dst), src.shape[0], _stream()), "l1attn_cache_copy_pages")
-
-
-def cache_attend(cache, q, mask, max_len, vo):
-    import torch
-    rows, h, _ = q.shape
-    dt = _tdt(q, allow16=True)
-    nb = lib().l1attn_cache_attend_bytes(_c.byref(cache), rows, h, max_len, dt)
-    work = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
-    st = (_c.c_int64 * 2)(*q.stride()[:2])
-    _check(lib().l1attn_cache_attend(_c.byref(cache), _dp(q), st, _dp(vo), _dp(work), rows, h, max_len, _c.byref(mask), dt, _stream()), "l1attn_cache_attend")
 
 
 def dense_bwd(d_attn, q, k, out=None, scratch="auto"):

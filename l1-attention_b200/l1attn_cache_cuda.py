@@ -32,51 +32,10 @@ No gradients (a cache answers, it does not train) and no CPU path.
 """
 import torch
 
-import l1attn_cabi as _c
-from l1attn_masked_cuda import _options, _side
+import l1attn_cache_cuda_drv  # torch must be imported first: the driver links against libtorch
+from l1attn_masked_cuda import _options, _tensors
 
-TYPES = (torch.float32, torch.float16, torch.bfloat16)
 PAGES = (16, 32, 64, 128, 256)
-
-
-def _cache(k_codes, v_codes, k_scale, v_scale, layers=False):
-    dims = (4, 5) if layers else (4,)
-    for name, t, dt in (("k_codes", k_codes, torch.int8), ("v_codes", v_codes, torch.int8), ("k_scale", k_scale, torch.float32), ("v_scale", v_scale, torch.float32)):
-        if not t.is_cuda:
-            raise RuntimeError("%s must be a CUDA tensor" % name)
-        if t.dtype != dt or not t.is_contiguous() or t.device != k_codes.device:
-            raise RuntimeError("%s must be a contiguous %s tensor on the cache's device" % (name, str(dt).replace("torch.", "")))
-    if k_codes.dim() not in dims or k_codes.shape[:-1] != v_codes.shape[:-1] or k_scale.shape != k_codes.shape[:-2] or v_scale.shape != k_scale.shape:
-        raise RuntimeError("a cache is k_codes [n_pages, hk, page, w], v_codes [n_pages, hk, page, wv], k_scale and v_scale [n_pages, hk]")
-    if k_codes.shape[-2] not in PAGES:
-        raise RuntimeError("page must be one of %s" % (PAGES,))
-    if not 1 <= k_codes.shape[-1] <= 256 or not 1 <= v_codes.shape[-1] <= 256 or k_codes.shape[-3] < 1:
-        raise RuntimeError("widths must be 1 to 256, and heads 1 or more")
-    if k_codes.data_ptr() % 16 or v_codes.data_ptr() % 16:
-        raise RuntimeError("k_codes and v_codes must be aligned to 16 bytes")
-    return k_codes, v_codes, k_scale, v_scale
-
-
-def _places(cache, table, start, cu, status):
-    for name, t in (("table", table), ("start", start), ("cu", cu), ("status", status)):
-        if t is not None and (not t.is_cuda or t.dtype != torch.int32 or t.device != cache[0].device or not t.is_contiguous()):
-            raise RuntimeError("%s must be a contiguous int32 tensor on the cache's device" % name)
-    if table.dim() != 2 or start.shape != table.shape[:1] or cu.dim() != 1 or cu.shape[0] != table.shape[0] + 1 or (status is not None and status.numel() < 1):
-        raise RuntimeError("table must be [n_seqs, max_pages], start [n_seqs], cu [n_seqs + 1], status [1]")
-    if table.shape[1] * cache[0].shape[2] > 0x7fffffff:
-        raise RuntimeError("max_pages * page must fit int32")
-    return _c.Cache(*cache, table, start, cu, status)
-
-
-def _tokens(t, name, cache, heads, width):
-    if not t.is_cuda or t.device != cache[0].device:
-        raise RuntimeError("%s must be a CUDA tensor on the cache's device" % name)
-    if t.dtype not in TYPES:
-        raise RuntimeError("%s must be float32, float16 or bfloat16" % name)
-    if t.dim() != 3 or t.shape[2] != width or (heads is not None and t.shape[1] != heads):
-        raise RuntimeError("%s must be [rows, %s, %d]" % (name, "heads" if heads is None else heads, width))
-    t = t.detach()
-    return t if t.stride(2) == 1 or width == 1 else t.contiguous()
 
 
 def append(k, v, k_codes, v_codes, k_scale, v_scale, table, start, cu, status=None):
@@ -85,33 +44,14 @@ def append(k, v, k_codes, v_codes, k_scale, v_scale, table, start, cu, status=No
     Per page and head the scale is max |x| / 127 over the page's new tokens, or stays where it is larger and the page holds earlier tokens of the
     sequence; code = x / scale to the nearest (ties to even); when a scale grows the earlier codes follow it.  No two sequences of a call may write
     the same page.  NaN is stored as 0, infinities as the largest code."""
-    cache = _cache(k_codes, v_codes, k_scale, v_scale)
-    _, hk, _, w = k_codes.shape
-    k, v = _tokens(k, "k", cache, hk, w), _tokens(v, "v", cache, hk, v_codes.shape[3])
-    if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
-        raise RuntimeError("k and v must share dtype and rows")
-    places = _places(cache, table, start, cu, status)
-    with torch.cuda.device(k.device):
-        _c.cache_append(places, k, v)
+    l1attn_cache_cuda_drv.append(k, v, (k_codes, v_codes, k_scale, v_scale), table, start, cu, status)
 
 
 def gather(k_codes, v_codes, k_scale, v_scale, table, start, cu, rows, dtype=torch.float32, out=None, status=None):
     """(k [rows, hk, w], v [rows, hk, wv]): the values that the cache holds at the given positions, rounded to dtype.  rows: cu[-1], or more
     (rows behind it are left as they were in `out`, and undefined without).  out: a pair of contiguous tensors to write."""
-    cache = _cache(k_codes, v_codes, k_scale, v_scale)
-    _, hk, _, w = k_codes.shape
-    if dtype not in TYPES:
-        raise RuntimeError("dtype must be float32, float16 or bfloat16")
-    shapes = (rows, hk, w), (rows, hk, v_codes.shape[3])
-    if out is None:
-        out = tuple(torch.empty(s, dtype=dtype, device=k_codes.device) for s in shapes)
-    for t, s in zip(out, shapes):
-        if tuple(t.shape) != s or t.dtype != dtype or t.device != k_codes.device or not t.is_contiguous():
-            raise RuntimeError("out must be contiguous %s tensors of shapes %s and %s on the cache's device" % ((str(dtype).replace("torch.", ""),) + shapes))
-    places = _places(cache, table, start, cu, status)
-    with torch.cuda.device(k_codes.device):
-        _c.cache_gather(places, *out)
-    return tuple(out)
+    k_out, v_out = (None, None) if out is None else out
+    return tuple(l1attn_cache_cuda_drv.gather((k_codes, v_codes, k_scale, v_scale), table, start, cu, rows, dtype, k_out, v_out, status))
 
 
 def attend(q, k_codes, v_codes, k_scale, v_scale, table, start, cu, mode="softmax", window=0, softcap=0.0, slopes=None, max_len=None, out=None, status=None):
@@ -122,46 +62,26 @@ def attend(q, k_codes, v_codes, k_scale, v_scale, table, start, cu, mode="softma
     out: a contiguous tensor to write; rows behind cu[-1] are left as they were in it, and undefined without it.
 
     16-bit q: query / scale is rounded to float16 next to codes that it holds exactly, weights to 11 bits; float32 q: float32 throughout."""
-    cache = _cache(k_codes, v_codes, k_scale, v_scale)
-    _, hk, page, w = k_codes.shape
     mode, _, window, softcap = _options(mode, True, window, softcap)
-    q = _tokens(q, "q", cache, None, w)
-    if q.shape[1] < 1 or q.shape[1] % hk:
-        raise RuntimeError("the heads of q must be a multiple of the cache's")
-    slopes = _side(slopes, "slopes", q.shape[1:2], torch.float32, q)
-    shape = (q.shape[0], q.shape[1], v_codes.shape[3])
-    if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-        raise RuntimeError("out must be a contiguous tensor of shape %s and the type of q on its device" % (shape,))
-    places = _places(cache, table, start, cu, status)
-    room = table.shape[1] * page
-    max_len = room if max_len is None else max(0, min(int(max_len), room))
-    with torch.cuda.device(q.device):
-        _c.cache_attend(places, q, _c.Mask(mode, True, window, softcap, slopes), max_len, out)
-    return out
+    return l1attn_cache_cuda_drv.attend(q, (k_codes, v_codes, k_scale, v_scale), table, start, cu, mode, window, softcap, slopes, -1 if max_len is None else max(0, int(max_len)),
+                                        out, status)
 
 
 def copy_pages(k_codes, v_codes, k_scale, v_scale, src, dst, status=None):
     """Page src[i] -> page dst[i], codes and scales of all heads; with a leading layer dimension, of all layers.  src, dst: int32 tensors on the device
     (they are not checked beyond their range), or lists, which are: a page may be copied to several places, but no destination may occur twice or
     be a source."""
-    cache = _cache(k_codes, v_codes, k_scale, v_scale, layers=True)
+    _tensors(k_codes=k_codes, v_codes=v_codes, k_scale=k_scale, v_scale=v_scale)
     if not isinstance(src, torch.Tensor) or not isinstance(dst, torch.Tensor):
+        if not k_codes.is_cuda:
+            raise RuntimeError("k_codes must be a CUDA tensor")
         src, dst = [int(i) for i in src], [int(i) for i in dst]
         if len(src) != len(dst) or len(set(dst)) != len(dst) or set(src) & set(dst) or any(not 0 <= i < k_codes.shape[-4] for i in src + dst):
             raise ValueError("pages must be in range, and no destination may occur twice or be a source")
         if not src:
             return
         src, dst = _upload(src + dst, k_codes.device).view(2, -1)
-    for t in (src, dst):
-        if not t.is_cuda or t.dtype != torch.int32 or t.device != k_codes.device or not t.is_contiguous() or t.dim() != 1 or t.shape != src.shape:
-            raise RuntimeError("src and dst must be contiguous int32 tensors of one length on the cache's device")
-    if status is not None and (not status.is_cuda or status.dtype != torch.int32 or status.device != k_codes.device or status.numel() < 1):
-        raise RuntimeError("status must be an int32 tensor on the cache's device")
-    layers = k_codes.shape[0] if k_codes.dim() == 5 else 1
-    with torch.cuda.device(k_codes.device):
-        _c.cache_copy_pages(_c.Cache(*cache, status=status), layers, src, dst)
+    l1attn_cache_cuda_drv.copy_pages((k_codes, v_codes, k_scale, v_scale), src, dst, status)
 
 
 def _upload(values, device):
