@@ -1,7 +1,7 @@
 // Pages of the 8-bit cache: quantising new tokens into them, reading sequences back, copying pages.
 //
-// All three are bound by memory: append reads a token's row twice (the second time from L1 or L2) and writes a quarter to a half of it,
-// gather reads codes and writes values, copies read and write.
+// All three are bound by memory: append reads a token's row and writes a quarter to a half of it, gather reads codes and writes values, copies read and write.
+#include <type_traits>
 #include "cache.cuh"
 
 namespace l1b {
@@ -25,8 +25,13 @@ __device__ __forceinline__ int quantise(float x, float s, float inv)
 	return int(fminf(fmaxf(q, -127.f), 127.f));
 }
 
+template <typename T> struct Vector { // 16 bytes of tokens
+	static constexpr int N = 16 / sizeof(T);
+};
+
 // A CTA per (page that new tokens touch, head, keys or values): it alone reads and writes that page's rows and scale of that head.
-template <typename T>
+// HELD: 16-byte vectors of its new rows that a thread keeps between the scale and the codes (0: element by element, the rows are read twice).
+template <typename T, int HELD>
 __global__ void __launch_bounds__(THREADS) append_kernel(CacheArgs c, const T *k, const T *v, long long k_row, long long k_head, long long v_row, long long v_head)
 {
 	const int seq = cache_find_warp(c, blockIdx.x, 1, c.page, 2), head = blockIdx.y, tid = threadIdx.x;
@@ -40,24 +45,46 @@ __global__ void __launch_bounds__(THREADS) append_kernel(CacheArgs c, const T *k
 	const bool values = blockIdx.z;
 	const int w = values ? c.v_width : c.width, first = int(slot) * c.page;
 	const int a = max(sv.start - first, 0), b = int(min((long long)sv.start + sv.count - first, (long long)c.page)); // new rows of the page
-	const T *src = (values ? v : k) + (values ? v_head : k_head) * head + (long long)(sv.row + first - sv.start) * (values ? v_row : k_row);
 	const long long src_row = values ? v_row : k_row, at = (long long)id * c.kv_heads + head;
-	int8_t *codes = (values ? c.v_codes : c.k_codes) + at * c.page * w;
-	float *scale = (values ? c.v_scale : c.k_scale) + at;
+	const T *src = (values ? v : k) + (values ? v_head : k_head) * head + (long long)(sv.row + first - sv.start + a) * src_row; // the first new row
+	int8_t *const codes = (values ? c.v_codes : c.k_codes) + at * c.page * w;
+	float *const scale = (values ? c.v_scale : c.k_scale) + at;
+	const float old = a > 0 ? *scale : 0.f;
 
+	constexpr int N = Vector<T>::N;
+	const int per_row = w / N, vectors = (b - a) * per_row;
+	uint4 held[HELD ? HELD : 1];
 	float most = 0.f;
-	for (int i = tid; i < (b - a) * w; i += THREADS) {
-		const float x = fabsf(to_float(src[(a + i / w) * src_row + i % w]));
-		most = finite(x) ? fmaxf(most, x) : most;
-	}
+	if (HELD) {
+#pragma unroll
+		for (int j = 0; j < HELD; j++) {
+			const int i = tid + j * THREADS;
+			if (i >= vectors)
+				break;
+			held[j] = *reinterpret_cast<const uint4 *>(src + (i / per_row) * src_row + i % per_row * N);
+		}
+#pragma unroll
+		for (int j = 0; j < HELD; j++) {
+			if (tid + j * THREADS >= vectors)
+				break;
+#pragma unroll
+			for (int e = 0; e < N; e++) {
+				const float x = fabsf(to_float(reinterpret_cast<const T *>(&held[j])[e]));
+				most = finite(x) ? fmaxf(most, x) : most;
+			}
+		}
+	} else
+		for (int i = tid; i < (b - a) * w; i += THREADS) {
+			const float x = fabsf(to_float(src[(i / w) * src_row + i % w]));
+			most = finite(x) ? fmaxf(most, x) : most;
+		}
 	__shared__ float part[THREADS / 32];
 #pragma unroll
 	for (int o = 16; o; o >>= 1)
 		most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
 	if (tid % 32 == 0)
 		part[tid / 32] = most;
-	const float old = a > 0 ? *scale : 0.f;
-	__syncthreads();
+	__syncthreads(); // (the scale has been read by all)
 #pragma unroll
 	for (int i = 0; i < THREADS / 32; i++)
 		most = fmaxf(most, part[i]);
@@ -65,18 +92,36 @@ __global__ void __launch_bounds__(THREADS) append_kernel(CacheArgs c, const T *k
 	if (a > 0 && now > old) // the rows that were there follow the new scale
 		for (int i = tid; i < a * w; i += THREADS)
 			codes[i] = int8_t(rint(double(codes[i]) * double(old) / double(now)));
-	for (int i = tid; i < (b - a) * w; i += THREADS)
-		codes[a * w + i] = int8_t(quantise(to_float(src[(a + i / w) * src_row + i % w]), now, inv));
+	if (HELD) {
+#pragma unroll
+		for (int j = 0; j < HELD; j++) {
+			const int i = tid + j * THREADS;
+			if (i >= vectors)
+				break;
+			uint32_t out[N / 4];
+#pragma unroll
+			for (int e = 0; e < N; e++) {
+				const uint32_t q = uint32_t(quantise(to_float(reinterpret_cast<const T *>(&held[j])[e]), now, inv)) & 0xffu;
+				out[e / 4] = e % 4 ? out[e / 4] | q << 8 * (e % 4) : q;
+			}
+			int8_t *const to = codes + (long long)a * w + i * N;
+			if constexpr (N == 8)
+				*reinterpret_cast<uint2 *>(to) = make_uint2(out[0], out[1]);
+			else
+				*reinterpret_cast<uint32_t *>(to) = out[0];
+		}
+	} else
+		for (int i = tid; i < (b - a) * w; i += THREADS)
+			codes[a * w + i] = int8_t(quantise(to_float(src[(i / w) * src_row + i % w]), now, inv));
 	if (tid == 0)
 		*scale = now;
 }
 
-// A warp per (row, head): keys and values of the row
-template <typename T> __global__ void __launch_bounds__(THREADS) gather_kernel(CacheArgs c, T *k, T *v)
+// A warp per row and group of heads: keys and values of the row, 16 bytes of codes at a time where widths allow it (VEC), else one by one.
+template <typename T, bool VEC> __global__ void __launch_bounds__(THREADS) gather_kernel(CacheArgs c, T *k, T *v)
 {
-	const long long unit = blockIdx.x * (long long)(THREADS / 32) + threadIdx.x / 32;
-	const int lane = threadIdx.x % 32, head = int(unit % c.kv_heads);
-	const long long row = unit / c.kv_heads;
+	const long long row = blockIdx.x * (long long)(THREADS / 32) + threadIdx.x / 32;
+	const int lane = threadIdx.x % 32;
 	if (row >= c.rows)
 		return;
 	const int seq = cache_find_row(c, row);
@@ -84,13 +129,31 @@ template <typename T> __global__ void __launch_bounds__(THREADS) gather_kernel(C
 	if (row < sv.row || row - sv.row >= sv.count)
 		return;
 	const int pos = sv.start + int(row - sv.row), id = cache_page(c, seq, pos / c.page);
-	const long long at = (long long)max(id, 0) * c.kv_heads + head;
-	const float ks = id < 0 ? 0.f : c.k_scale[at], vs = id < 0 ? 0.f : c.v_scale[at];
-	const int8_t *kc = c.k_codes + (at * c.page + pos % c.page) * c.width, *vc = c.v_codes + (at * c.page + pos % c.page) * c.v_width;
-	for (int w = lane; w < c.width; w += 32)
-		k[unit * c.width + w] = from_float<T>(id < 0 ? 0.f : kc[w] * ks);
-	for (int w = lane; w < c.v_width; w += 32)
-		v[unit * c.v_width + w] = from_float<T>(id < 0 ? 0.f : vc[w] * vs);
+	const long long at = (long long)max(id, 0) * c.kv_heads;
+	for (int values = 0; values < 2; values++) {
+		const int w = values ? c.v_width : c.width;
+		const int8_t *const codes = (values ? c.v_codes : c.k_codes) + (at * c.page + pos % c.page) * w;
+		const float *const scale = (values ? c.v_scale : c.k_scale) + at;
+		T *const out = (values ? v : k) + row * c.kv_heads * w;
+		const long long head = (long long)c.page * w;
+		if (VEC) {
+			const int per_head = w / 16;
+			for (int i = lane; i < c.kv_heads * per_head; i += 32) {
+				const int h = i / per_head;
+				const uint4 x = id < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4 *>(codes + h * head + i % per_head * 16);
+				const float s = id < 0 ? 0.f : scale[h];
+				alignas(16) T y[16];
+#pragma unroll
+				for (int e = 0; e < 16; e++)
+					y[e] = from_float<T>(float(reinterpret_cast<const int8_t *>(&x)[e]) * s);
+#pragma unroll
+				for (int e = 0; e < int(sizeof(T)); e++)
+					reinterpret_cast<uint4 *>(out + i * 16)[e] = reinterpret_cast<const uint4 *>(y)[e];
+			}
+		} else
+			for (int i = lane; i < c.kv_heads * w; i += 32)
+				out[i] = from_float<T>(id < 0 ? 0.f : codes[i / w * head + i % w] * scale[i / w]);
+	}
 }
 
 struct CopyArgs {
@@ -115,13 +178,43 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(CopyArgs c)
 	}
 	const uint4 *a = c.codes[kind] + (layer * c.n_pages + from) * c.vecs[kind];
 	uint4 *b = c.codes[kind] + (layer * c.n_pages + to) * c.vecs[kind];
-	for (long long i = blockIdx.y * 256ll + threadIdx.x; i < c.vecs[kind]; i += gridDim.y * 256ll)
-		b[i] = a[i];
+	for (long long i = blockIdx.y * 1024ll + threadIdx.x; i < c.vecs[kind]; i += gridDim.y * 1024ll) { // four vectors of a thread at once
+		uint4 x[4];
+#pragma unroll
+		for (int j = 0; j < 4; j++)
+			if (i + 256 * j < c.vecs[kind])
+				x[j] = a[i + 256 * j];
+#pragma unroll
+		for (int j = 0; j < 4; j++)
+			if (i + 256 * j < c.vecs[kind])
+				b[i + 256 * j] = x[j];
+	}
 	if (blockIdx.y == 0)
 		for (int i = threadIdx.x; i < c.kv_heads; i += 256)
 			c.scale[kind][(layer * c.n_pages + to) * c.kv_heads + i] = c.scale[kind][(layer * c.n_pages + from) * c.kv_heads + i];
 }
 
+} // namespace
+
+namespace {
+template <typename T> int append_type(const CacheArgs &c, const void *k_, const void *v_, const long long *st4, dim3 grid, cudaStream_t st)
+{
+	const T *k = static_cast<const T *>(k_), *v = static_cast<const T *>(v_);
+	constexpr int N = Vector<T>::N;
+	bool vec = aligned(k, 16) && aligned(v, 16) && c.width % N == 0 && c.v_width % N == 0;
+	for (int i = 0; i < 4; i++)
+		vec = vec && st4[i] % N == 0;
+	// vectors of a page's rows, at most, by thread
+	const int wide = c.width > c.v_width ? c.width : c.v_width, most = (c.page * (wide / N) + THREADS - 1) / THREADS;
+	if (vec && most <= 8)
+		append_kernel<T, 8><<<grid, THREADS, 0, st>>>(c, k, v, st4[0], st4[1], st4[2], st4[3]);
+	else if (vec && most <= 16)
+		append_kernel<T, 16><<<grid, THREADS, 0, st>>>(c, k, v, st4[0], st4[1], st4[2], st4[3]);
+	else
+		append_kernel<T, 0><<<grid, THREADS, 0, st>>>(c, k, v, st4[0], st4[1], st4[2], st4[3]);
+	L1B_LAUNCH_CHECK();
+	return L1ATTN_OK;
+}
 } // namespace
 
 int append_launch(const CacheArgs &c, const void *k, const void *v, const long long *strides, int dtype, cudaStream_t st)
@@ -131,27 +224,28 @@ int append_launch(const CacheArgs &c, const void *k, const void *v, const long l
 		return L1ATTN_ERR_SHAPE;
 	const dim3 grid(unsigned(units), c.kv_heads, 2);
 	if (dtype == L1ATTN_F32)
-		append_kernel<<<grid, THREADS, 0, st>>>(c, static_cast<const float *>(k), static_cast<const float *>(v), strides[0], strides[1], strides[2], strides[3]);
-	else if (dtype == L1ATTN_F16)
-		append_kernel<<<grid, THREADS, 0, st>>>(c, static_cast<const __half *>(k), static_cast<const __half *>(v), strides[0], strides[1], strides[2], strides[3]);
-	else
-		append_kernel<<<grid, THREADS, 0, st>>>(c, static_cast<const __nv_bfloat16 *>(k), static_cast<const __nv_bfloat16 *>(v), strides[0], strides[1], strides[2],
-							strides[3]);
-	L1B_LAUNCH_CHECK();
-	return L1ATTN_OK;
+		return append_type<float>(c, k, v, strides, grid, st);
+	return dtype == L1ATTN_F16 ? append_type<__half>(c, k, v, strides, grid, st) : append_type<__nv_bfloat16>(c, k, v, strides, grid, st);
 }
 
 int gather_launch(const CacheArgs &c, void *k, void *v, int dtype, cudaStream_t st)
 {
-	const long long units = ((long long)c.rows * c.kv_heads + THREADS / 32 - 1) / (THREADS / 32);
-	if (units > 0x7fffffffll)
+	const long long blocks = ((long long)c.rows + THREADS / 32 - 1) / (THREADS / 32);
+	if (blocks > 0x7fffffffll)
 		return L1ATTN_ERR_SHAPE;
+	const bool vec = c.width % 16 == 0 && c.v_width % 16 == 0 && aligned(k, 16) && aligned(v, 16);
+	auto launch = [&](auto *k_, auto *v_) {
+		if (vec)
+			gather_kernel<std::remove_pointer_t<decltype(k_)>, true><<<unsigned(blocks), THREADS, 0, st>>>(c, k_, v_);
+		else
+			gather_kernel<std::remove_pointer_t<decltype(k_)>, false><<<unsigned(blocks), THREADS, 0, st>>>(c, k_, v_);
+	};
 	if (dtype == L1ATTN_F32)
-		gather_kernel<<<unsigned(units), THREADS, 0, st>>>(c, static_cast<float *>(k), static_cast<float *>(v));
+		launch(static_cast<float *>(k), static_cast<float *>(v));
 	else if (dtype == L1ATTN_F16)
-		gather_kernel<<<unsigned(units), THREADS, 0, st>>>(c, static_cast<__half *>(k), static_cast<__half *>(v));
+		launch(static_cast<__half *>(k), static_cast<__half *>(v));
 	else
-		gather_kernel<<<unsigned(units), THREADS, 0, st>>>(c, static_cast<__nv_bfloat16 *>(k), static_cast<__nv_bfloat16 *>(v));
+		launch(static_cast<__nv_bfloat16 *>(k), static_cast<__nv_bfloat16 *>(v));
 	L1B_LAUNCH_CHECK();
 	return L1ATTN_OK;
 }

@@ -121,7 +121,7 @@ long long masked_units_at_once(int bs, int n, int heads);
 int masked_mma_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, float *e, int dtype,
 			  cudaStream_t st);
 int masked_simple_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st);
-int masked_simple_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, int dtype,
+int masked_simple_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, int dtype,
 			     cudaStream_t st);
 
 } // namespace l1b

@@ -53,6 +53,34 @@ template <typename T> __global__ void delta_kernel(const T *dvo, const T *vo, fl
 		delta[row] = sum;
 }
 
+// dk and dv of shared heads: the query heads' shares, in order
+template <typename T> __global__ void __launch_bounds__(256) sum_shares_kernel(const float *part, T *out, long long values, int group, int width)
+{
+	const long long i = blockIdx.x * 256ll + threadIdx.x; // [bs][n][kv_heads][width]
+	if (i >= values)
+		return;
+	const float *from = part + i / width * group * width + i % width;
+	float sum = 0.f;
+	for (int g = 0; g < group; g++)
+		sum += from[(long long)g * width];
+	out[i] = from_float<T>(sum);
+}
+
+template <typename T> int sum_shares(const MaskedArgs &a, const float *shares, void *dk, void *dv, cudaStream_t st)
+{
+	const long long rows = (long long)a.bs * a.n * a.kv_heads;
+	for (int i = 0; i < 2; i++) {
+		const int width = i ? a.v_width : a.width;
+		const long long blocks = (rows * width + 255) / 256;
+		if (blocks > 0x7fffffffll)
+			return L1ATTN_ERR_SHAPE;
+		sum_shares_kernel<<<unsigned(blocks), 256, 0, st>>>(shares + (i ? (long long)a.bs * a.n * a.heads * a.width : 0), static_cast<T *>(i ? dv : dk), rows * width,
+								     a.heads / a.kv_heads, width);
+		L1B_LAUNCH_CHECK();
+	}
+	return L1ATTN_OK;
+}
+
 size_t pad256(size_t x) { return (x + 255) / 256 * 256; }
 size_t ranges_bytes(int bs, int n) { return pad256(size_t(bs) * ((n + DOC_TILE - 1) / DOC_TILE) * sizeof(DocRange)); }
 
@@ -127,7 +155,7 @@ struct BackwardWork {
 		const long long units = mma ? masked_units_at_once(bs, n, heads) : 0;
 		delta = ranges_bytes(bs, n);
 		shares = delta + pad256(rows * sizeof(float));
-		e = shares + (mma && heads != kv_heads ? pad256(rows * (width + v_width) * sizeof(float)) : 0);
+		e = shares + (heads != kv_heads ? pad256(rows * (width + v_width) * sizeof(float)) : 0);
 		keeps_e = units > 0;
 		bytes = e + size_t(units) * masked_unit_floats(n) * sizeof(float);
 	}
@@ -187,7 +215,10 @@ extern "C" int l1attn_masked_bwd(const void *q, const void *k, const void *v, co
 	else
 		launch_delta<__nv_bfloat16>(a, dvo, vo, delta, rows, st);
 	L1B_LAUNCH_CHECK();
-	if (masked_mma_fits(width, v_width, dtype))
-		return masked_mma_bwd_launch(a, dvo, lse, delta, dq, dk, dv, shares, e, dtype, st);
-	return masked_simple_bwd_launch(a, dvo, lse, delta, dq, dk, dv, dtype, st);
+	rc = masked_mma_fits(width, v_width, dtype) ? masked_mma_bwd_launch(a, dvo, lse, delta, dq, dk, dv, shares, e, dtype, st) :
+						      masked_simple_bwd_launch(a, dvo, lse, delta, dq, dk, dv, shares, dtype, st);
+	if (rc || n_heads == n_kv_heads)
+		return rc;
+	return dtype == L1ATTN_F32 ? sum_shares<float>(a, shares, dk, dv, st) : dtype == L1ATTN_F16 ? sum_shares<__half>(a, shares, dk, dv, st) :
+												     sum_shares<__nv_bfloat16>(a, shares, dk, dv, st);
 }

@@ -979,20 +979,6 @@ __global__ void __launch_bounds__(THREADS, 3) masked_dq_mma_kernel(MaskedArgs a,
 			exact_gradient_row<T, false>(a, mask, b, head, o0 + 16 * warp + r, dvo, lse, delta, dq, dq);
 }
 
-// dk and dv of shared heads: the query heads' shares, in order
-template <typename T> __global__ void __launch_bounds__(256) sum_shares_kernel(const float *part, T *out, long long rows, int group, int width)
-{
-	const long long i = blockIdx.x * 256ll + threadIdx.x; // [bs][n][kv_heads][width]
-	if (i >= rows * width)
-		return;
-	const long long row = i / width;
-	const float *from = part + row * group * width + i % width;
-	float sum = 0.f;
-	for (int g = 0; g < group; g++)
-		sum += from[(long long)g * width];
-	out[i] = from_float<T>(sum);
-}
-
 template <typename T, int W, int V>
 int bwd(const MaskedArgs &a, const void *dvo_, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, float *e, int vec, cudaStream_t st)
 {
@@ -1003,8 +989,8 @@ int bwd(const MaskedArgs &a, const void *dvo_, const float *lse, const float *de
 	static_assert(2 * STREAM * KP >= ROWS * 4 * W, "own rows pass through the stages");
 	const T *dvo = static_cast<const T *>(dvo_);
 	const int tiles = (a.n + ROWS - 1) / ROWS, group = a.heads / a.kv_heads;
-	const long long all = (long long)a.bs * a.heads, rows = (long long)a.bs * a.n * a.kv_heads;
-	if (all * tiles > 0x7fffffffll || rows * (a.width > a.v_width ? a.width : a.v_width) / 256 >= 0x7fffffffll)
+	const long long all = (long long)a.bs * a.heads;
+	if (all * tiles > 0x7fffffffll)
 		return L1ATTN_ERR_SHAPE;
 	BackwardParts parts = {0, int(all), e, masked_unit_floats(a.n), int((a.n + 63ll) / 64 * 64), nullptr, nullptr};
 	if (group > 1) {
@@ -1026,12 +1012,6 @@ int bwd(const MaskedArgs &a, const void *dvo_, const float *lse, const float *de
 			L1B_SHARED_MEMORY((masked_bwd_mma_kernel<T, false, W, V>), bytes);
 			masked_bwd_mma_kernel<T, false, W, V><<<grid, THREADS, bytes, st>>>(a, dvo, lse, delta, static_cast<T *>(dq), nullptr, parts, tiles, vec);
 		}
-		L1B_LAUNCH_CHECK();
-	}
-	if (group > 1) {
-		sum_shares_kernel<<<unsigned((rows * a.width + 255) / 256), 256, 0, st>>>(parts.dk, static_cast<T *>(dk), rows, group, a.width);
-		L1B_LAUNCH_CHECK();
-		sum_shares_kernel<<<unsigned((rows * a.v_width + 255) / 256), 256, 0, st>>>(parts.dv, static_cast<T *>(dv), rows, group, a.v_width);
 		L1B_LAUNCH_CHECK();
 	}
 	return L1ATTN_OK;

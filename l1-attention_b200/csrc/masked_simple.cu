@@ -1,10 +1,11 @@
 // Masked L1 attention (mask.cuh), float32 arithmetic for every storage type and widths up to 256.
 //
-// Forward: a CTA owns 64 query rows of one head; keys and values stream in tiles of 64, all operands as floats in shared memory.  256
-// threads, a 4 x 4 tile of scores each (rows 4 ty + i, keys tx + 16 j); the 16 lanes of a half-warp own their four rows, so the running maximum
-// and sum (one pass over the keys) and the weights never leave the half-warp.  Bound: FP32 instructions, two per term of the distance.
-// Backward: two kernels without atomics.  One owns 64 query rows and makes dq, the other 64 key rows and makes dk and dv (summed
-// over the query heads that share them, in order); both recompute the weights from the log-normalisers and stream the other side in
+// Forward: a CTA owns 64 query rows of one head; keys and values stream in tiles of 64 (32), all operands as floats in shared memory.  256
+// threads, a 4 x 4 (4 x 2) tile of scores each (rows 4 ty + i, keys tx + 16 j); the 16 lanes of a half-warp own their four rows, so the running maximum
+// and sum (one pass over the keys) and the weights never leave the half-warp.  Bound: FP32 instructions -- two per term of the distance, one per term
+// of a product -- and, at 12 terms per clock and SM ([4,2048,8,128], no mask: 5.05 ms), the loads of the tiles, which nothing hides.
+// Backward: two kernels without atomics.  One owns 64 query rows and makes dq, the other 64 key rows of one query head and makes its share of dk and dv;
+// both recompute the weights from the log-normalisers and stream the other side in
 // tiles of 32.  sign(0) = 0.
 #include "mask.cuh"
 
@@ -12,7 +13,7 @@ namespace l1b {
 
 namespace {
 
-constexpr int OWN = 64, KEYS = 64, STREAM = 32, THREADS = 256;
+constexpr int OWN = 64, STREAM = 32, THREADS = 256;
 
 // floats of a row of `w` values: whole float4s, an odd number of them so that 8 rows at one column lie in different banks
 __host__ __device__ inline int pitch(int w)
@@ -97,7 +98,7 @@ template <int J> __device__ __forceinline__ void products(const float *A, const 
 	}
 }
 
-template <typename T, int NV> __global__ void __launch_bounds__(THREADS) masked_fwd_simple_kernel(MaskedArgs a, T *vo, float *lse, int tiles)
+template <typename T, int NV, int KEYS> __global__ void __launch_bounds__(THREADS) masked_fwd_simple_kernel(MaskedArgs a, T *vo, float *lse, int tiles)
 {
 	extern __shared__ float4 smem4[];
 	const int wp = pitch(a.width), vp = 64 * NV, tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
@@ -127,14 +128,15 @@ template <typename T, int NV> __global__ void __launch_bounds__(THREADS) masked_
 		__syncthreads();
 		load_rows<T>(K, wp, wp, a.k, b, kv, s0, KEYS, a.n, a.width);
 		const bool odd = __syncthreads_or(load_rows<T>(V, vp, vp, a.v, b, kv, s0, KEYS, a.n, a.v_width));
-		float x[4][4];
-		distances<4>(Q, K, wp, a.width, ty, tx, x);
+		constexpr int J = KEYS / 16;
+		float x[4][J];
+		distances<J>(Q, K, wp, a.width, ty, tx, x);
 #pragma unroll
 		for (int i = 0; i < 4; i++) {
 			const int t = t0 + 4 * ty + i;
 			float top = m[i];
 #pragma unroll
-			for (int j = 0; j < 4; j++) {
+			for (int j = 0; j < J; j++) {
 				const int s = s0 + tx + 16 * j;
 				float y = -a.scale * x[i][j];
 				if (a.cap > 0.f)
@@ -147,7 +149,7 @@ template <typename T, int NV> __global__ void __launch_bounds__(THREADS) masked_
 			const float ref = top == -INFINITY ? 0.f : top, keep = expf(m[i] - ref);
 			float sum = 0.f;
 #pragma unroll
-			for (int j = 0; j < 4; j++) {
+			for (int j = 0; j < J; j++) {
 				const float p = expf(x[i][j] - ref);
 				sum += p;
 				P[(4 * ty + i) * PP + tx + 16 * j] = p;
@@ -198,102 +200,107 @@ template <typename T, int NV> __global__ void __launch_bounds__(THREADS) masked_
 	}
 }
 
-// OWN_KEYS: a CTA owns 64 keys of one key-value head and makes their dk and dv; else 64 queries of one head, dq.
-template <typename T, bool OWN_KEYS, int NW, int NV>
-__global__ void __launch_bounds__(THREADS) masked_bwd_simple_kernel(MaskedArgs a, const T *dvo, const float *lse, const float *delta, T *dq, T *dk, T *dv, int tiles)
+// sum += sign(a - b) e, minus = -e: two compares and two predicated additions (left to the compiler, selections: 21.4 instead of 19.4 ms for
+// [4,2048,8,128] without a mask)
+__device__ __forceinline__ void add_by_sign(float &sum, float a, float b, float e, float minus)
+{
+	asm("{\n\t.reg .pred p, q;\n\t"
+	    "setp.gt.f32 p, %1, %2;\n\t"
+	    "setp.lt.f32 q, %1, %2;\n\t"
+	    "@p add.f32 %0, %0, %3;\n\t"
+	    "@q add.f32 %0, %0, %4;\n\t}"
+	    : "+f"(sum)
+	    : "f"(a), "f"(b), "f"(e), "f"(minus));
+}
+
+// OWN_KEYS: a CTA owns 64 keys of one query head and makes its share of their dk and dv; else 64 queries, dq.  A thread owns the columns tx + 16 c of
+// four own rows, c < NW (NV), its own values in registers: a streamed row costs a 4-byte load a column and one 16-byte load of the four rows' e.
+// OUT: T, or float for the shares of shared heads.
+template <typename T, typename OUT, bool OWN_KEYS, int NW, int NV>
+__global__ void __launch_bounds__(THREADS, NW >= 6 ? 1 : 0) masked_bwd_simple_kernel(MaskedArgs a, const T *dvo, const float *lse, const float *delta, OUT *dx, OUT *dv, int tiles)
 {
 	extern __shared__ float4 smem4[];
-	const int wp = pitch(64 * NW), vp = pitch(64 * NV), tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
-	constexpr int GP = STREAM + 4;
-	float *A = reinterpret_cast<float *>(smem4), *B = A + OWN * wp, *C = B + OWN * vp, *D = C + STREAM * wp, *G = D + STREAM * vp, *P = G + OWN * GP;
-	const int own_heads = OWN_KEYS ? a.kv_heads : a.heads, group = a.heads / a.kv_heads;
+	const int wp = pitch(a.width), vp = pitch(a.v_width), tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
+	constexpr int GP = OWN + 4;
+	// (columns past a row's pitch read the next row, the last ones' G: what they come to is not stored)
+	float *A = reinterpret_cast<float *>(smem4), *B = A + OWN * wp, *C = B + OWN * vp, *D = C + STREAM * wp, *G = D + STREAM * vp, *P = G + STREAM * GP;
 	const int tile = OWN_KEYS ? int(blockIdx.x % tiles) : tiles - 1 - int(blockIdx.x % tiles);
-	const int own = (blockIdx.x / tiles) % own_heads, b = blockIdx.x / tiles / own_heads;
+	const int head = (blockIdx.x / tiles) % a.heads, b = blockIdx.x / tiles / a.heads, kv = head / (a.heads / a.kv_heads);
 	const MaskView mask(a, b);
 	const int o0 = tile * OWN, o1 = min(a.n, o0 + OWN);
-	const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
+	const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f, slope = a.slopes ? a.slopes[head] : 0.f;
 	const Strided go = {dvo, (long long)a.n * a.heads * a.v_width, (long long)a.heads * a.v_width, a.v_width};
-	load_rows<T>(A, wp, wp, OWN_KEYS ? a.k : a.q, b, own, o0, OWN, a.n, a.width);
-	load_rows<T>(B, vp, vp, OWN_KEYS ? a.v : go, b, own, o0, OWN, a.n, a.v_width);
-	float acc[4][4 * NW], accv[4][OWN_KEYS ? 4 * NV : 1];
+	load_rows<T>(A, wp, wp, OWN_KEYS ? a.k : a.q, b, OWN_KEYS ? kv : head, o0, OWN, a.n, a.width);
+	load_rows<T>(B, vp, vp, OWN_KEYS ? a.v : go, b, OWN_KEYS ? kv : head, o0, OWN, a.n, a.v_width);
+	__syncthreads();
+	float own[4][NW], acc[4][NW], accv[4][OWN_KEYS ? NV : 1];
 #pragma unroll
 	for (int i = 0; i < 4; i++) {
 #pragma unroll
-		for (int c = 0; c < 4 * NW; c++)
+		for (int c = 0; c < NW; c++) {
+			own[i][c] = A[(4 * ty + i) * wp + tx + 16 * c];
 			acc[i][c] = 0.f;
+		}
 #pragma unroll
-		for (int c = 0; c < (OWN_KEYS ? 4 * NV : 1); c++)
+		for (int c = 0; c < (OWN_KEYS ? NV : 1); c++)
 			accv[i][c] = 0.f;
 	}
-	for (int g = 0; g < (OWN_KEYS ? group : 1); g++) {
-		const int head = OWN_KEYS ? own * group + g : own;
-		const float slope = a.slopes ? a.slopes[head] : 0.f;
-		for (int r0 = 0; r0 < a.n; r0 += STREAM) {
-			const int r1 = min(a.n, r0 + STREAM);
-			if (OWN_KEYS ? !mask.any(r0, r1, o0, o1) : !mask.any(o0, o1, r0, r1))
-				continue;
-			__syncthreads();
-			load_rows<T>(C, wp, wp, OWN_KEYS ? a.q : a.k, b, OWN_KEYS ? head : own / group, r0, STREAM, a.n, a.width);
-			const bool odd = __syncthreads_or(load_rows<T>(D, vp, vp, OWN_KEYS ? go : a.v, b, OWN_KEYS ? head : own / group, r0, STREAM, a.n, a.v_width));
-			float x[4][2], dp[4][2];
-			distances<2>(A, C, wp, a.width, ty, tx, x);
-			products<2>(B, D, vp, a.v_width, ty, tx, dp);
+	for (int r0 = 0; r0 < a.n; r0 += STREAM) {
+		const int r1 = min(a.n, r0 + STREAM);
+		if (OWN_KEYS ? !mask.any(r0, r1, o0, o1) : !mask.any(o0, o1, r0, r1))
+			continue;
+		__syncthreads();
+		load_rows<T>(C, wp, wp, OWN_KEYS ? a.q : a.k, b, OWN_KEYS ? head : kv, r0, STREAM, a.n, a.width);
+		const bool odd = __syncthreads_or(load_rows<T>(D, vp, vp, OWN_KEYS ? go : a.v, b, OWN_KEYS ? head : kv, r0, STREAM, a.n, a.v_width));
+		constexpr int J = STREAM / 16;
+		float x[4][J], dp[4][J];
+		distances<J>(A, C, wp, a.width, ty, tx, x);
+		products<J>(B, D, vp, a.v_width, ty, tx, dp);
 #pragma unroll
-			for (int i = 0; i < 4; i++)
+		for (int j = 0; j < J; j++) {
+			float e[4], p[4];
 #pragma unroll
-				for (int j = 0; j < 2; j++) {
-					const int o = o0 + 4 * ty + i, r = r0 + tx + 16 * j, t = OWN_KEYS ? r : o, s = OWN_KEYS ? o : r;
-					float p = 0.f, e = 0.f;
-					if (t < a.n && s < a.n && mask.sees(t, s, mask.doc ? mask.doc[t] : 0, mask.doc ? mask.doc[s] : 0)) {
-						const long long row = ((long long)b * a.n + t) * a.heads + head;
-						float y = -a.scale * x[i][j], slant = 1.f;
-						if (a.cap > 0.f) {
-							const float th = tanhf(y * inv_cap);
-							slant = 1.f - th * th;
-							y = a.cap * th;
-						}
-						p = weight_of(y - slope * fabsf(float(t - s)), lse[row]);
-						if (p != 0.f)
-							e = -a.scale * slant * p * (dp[i][j] - delta[row]);
+			for (int i = 0; i < 4; i++) {
+				const int o = o0 + 4 * ty + i, r = r0 + tx + 16 * j, t = OWN_KEYS ? r : o, s = OWN_KEYS ? o : r;
+				p[i] = e[i] = 0.f;
+				if (t < a.n && s < a.n && mask.sees(t, s, mask.doc ? mask.doc[t] : 0, mask.doc ? mask.doc[s] : 0)) {
+					const long long row = ((long long)b * a.n + t) * a.heads + head;
+					float y = -a.scale * x[i][j], slant = 1.f;
+					if (a.cap > 0.f) {
+						const float th = tanhf(y * inv_cap);
+						slant = 1.f - th * th;
+						y = a.cap * th;
 					}
-					G[(4 * ty + i) * GP + tx + 16 * j] = e;
-					if (OWN_KEYS)
-						P[(4 * ty + i) * GP + tx + 16 * j] = p;
+					p[i] = weight_of(y - slope * fabsf(float(t - s)), lse[row]);
+					if (p[i] != 0.f)
+						e[i] = -a.scale * slant * p[i] * (dp[i][j] - delta[row]);
 				}
-			__syncwarp();
-			for (int r = 0; r < r1 - r0; r++) {
-				float e[4], p[4];
+			}
+			*reinterpret_cast<float4 *>(G + (tx + 16 * j) * GP + 4 * ty) = make_float4(e[0], e[1], e[2], e[3]);
+			if (OWN_KEYS)
+				*reinterpret_cast<float4 *>(P + (tx + 16 * j) * GP + 4 * ty) = make_float4(p[0], p[1], p[2], p[3]);
+		}
+		__syncwarp(); // (a half-warp's rows are its own)
+		for (int r = 0; r < r1 - r0; r++) {
+			const float4 e4 = *reinterpret_cast<const float4 *>(G + r * GP + 4 * ty);
+			const float e[4] = {e4.x, e4.y, e4.z, e4.w}, minus[4] = {-e4.x, -e4.y, -e4.z, -e4.w};
 #pragma unroll
-				for (int i = 0; i < 4; i++) {
-					e[i] = G[(4 * ty + i) * GP + r];
-					p[i] = OWN_KEYS ? P[(4 * ty + i) * GP + r] : 0.f;
-				}
+			for (int c = 0; c < NW; c++) {
+				const float y = C[r * wp + tx + 16 * c];
 #pragma unroll
-				for (int u = 0; u < NW; u++) {
-					const float4 y = *reinterpret_cast<const float4 *>(C + r * wp + 64 * u + 4 * tx);
+				for (int i = 0; i < 4; i++)
+					add_by_sign(acc[i][c], own[i][c], y, e[i], minus[i]);
+			}
+			if (OWN_KEYS) {
+				const float4 p4 = *reinterpret_cast<const float4 *>(P + r * GP + 4 * ty);
+				const float p[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
-					for (int i = 0; i < 4; i++) {
-						const float4 z = *reinterpret_cast<const float4 *>(A + (4 * ty + i) * wp + 64 * u + 4 * tx);
-						acc[i][4 * u] += sign_apply(z.x - y.x, e[i]);
-						acc[i][4 * u + 1] += sign_apply(z.y - y.y, e[i]);
-						acc[i][4 * u + 2] += sign_apply(z.z - y.z, e[i]);
-						acc[i][4 * u + 3] += sign_apply(z.w - y.w, e[i]);
-					}
-				}
-				if (OWN_KEYS) {
+				for (int c = 0; c < NV; c++) {
+					const float y = D[r * vp + tx + 16 * c];
 #pragma unroll
-					for (int u = 0; u < NV; u++) {
-						const float4 y = *reinterpret_cast<const float4 *>(D + r * vp + 64 * u + 4 * tx);
-#pragma unroll
-						for (int i = 0; i < 4; i++) {
-							if (odd && p[i] == 0.f)
-								continue;
-							accv[i][(4 * u) % (OWN_KEYS ? 4 * NV : 1)] += p[i] * y.x;
-							accv[i][(4 * u + 1) % (OWN_KEYS ? 4 * NV : 1)] += p[i] * y.y;
-							accv[i][(4 * u + 2) % (OWN_KEYS ? 4 * NV : 1)] += p[i] * y.z;
-							accv[i][(4 * u + 3) % (OWN_KEYS ? 4 * NV : 1)] += p[i] * y.w;
-						}
-					}
+					for (int i = 0; i < 4; i++)
+						if (!odd || p[i] != 0.f)
+							accv[i][c % (OWN_KEYS ? NV : 1)] = fmaf(p[i], y, accv[i][c % (OWN_KEYS ? NV : 1)]);
 				}
 			}
 		}
@@ -303,20 +310,16 @@ __global__ void __launch_bounds__(THREADS) masked_bwd_simple_kernel(MaskedArgs a
 		const int o = o0 + 4 * ty + i;
 		if (o >= a.n)
 			continue;
-		const long long row = ((long long)b * a.n + o) * own_heads + own;
+		const long long row = ((long long)b * a.n + o) * a.heads + head;
 #pragma unroll
-		for (int c = 0; c < 4 * NW; c++) {
-			const int w = 64 * (c / 4) + 4 * tx + c % 4;
-			if (w < a.width)
-				(OWN_KEYS ? dk : dq)[row * a.width + w] = from_float<T>(acc[i][c]);
-		}
+		for (int c = 0; c < NW; c++)
+			if (tx + 16 * c < a.width)
+				dx[row * a.width + tx + 16 * c] = from_float<OUT>(acc[i][c]);
 		if (OWN_KEYS)
 #pragma unroll
-			for (int c = 0; c < (OWN_KEYS ? 4 * NV : 1); c++) {
-				const int w = 64 * (c / 4) + 4 * tx + c % 4;
-				if (w < a.v_width)
-					dv[row * a.v_width + w] = from_float<T>(accv[i][c]);
-			}
+			for (int c = 0; c < NV; c++)
+				if (tx + 16 * c < a.v_width)
+					dv[row * a.v_width + tx + 16 * c] = from_float<OUT>(accv[i][c % (OWN_KEYS ? NV : 1)]);
 	}
 }
 
@@ -328,51 +331,74 @@ int grid_of(long long n, unsigned *out)
 	return L1ATTN_OK;
 }
 
-template <typename T, int NV> int fwd(const MaskedArgs &a, void *vo, float *lse, cudaStream_t st)
+inline int fwd_bytes(int width, int nv, int keys) { return 4 * ((OWN + keys) * pitch(width) + keys * 64 * nv + OWN * (keys + 4)); }
+
+template <typename T, int NV, int KEYS> int fwd_tiles(const MaskedArgs &a, void *vo, float *lse, cudaStream_t st)
 {
-	const int tiles = (a.n + OWN - 1) / OWN, bytes = 4 * (OWN * pitch(a.width) + KEYS * pitch(a.width) + KEYS * 64 * NV + OWN * (KEYS + 4));
+	const int tiles = (a.n + OWN - 1) / OWN, bytes = fwd_bytes(a.width, NV, KEYS);
 	unsigned grid = 0;
 	if (int rc = grid_of((long long)tiles * a.heads * a.bs, &grid))
 		return rc;
-	L1B_SHARED_MEMORY((masked_fwd_simple_kernel<T, NV>), bytes);
-	masked_fwd_simple_kernel<T, NV><<<grid, THREADS, bytes, st>>>(a, static_cast<T *>(vo), lse, tiles);
+	L1B_SHARED_MEMORY((masked_fwd_simple_kernel<T, NV, KEYS>), bytes);
+	masked_fwd_simple_kernel<T, NV, KEYS><<<grid, THREADS, bytes, st>>>(a, static_cast<T *>(vo), lse, tiles);
 	L1B_LAUNCH_CHECK();
 	return L1ATTN_OK;
 }
 
-template <typename T, bool OWN_KEYS, int NW, int NV>
-int bwd_one(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, cudaStream_t st)
+// Tiles of 64 keys where two CTAs of them fit an SM, else of 32: [4,2048,8,128], no mask, 5.05 against 7.66 ms; but [2,2048,8,64], causal, 0.99 / 0.84, and
+// [3,501,6,65] with values of 40 169 / 143 us.
+template <typename T, int NV> int fwd(const MaskedArgs &a, void *vo, float *lse, cudaStream_t st)
 {
-	const int wp = pitch(64 * NW), vp = pitch(64 * NV);
-	const int tiles = (a.n + OWN - 1) / OWN, bytes = 4 * ((OWN + STREAM) * (wp + vp) + (OWN_KEYS ? 2 : 1) * OWN * (STREAM + 4));
+	return fwd_bytes(a.width, NV, 64) <= 113 * 1024 ? fwd_tiles<T, NV, 64>(a, vo, lse, st) : fwd_tiles<T, NV, 32>(a, vo, lse, st);
+}
+
+template <typename T, typename OUT, bool OWN_KEYS, int NW, int NV>
+int bwd_one(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, OUT *dx, OUT *dv, cudaStream_t st)
+{
+	const int tiles = (a.n + OWN - 1) / OWN;
+	const int bytes = 4 * ((OWN + STREAM) * (pitch(a.width) + pitch(a.v_width)) + (OWN_KEYS ? 2 : 1) * STREAM * (OWN + 4)); // (G alone takes in what is read past C and D)
 	unsigned grid = 0;
-	if (int rc = grid_of((long long)tiles * (OWN_KEYS ? a.kv_heads : a.heads) * a.bs, &grid))
+	if (int rc = grid_of((long long)tiles * a.heads * a.bs, &grid))
 		return rc;
-	L1B_SHARED_MEMORY((masked_bwd_simple_kernel<T, OWN_KEYS, NW, NV>), bytes);
-	masked_bwd_simple_kernel<T, OWN_KEYS, NW, NV>
-	    <<<grid, THREADS, bytes, st>>>(a, static_cast<const T *>(dvo), lse, delta, static_cast<T *>(dq), static_cast<T *>(dk), static_cast<T *>(dv), tiles);
+	L1B_SHARED_MEMORY((masked_bwd_simple_kernel<T, OUT, OWN_KEYS, NW, NV>), bytes);
+	masked_bwd_simple_kernel<T, OUT, OWN_KEYS, NW, NV><<<grid, THREADS, bytes, st>>>(a, static_cast<const T *>(dvo), lse, delta, dx, dv, tiles);
 	L1B_LAUNCH_CHECK();
 	return L1ATTN_OK;
 }
 
 template <typename T, int NW, int NV>
-int bwd(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, cudaStream_t st)
+int bwd(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, cudaStream_t st)
 {
-	if (int rc = bwd_one<T, false, NW, NV>(a, dvo, lse, delta, dq, dk, dv, st))
+	if (int rc = bwd_one<T, T, false, NW, NV>(a, dvo, lse, delta, static_cast<T *>(dq), static_cast<T *>(nullptr), st))
 		return rc;
-	return bwd_one<T, true, NW, NV>(a, dvo, lse, delta, dq, dk, dv, st);
+	if (a.heads != a.kv_heads)
+		return bwd_one<T, float, true, NW, NV>(a, dvo, lse, delta, shares, shares + (long long)a.bs * a.n * a.heads * a.width, st);
+	return bwd_one<T, T, true, NW, NV>(a, dvo, lse, delta, static_cast<T *>(dk), static_cast<T *>(dv), st);
 }
 
 template <typename T> int fwd_type(const MaskedArgs &a, void *vo, float *lse, cudaStream_t st)
 {
+	if constexpr (sizeof(T) == 2) // (smaller ones of 16 bits are done on the tensor cores)
+		return fwd<T, 4>(a, vo, lse, st);
+	else
 	return a.v_width <= 64 ? fwd<T, 1>(a, vo, lse, st) : a.v_width <= 128 ? fwd<T, 2>(a, vo, lse, st) : fwd<T, 4>(a, vo, lse, st);
 }
-template <typename T>
-int bwd_type(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, cudaStream_t st)
+// columns a thread, for the width and for the values: 32, 64, 96, 128, 256 columns in all
+template <typename T, int NW>
+int bwd_values(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, cudaStream_t st)
 {
-	const int w = a.width > a.v_width ? a.width : a.v_width;
-	return w <= 64 ? bwd<T, 1, 1>(a, dvo, lse, delta, dq, dk, dv, st) : w <= 128 ? bwd<T, 2, 2>(a, dvo, lse, delta, dq, dk, dv, st) :
-											    bwd<T, 4, 4>(a, dvo, lse, delta, dq, dk, dv, st);
+	return a.v_width <= 64 ? bwd<T, NW, 4>(a, dvo, lse, delta, dq, dk, dv, shares, st) : a.v_width <= 128 ? bwd<T, NW, 8>(a, dvo, lse, delta, dq, dk, dv, shares, st) :
+														       bwd<T, NW, 16>(a, dvo, lse, delta, dq, dk, dv, shares, st);
+}
+template <typename T>
+int bwd_type(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, cudaStream_t st)
+{
+	if constexpr (sizeof(T) == 2) // (smaller ones of 16 bits are done on the tensor cores)
+		return bwd<T, 16, 16>(a, dvo, lse, delta, dq, dk, dv, shares, st);
+	else
+	return a.width <= 32 ? bwd_values<T, 2>(a, dvo, lse, delta, dq, dk, dv, shares, st) : a.width <= 64 ? bwd_values<T, 4>(a, dvo, lse, delta, dq, dk, dv, shares, st) :
+	       a.width <= 96 ? bwd_values<T, 6>(a, dvo, lse, delta, dq, dk, dv, shares, st) : a.width <= 128 ? bwd_values<T, 8>(a, dvo, lse, delta, dq, dk, dv, shares, st) :
+														bwd_values<T, 16>(a, dvo, lse, delta, dq, dk, dv, shares, st);
 }
 
 } // namespace
@@ -383,12 +409,12 @@ int masked_simple_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtyp
 											     fwd_type<__nv_bfloat16>(a, vo, lse, st);
 }
 
-int masked_simple_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, int dtype,
+int masked_simple_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, int dtype,
 			     cudaStream_t st)
 {
-	return dtype == L1ATTN_F32 ? bwd_type<float>(a, dvo, lse, delta, dq, dk, dv, st) :
-	       dtype == L1ATTN_F16 ? bwd_type<__half>(a, dvo, lse, delta, dq, dk, dv, st) :
-				     bwd_type<__nv_bfloat16>(a, dvo, lse, delta, dq, dk, dv, st);
+	return dtype == L1ATTN_F32 ? bwd_type<float>(a, dvo, lse, delta, dq, dk, dv, shares, st) :
+	       dtype == L1ATTN_F16 ? bwd_type<__half>(a, dvo, lse, delta, dq, dk, dv, shares, st) :
+				     bwd_type<__nv_bfloat16>(a, dvo, lse, delta, dq, dk, dv, shares, st);
 }
 
 } // namespace l1b
