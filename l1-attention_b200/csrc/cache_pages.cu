@@ -14,7 +14,7 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
 // x / s to the nearest whole number, ties to even, of the exact quotient: an estimate, put right by its residual, which one FMA gives
 // exactly where it decides (it is a multiple of the smaller last bit and at most about s).  NaN is stored as 0, values beyond as +-127.
-__device__ __forceinline__ int quantise(float x, float s, float inv)
+__device__ __noinline__ int quantise_any(float x, float s, float inv)
 {
 	if (!finite(x) || s == 0.f)
 		return x > 0.f && s > 0.f ? 127 : x < 0.f && s > 0.f ? -127 : 0;
@@ -23,6 +23,13 @@ __device__ __forceinline__ int quantise(float x, float s, float inv)
 	if (r2 > s || (r2 == s && (int(q) & 1)))
 		q += copysignf(1.f, r);
 	return int(fminf(fmaxf(q, -127.f), 127.f));
+}
+// The low byte of the same.  1.5 * 2^23 leaves the whole number in the low bits of the sum; where the residual says that it is the nearest for sure
+// (almost always), that is all.
+__device__ __forceinline__ uint32_t quantise(float x, float s, float inv)
+{
+	const float t = fmaf(x, inv, 12582912.f), r = fmaf(12582912.f - t, s, x);
+	return (fabsf(r + r) < s ? __float_as_uint(t) : uint32_t(quantise_any(x, s, inv))) & 0xffu;
 }
 
 template <typename T> struct Vector { // 16 bytes of tokens
@@ -101,7 +108,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(CacheArgs c, const T *k
 			uint32_t out[N / 4];
 #pragma unroll
 			for (int e = 0; e < N; e++) {
-				const uint32_t q = uint32_t(quantise(to_float(reinterpret_cast<const T *>(&held[j])[e]), now, inv)) & 0xffu;
+				const uint32_t q = quantise(to_float(reinterpret_cast<const T *>(&held[j])[e]), now, inv);
 				out[e / 4] = e % 4 ? out[e / 4] | q << 8 * (e % 4) : q;
 			}
 			int8_t *const to = codes + (long long)a * w + i * N;
@@ -117,14 +124,14 @@ __global__ void __launch_bounds__(THREADS) append_kernel(CacheArgs c, const T *k
 		*scale = now;
 }
 
-// A warp per row and group of heads: keys and values of the row, 16 bytes of codes at a time where widths allow it (VEC), else one by one.
+// A warp per row: its keys and values, 16 bytes of them at a time where widths allow it (VEC), else one by one.
 template <typename T, bool VEC> __global__ void __launch_bounds__(THREADS) gather_kernel(CacheArgs c, T *k, T *v)
 {
 	const long long row = blockIdx.x * (long long)(THREADS / 32) + threadIdx.x / 32;
 	const int lane = threadIdx.x % 32;
 	if (row >= c.rows)
 		return;
-	const int seq = cache_find_row(c, row);
+	const int seq = cache_find_warp(c, row, 1, 1, 0);
 	const SeqView sv = cache_seq(c, seq);
 	if (row < sv.row || row - sv.row >= sv.count)
 		return;
@@ -137,18 +144,24 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(THREADS) gathe
 		T *const out = (values ? v : k) + row * c.kv_heads * w;
 		const long long head = (long long)c.page * w;
 		if (VEC) {
-			const int per_head = w / 16;
+			constexpr int N = Vector<T>::N;
+			const int per_head = w / N;
+#pragma unroll 4
 			for (int i = lane; i < c.kv_heads * per_head; i += 32) {
 				const int h = i / per_head;
-				const uint4 x = id < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4 *>(codes + h * head + i % per_head * 16);
-				const float s = id < 0 ? 0.f : scale[h];
-				alignas(16) T y[16];
+				const int8_t *const from = codes + h * head + i % per_head * N;
+				uint32_t x[N / 4];
+				if constexpr (N == 8) {
+					const uint2 y = *reinterpret_cast<const uint2 *>(from);
+					x[0] = y.x, x[N / 4 - 1] = y.y;
+				} else
+					x[0] = *reinterpret_cast<const uint32_t *>(from);
+				const float s = scale[h];
+				uint4 y;
 #pragma unroll
-				for (int e = 0; e < 16; e++)
-					y[e] = from_float<T>(float(reinterpret_cast<const int8_t *>(&x)[e]) * s);
-#pragma unroll
-				for (int e = 0; e < int(sizeof(T)); e++)
-					reinterpret_cast<uint4 *>(out + i * 16)[e] = reinterpret_cast<const uint4 *>(y)[e];
+				for (int e = 0; e < N; e++) // (a page out of range: zeros, whatever has been read)
+					reinterpret_cast<T *>(&y)[e] = from_float<T>(id < 0 ? 0.f : float(int8_t(x[e / 4] >> 8 * (e % 4))) * s);
+				reinterpret_cast<uint4 *>(out)[i] = y;
 			}
 		} else
 			for (int i = lane; i < c.kv_heads * w; i += 32)
@@ -233,7 +246,8 @@ int gather_launch(const CacheArgs &c, void *k, void *v, int dtype, cudaStream_t 
 	const long long blocks = ((long long)c.rows + THREADS / 32 - 1) / (THREADS / 32);
 	if (blocks > 0x7fffffffll)
 		return L1ATTN_ERR_SHAPE;
-	const bool vec = c.width % 16 == 0 && c.v_width % 16 == 0 && aligned(k, 16) && aligned(v, 16);
+	const int n = dtype == L1ATTN_F32 ? 4 : 8;
+	const bool vec = c.width % n == 0 && c.v_width % n == 0 && aligned(k, 16) && aligned(v, 16);
 	auto launch = [&](auto *k_, auto *v_) {
 		if (vec)
 			gather_kernel<std::remove_pointer_t<decltype(k_)>, true><<<unsigned(blocks), THREADS, 0, st>>>(c, k_, v_);
