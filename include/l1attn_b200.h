@@ -204,7 +204,7 @@ typedef struct l1attn_mask {
  * kept).  work: device memory of l1attn_masked_work_bytes() bytes, 256-byte aligned (the forward uses it only with documents and takes NULL
  * without); nothing in it needs to be initialised or outlives the call, and calls that share it must not overlap on the GPU.
  * The backward in 16 bits with widths up to 128 keeps gradients of the distances there, up to a gigabyte at once (a float per pair and query head of a
- * batch item; none beyond 16384 tokens).  Sums, weights and their normalisers are float32 in every case.  The backward is deterministic.
+ * batch item; none beyond 16384 tokens).  Sums and normalisers are float32 in every case.  The backward is deterministic.  n_tok: up to 2^30.
  */
 size_t l1attn_masked_work_bytes(int bs, int n_tok, int n_heads, int n_kv_heads, int width, int v_width, int dtype, int backward);
 int l1attn_masked_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *vo, float *lse, void *work,
@@ -221,7 +221,7 @@ int l1attn_masked_bwd(const void *q, const void *k, const void *v, const int64_t
  * A paged cache of keys and values in 8 bits (no counterpart in the reference).  A page holds `page` consecutive tokens of one sequence, for
  * all heads; the tokens of a page share one float scale per head, for keys and for values: value = scale * code, codes -127 .. 127.
  *   k_codes [n_pages][n_kv_heads][page][width], v_codes [n_pages][n_kv_heads][page][v_width], k_scale, v_scale [n_pages][n_kv_heads]
- * page: 16, 32, 64, 128 or 256; widths 1 .. 256; codes 16-byte aligned.
+ * page: 16, 32, 64, 128 or 256; widths 1 .. 256; one page or more; max_pages * page up to 2^30; codes 16-byte aligned.
  * Calls take some sequences at once.  Sequence i's rows of the token tensors are [cu[i], cu[i+1]) and stand at its positions start[i],
  * start[i] + 1, ...; its position p is in page table[i][p / page].  Rows behind cu[n_seqs] belong to no sequence: nothing reads or writes them.
  * table, start and cu are device memory and may change between replays of a captured call.  Entries of table past a sequence's last page
@@ -257,7 +257,7 @@ int l1attn_cache_copy_pages(const l1attn_cache *cache, int layers, const int32_t
 /*
  * Attention of q [rows][n_heads][width] (n_heads a multiple of n_kv_heads; strides: row and head) to the cache: each row sees the keys at its own and
  * earlier positions of its sequence, scored, capped, biased, windowed and normalised as l1attn_mask says (causal must be 1, doc and prefix NULL);
- * vo [rows][n_heads][v_width] contiguous.  max_len: the longest start + count that the caller knows of; it shapes the launch alone, any value gives
+ * vo [rows][n_heads][v_width] contiguous, not over q; rows * n_heads up to 2^31.  max_len: the longest start + count that the caller knows of; it shapes the launch alone, any value gives
  * right results.  work: device memory of l1attn_cache_attend_bytes() bytes for the same sizes, 256-byte aligned, as in l1attn_masked_fwd.
  */
 size_t l1attn_cache_attend_bytes(const l1attn_cache *cache, int rows, int n_heads, int max_len, int dtype);

@@ -8,7 +8,7 @@ namespace {
 
 int check(const l1attn_cache *c, int rows, int dtype, bool tokens, CacheArgs *out)
 {
-	if (!c || rows < 0 || c->n_pages < 0 || c->n_kv_heads < 1 || c->width < 1 || c->v_width < 1)
+	if (!c || rows < 0 || c->n_pages < 1 || c->n_kv_heads < 1 || c->width < 1 || c->v_width < 1)
 		return L1ATTN_ERR_ARG;
 	if (dtype != L1ATTN_F32 && dtype != L1ATTN_F16 && dtype != L1ATTN_BF16)
 		return L1ATTN_ERR_ARG;
@@ -23,7 +23,7 @@ int check(const l1attn_cache *c, int rows, int dtype, bool tokens, CacheArgs *ou
 	if (tokens) {
 		if (c->n_seqs < 0 || c->max_pages < 0)
 			return L1ATTN_ERR_ARG;
-		if ((long long)c->max_pages * c->page > 0x7fffffffll)
+		if ((long long)c->max_pages * c->page > 1 << 30) // (positions and tile ends stay within int)
 			return L1ATTN_ERR_SHAPE;
 		if (rows == 0 || c->n_seqs == 0)
 			return 1; // nothing to do
@@ -42,6 +42,8 @@ int plan(AttendArgs *a, int rows, int heads, int max_len, int dtype, size_t *byt
 {
 	a->heads = heads;
 	a->group = heads / a->c.kv_heads;
+	if ((long long)rows * heads > 0x7fffffffll)
+		return L1ATTN_ERR_SHAPE;
 	const size_t part = (a->c.v_width + 2) * sizeof(float);
 	if (attend_mma_fits(a->c.width, a->c.v_width, dtype)) { // one wave of CTAs that share the chunks; at least 16 chunks each
 		// eight rows cost half of sixteen; sequences of one token have as many rows as a group has heads
@@ -51,8 +53,6 @@ int plan(AttendArgs *a, int rows, int heads, int max_len, int dtype, size_t *byt
 			return rc;
 		a->ctas = attend_mma_ctas(a->tile_rows, sms);
 		a->least = 16;
-		if ((long long)rows * a->group > 0x7fffffffll - 16)
-			return L1ATTN_ERR_SHAPE;
 		a->splits = 1;
 		*bytes = (2ull * a->ctas * a->tile_rows * part + 255) / 256 * 256 + a->ctas * sizeof(AttendSplit);
 		return L1ATTN_OK;

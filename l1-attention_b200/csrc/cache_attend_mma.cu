@@ -247,7 +247,7 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 			fetch(k);
 
 		int page_before = -2;
-		float k_unit = 0.f, v_unit = 0.f, q_part[TILES][2]; // k_unit: 2 scale s (log2 e); v_unit: power of two that value scales are taken relative to; q_part: of the score
+		float k_unit = 0.f, v_unit = 0.f, q_part[TILES][2]; // k_unit: 2 scale s (log2 e); v_unit: power of two that value scales are taken relative to (2^6 more, so that weights far below the largest keep bits; at most 2^15 then); q_part: of the score
 		for (int k = 0; k < chunks; k++) {
 			if (k && k % 32 == 0)
 				look_up(k / 32 + 1);
@@ -305,9 +305,9 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 					for (int b = 0; b < 2; b++)
 						q_part[i][b] = -0.5f * k_unit * sum[b] - a.scale * (straight ? LOG2E : 1.f) * (clips ? rest[8 * i + 2 * j + b] : 0.f);
 				}
-				if (vs * v_unit > 2.f || v_unit == 0.f) { // (a power of two from the first scale that is not zero; larger ones take it along)
-					const int e = min(max(int(__float_as_uint(vs) >> 23), 1), 253);
-					const float now = vs > 0.f ? __uint_as_float(uint32_t(254 - e) << 23) : 0.f, keep = v_unit == 0.f ? 0.f : now / v_unit;
+				if (vs * v_unit > 128.f || v_unit == 0.f) { // (a power of two from the first scale that is not zero; larger ones take it along)
+					const int e = min(max(int(__float_as_uint(vs) >> 23), 7), 253);
+					const float now = vs > 0.f ? __uint_as_float(uint32_t(260 - e) << 23) : 0.f, keep = v_unit == 0.f ? 0.f : now / v_unit;
 					v_unit = now;
 #pragma unroll
 					for (int i = 0; i < TILES * 2 * VG * 4; i++)

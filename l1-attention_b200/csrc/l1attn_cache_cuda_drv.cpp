@@ -66,7 +66,7 @@ l1attn_cache places(const std::vector<torch::Tensor> &c, const torch::Tensor &ta
 	r.status = status_of(status, c[0]);
 	TORCH_CHECK(table.dim() == 2 && start.dim() == 1 && start.size(0) == table.size(0) && cu.dim() == 1 && cu.size(0) == table.size(0) + 1,
 		    "table must be [n_seqs, max_pages], start [n_seqs], cu [n_seqs + 1], status [1]");
-	TORCH_CHECK(table.size(0) < INT32_MAX && table.size(1) * r.page <= INT32_MAX, "max_pages * page must fit int32");
+	TORCH_CHECK(table.size(0) < INT32_MAX && table.size(1) * r.page <= 1 << 30, "max_pages * page must be 2^30 at most");
 	r.n_seqs = int(table.size(0));
 	r.max_pages = int(table.size(1));
 	return r;
@@ -123,7 +123,7 @@ torch::Tensor attend(torch::Tensor q, std::vector<torch::Tensor> cache, torch::T
 	const l1attn_cache c = places(cache, table, start, cu, status);
 	q = tokens(q, "q", cache[0], -1, c.width);
 	const int64_t h = q.size(1);
-	TORCH_CHECK(h >= 1 && h % c.n_kv_heads == 0 && h <= INT32_MAX, "the heads of q must be a multiple of the cache's");
+	TORCH_CHECK(h >= 1 && h % c.n_kv_heads == 0 && q.size(0) * h <= INT32_MAX, "the heads of q must be a multiple of the cache's");
 	torch::Tensor sl;
 	if (slopes.has_value() && slopes->defined()) {
 		TORCH_CHECK(slopes->scalar_type() == torch::kFloat32 && slopes->dim() == 1 && slopes->size(0) == h && slopes->device() == q.device(),

@@ -36,14 +36,14 @@ struct Call {
 		CHECK_CUDA(v_);
 		TORCH_CHECK(q_.dim() == 4 && k_.dim() == 4 && v_.dim() == 4, SHAPES);
 		TORCH_CHECK(k_.size(0) == q_.size(0) && k_.size(1) == q_.size(1) && k_.size(3) == q_.size(3) && v_.sizes().slice(0, 3) == k_.sizes().slice(0, 3), SHAPES);
-		TORCH_CHECK(k_.size(2) ? q_.size(2) % k_.size(2) == 0 : q_.size(2) == 0, "the heads of q must be a multiple of those of k and v");
+		TORCH_CHECK(k_.size(2) ? q_.size(2) > 0 && q_.size(2) % k_.size(2) == 0 : q_.size(2) == 0, "the heads of q must be a multiple of those of k and v");
 		const auto t = q_.scalar_type();
 		TORCH_CHECK((t == torch::kFloat32 || t == torch::kFloat16 || t == torch::kBFloat16) && k_.scalar_type() == t && v_.scalar_type() == t,
 			    "q, k, v must share dtype float32, float16 or bfloat16");
 		TORCH_CHECK(k_.device() == q_.device() && v_.device() == q_.device(), "q, k, v must be on one device");
 		TORCH_CHECK(q_.size(3) >= 1 && q_.size(3) <= 256 && v_.size(3) >= 1 && v_.size(3) <= 256, "widths must be 1 to 256");
 		for (int64_t s : {q_.size(0), q_.size(1), q_.size(2)})
-			TORCH_CHECK(s <= INT32_MAX, "sizes must fit int32");
+			TORCH_CHECK(s <= 1 << 30, "sizes must be 2^30 at most");
 		q = rows(q_);
 		k = rows(k_);
 		v = rows(v_);

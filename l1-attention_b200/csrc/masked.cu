@@ -93,8 +93,10 @@ int check(const void *q, const void *k, const void *v, const int64_t *strides, c
 		return L1ATTN_ERR_ARG;
 	if (mask->mode < 0 || mask->mode > 2 || mask->window < 0 || !(mask->softcap >= 0.f) || std::isinf(mask->softcap))
 		return L1ATTN_ERR_ARG;
-	if (width > 256 || v_width > 256)
+	if (width > 256 || v_width > 256 || n_tok > 1 << 30) // (ends of tiles stay within int)
 		return L1ATTN_ERR_SHAPE;
+	if (n_heads == 0 && n_kv_heads > 0)
+		return L1ATTN_ERR_ARG;
 	if (bs == 0 || n_tok == 0 || n_heads == 0)
 		return 1; // nothing to do
 	if (n_kv_heads == 0 || n_heads % n_kv_heads)

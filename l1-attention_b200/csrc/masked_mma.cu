@@ -15,6 +15,8 @@ namespace {
 
 constexpr int MB = 1, WARPS = 4, ROWS = 16 * MB * WARPS, KEYS = 64, STREAM = 32, THREADS = 32 * WARPS; // MB: blocks of 16 rows a warp
 constexpr float LOG2E = 1.4426950408889634f, LAG = 8.f;
+// float16 weights are formed times 2^LIFT, so that those of long flat rows are not lost below 2^-24 of the largest: at most 2^(LAG + LIFT)
+template <typename T> constexpr float LIFT = Half2<T>::ONES == Half2<__half>::ONES ? 6.f : 0.f;
 
 // One query row, by the definition: a warp, 32 keys at a time.  Rare, so simple.
 template <typename T> __device__ __noinline__ void exact_row(const MaskedArgs &a, const MaskView &mask, int b, int head, int t, T *vo, float *lse)
@@ -137,12 +139,13 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 		load_tile16<T, true, VP, KEYS, THREADS>(at + KEYS * KP * 16, a.v, b, kv, it * KEYS, a.n, a.v_width, doc, vec & 4, tid);
 	};
 
-	float m[2 * MB], l[2 * MB], ref[2 * MB]; // per row: the reference of its exponentials (times log2 e; ref: 0 while it is infinite), this lane's share of its sum
+	float m[2 * MB], l[2 * MB], ref[2 * MB]; // per row: the largest score (times log2 e; it may lag), this lane's share of the sum, what exponents are taken relative to
 	float o[MB][2 * V][4];
 #pragma unroll
 	for (int r = 0; r < 2 * MB; r++) {
 		m[r] = start_max(a.mode);
-		l[r] = ref[r] = 0.f;
+		ref[r] = m[r] == -INFINITY ? 0.f : m[r] - LIFT<T>;
+		l[r] = 0.f;
 	}
 #pragma unroll
 	for (int i = 0; i < MB * 2 * V * 4; i++)
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 				top[r] = fmaxf(fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)), m[r]);
 				const float keep = top[r] == -INFINITY ? 1.f : exp2_fast(m[r] - top[r]);
 				m[r] = top[r];
-				ref[r] = top[r] == -INFINITY ? 0.f : top[r];
+				ref[r] = top[r] == -INFINITY ? 0.f : top[r] - LIFT<T>;
 				l[r] *= keep;
 #pragma unroll
 				for (int v = 0; v < 2 * V; v++) {
@@ -336,6 +339,7 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 	for (int r = 0; r < 2 * MB; r++) {
 		l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
 		l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+		l[r] *= exp2f(-LIFT<T>);
 		if (a.mode == L1ATTN_SV_SOFTMAX_PLUS_ONE)
 			l[r] += exp2_fast(-m[r]);
 		float ls;
@@ -348,7 +352,7 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 #pragma unroll
 		for (int i = 0; i < 2 * V; i++) {
 			const int w = 8 * i + 2 * j;
-			const float y0 = f == 0.f ? 0.f : o[r / 2][i][2 * (r % 2)] * f, y1 = f == 0.f ? 0.f : o[r / 2][i][2 * (r % 2) + 1] * f;
+			const float y0 = f == 0.f ? 0.f : o[r / 2][i][2 * (r % 2)] * exp2f(-LIFT<T>) * f, y1 = f == 0.f ? 0.f : o[r / 2][i][2 * (r % 2) + 1] * exp2f(-LIFT<T>) * f;
 			odd |= !(fabsf(y0) < INFINITY) || !(fabsf(y1) < INFINITY);
 			if (t < a.n && w < a.v_width) {
 				if (vec & 8)

@@ -59,9 +59,9 @@ def attend(q, k_codes, v_codes, k_scale, v_scale, table, start, cu, mode="softma
     the row's own and earlier positions of its sequence.  Append a step's keys before its queries attend.
 
     max_len: the longest start + count, where the program knows it (default: what the table has room for); it shapes the launch alone.
-    out: a contiguous tensor to write; rows behind cu[-1] are left as they were in it, and undefined without it.
+    out: a contiguous tensor to write, not q itself; rows behind cu[-1] are left as they were in it, and undefined without it.
 
-    16-bit q: query / scale is rounded to float16 next to codes that it holds exactly, weights to 11 bits; float32 q: float32 throughout."""
+    16-bit q: query / scale is rounded to float16 next to codes that it holds exactly, weights to 11 bits or 2^-31 of the row's largest; float32 q: float32 throughout."""
     mode, _, window, softcap = _options(mode, True, window, softcap)
     return l1attn_cache_cuda_drv.attend(q, (k_codes, v_codes, k_scale, v_scale), table, start, cu, mode, window, softcap, slopes, -1 if max_len is None else max(0, int(max_len)),
                                         out, status)
@@ -170,6 +170,10 @@ class L1Cache:
         seqs, counts = [int(s) for s in seqs], [int(c) for c in counts]
         if len(seqs) != len(counts) or not seqs or min(counts) < 0 or len(set(seqs)) != len(seqs):
             raise ValueError("extend takes sequences, each once, and a count of 0 or more for each")
+        if isinstance(room, bool) or int(room) != room or room < 0:
+            raise ValueError("room must be a whole number of columns")
+        if sum(counts) > 0x7fffffff:
+            raise ValueError("a call's tokens must fit int32")
         need = max(max(-(-(self.length(s) + c) // self.page) for s, c in zip(seqs, counts)), 1)
         if into is not None and (into.n != len(seqs) or into.max_pages < need):
             raise ValueError("the plan to refresh has room for %d sequences of %d pages, not %d of %d" % (into.n, into.max_pages, len(seqs), need))

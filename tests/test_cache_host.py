@@ -193,6 +193,24 @@ def test_abi_refusals_of_one_call():
         assert _abi(what, rows=0) == 0 and _abi(what, n_seqs=0) == 0
 
 
+@pytest.mark.parametrize("what", ["append", "gather", "attend"])
+def test_abi_refuses_what_no_kernel_covers(what):
+    """A cache without pages (bad ids fall back on the first), and positions whose tiles would end past int."""
+    assert _abi(what, n_pages=0) == -1
+    assert _abi(what, max_pages=(1 << 26) + 1) == -2
+    assert what != "attend" or _abi(what, rows=1 << 30, heads=4) == -2
+
+
+def test_extend_refuses_before_it_changes_anything():
+    cache = L1Cache.__new__(L1Cache)
+    cache.page, cache._book, cache._epoch = 16, PageBook(4, 16), 0
+    s = cache._book.open()
+    for change in (dict(room=-1), dict(room=1.5), dict(room=True), dict(counts=[1 << 31])):
+        with pytest.raises(ValueError):
+            cache.extend([s], **dict(dict(counts=[1]), **change))
+    assert cache.length(s) == 0 and len(cache._book.free) == 4
+
+
 def test_module_refusals():
     for bad in (dict(n_pages=0), dict(width=0), dict(width=257), dict(v_width=1.5), dict(n_layers=0), dict(page=24), dict(n_kv_heads=True)):
         with pytest.raises(ValueError):

@@ -51,7 +51,8 @@ def test_work_bytes():
     f32, bf16 = l1attn_cabi.F32, l1attn_cabi.BF16
     assert f(2, 65, 3, 3, 64, 64, bf16, 0) == 256 and f(2, 1024, 3, 3, 64, 64, bf16, 0) == 2 * 16 * 16 and f(0, 0, 0, 0, 0, 0, bf16, 1) == 256
     rows = 2 * 1024 * 4 * 4
-    assert f(2, 1024, 4, 4, 64, 64, f32, 1) == f(2, 1024, 4, 2, 129, 64, bf16, 1) == 512 + rows  # ranges, delta
+    assert f(2, 1024, 4, 4, 64, 64, f32, 1) == f(2, 1024, 4, 4, 129, 64, bf16, 1) == 512 + rows  # ranges, delta
+    assert f(2, 1024, 4, 2, 64, 64, f32, 1) == 512 + rows + rows * 128 and f(2, 1024, 4, 2, 129, 64, bf16, 1) == 512 + rows + rows * 193  # shares of shared heads
     assert f(2, 1024, 4, 4, 64, 32, bf16, 1) == 512 + rows + 8 * 1024 * 1024 * 4  # and a float per pair
     assert f(2, 1024, 4, 2, 64, 32, bf16, 1) == 512 + rows + rows * 96 + 8 * 1024 * 1024 * 4  # and shares of shared heads
     assert f(8, 8192, 8, 8, 64, 64, bf16, 1) == 8 * 128 * 16 + 8 * 8192 * 8 * 4 + (1 << 30)  # never more than a gigabyte of pairs
@@ -66,6 +67,22 @@ def test_module_refusals():
     x = torch.zeros(1, 2, 2, 4)
     with pytest.raises(RuntimeError, match="CUDA"):
         L1AttnMasked()(x, x, x)
+
+
+def test_abi_refuses_what_no_kernel_covers():
+    """Keys without query heads (their gradients would be left unwritten), and positions whose tiles would end past int."""
+    for back in (False, True):
+        assert _call(back=back, h=0) == -1 and _call(back=back, h=0, hk=0) == 0
+        assert _call(back=back, n=(1 << 30) + 1) == -2
+
+
+@pytest.mark.gpu
+def test_module_refuses_keys_without_queries():
+    from l1attn_masked_cuda import L1AttnMasked
+    z = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+    with pytest.raises(RuntimeError, match="multiple"):
+        L1AttnMasked()(z(2, 5, 0, 8), z(2, 5, 2, 8), z(2, 5, 2, 8))
+    assert L1AttnMasked()(z(2, 5, 0, 8), z(2, 5, 0, 8), z(2, 5, 0, 6)).shape == (2, 5, 0, 6)
 
 
 @pytest.mark.gpu
