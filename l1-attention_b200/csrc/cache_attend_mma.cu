@@ -4,8 +4,8 @@
 // Codes are exact as float16, so is the minimum; q' carries 11 bits, at worst 1/32 of a code's step (and what is clipped off is added in float32).
 // The minima go through mma.m16n8k16 as in mma.cuh with the sides swapped: A's rows are 16 keys, unpacked once into registers, and the
 // query rows -- (token, head of the group) pairs that all read these keys -- are streamed from shared memory, one column each.  Nothing is wasted on
-// few query rows.  A second product with B = -1/2 takes off half the sum of the codes, one per page gives the sum of q'.  Weights go to float16 (11 bits)
-// times the page's value scale, by movmatrix into the columns of the value product, whose A's rows are 16 channels, unpacked from the codes.
+// few query rows.  A second product with B = -1/2 takes off half the sum of the codes, one per page gives the sum of q'.  Weights go to float16 (11 bits;
+// for float16 outputs what that leaves, in a second product) times the page's value scale, by movmatrix into the columns of the value product, whose A's rows are 16 channels, unpacked from the codes.
 //
 // A warp streams chunks of 16 or 32 keys on its own (asynchronous copies into its own stages, no barrier in the loop); the four warps of a CTA
 // take runs of its chunks and join at the end.  The chunks of all units -- a tile of query rows and a head of keys and values -- lie behind one
@@ -73,6 +73,7 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 	extern __shared__ uint4 smem16[];
 	using L = Layout<T, WG, VG, TILES, NG>;
 	constexpr int CHUNK = L::CHUNK, ROWS = 8 * TILES, W = 64 * WG;
+	constexpr bool TWICE = H::ONES == Half2<T>::ONES; // float16 outputs are finer than weights of 11 bits: the rest of a weight takes a product of its own
 	const CacheArgs &c = a.c;
 	unsigned char *const smem = reinterpret_cast<unsigned char *>(smem16);
 	const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4;
@@ -183,8 +184,8 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 		// (chunk0 + k) CHUNK.  Pages are looked up for 32 chunks at a time, one a lane, two such sets.
 		const int in_range = hi > lo ? (hi + CHUNK - 1) / CHUNK - lo / CHUNK : 0;
 		const int chunk0 = lo / CHUNK + in_range * warp / WARPS, chunks = lo / CHUNK + in_range * (warp + 1) / WARPS - chunk0;
-		int page_id[2];
-		float page_k[2], page_v[2];
+		int page_id[2] = {-1, -1};
+		float page_k[2] = {0.f, 0.f}, page_v[2] = {0.f, 0.f};
 		auto look_up = [&](int block) {
 			const int k = block * 32 + lane, pos = (chunk0 + k) * CHUNK;
 			int id = -1;
@@ -196,9 +197,10 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 					vs = c.v_scale[(long long)id * c.kv_heads + kv];
 				}
 			}
-			page_id[block & 1] = id;
-			page_k[block & 1] = ks;
-			page_v[block & 1] = vs;
+			const bool odd = block & 1; // (no index: the sets stay in registers)
+			page_id[0] = odd ? page_id[0] : id, page_id[1] = odd ? id : page_id[1];
+			page_k[0] = odd ? page_k[0] : ks, page_k[1] = odd ? ks : page_k[1];
+			page_v[0] = odd ? page_v[0] : vs, page_v[1] = odd ? vs : page_v[1];
 		};
 		// this lane's pieces of a chunk: rows lane / pieces + i K_ROWS; where they go differs by whole rows, for values also in the bit that i's parity flips
 		constexpr int K_ROWS = 8 / WG, V_ROWS = 16 / VG;
@@ -425,7 +427,7 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 			// weights, and their products with the values: A's rows are channels 32 i + 4 g + 2 h, + 1
 #pragma unroll
 			for (int n = 0; n < NG; n++) {
-				uint32_t p[TILES][2];
+				uint32_t p[TILES][2], low[TILES][2];
 #pragma unroll
 				for (int i = 0; i < TILES; i++) {
 					float e[4];
@@ -433,9 +435,15 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 					for (int d = 0; d < 4; d++) {
 						e[d] = exp2_fast(x[n][i][d] - ref[i][d & 1]);
 						l[i][d & 1] += e[d];
+						e[d] *= v_rel;
 					}
-					p[i][0] = transpose8x8(H::pack(e[0] * v_rel, e[1] * v_rel));
-					p[i][1] = transpose8x8(H::pack(e[2] * v_rel, e[3] * v_rel));
+#pragma unroll
+					for (int d = 0; d < 2; d++) {
+						const uint32_t high = H::pack(e[2 * d], e[2 * d + 1]);
+						p[i][d] = transpose8x8(high);
+						if (TWICE)
+							low[i][d] = transpose8x8(H::pack(e[2 * d] - to_float(half_of<__half>(high, 0)), e[2 * d + 1] - to_float(half_of<__half>(high, 1))));
+					}
 				}
 #pragma unroll
 				for (int v = 0; v < VG; v++) {
@@ -450,7 +458,11 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 					for (int i = 0; i < TILES; i++)
 #pragma unroll
 						for (int h = 0; h < 2; h++)
+						{
 							H::mma(o[i][2 * v + h], f[h][0], f[h][1], f[h][2], f[h][3], p[i][0], p[i][1]);
+							if (TWICE)
+								H::mma(o[i][2 * v + h], f[h][0], f[h][1], f[h][2], f[h][3], low[i][0], low[i][1]);
+						}
 				}
 			}
 		}

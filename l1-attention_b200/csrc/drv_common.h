@@ -1,4 +1,4 @@
-// Shared pieces of the three pybind drivers: input checks with the reference's messages
+// Shared pieces of the pybind drivers: input checks with the reference's messages
 // (cuda/l1attn_cuda_drv.cpp:38-40), status -> exception, dtype code, current stream.
 #pragma once
 #include <torch/extension.h>
@@ -14,7 +14,7 @@
 	CHECK_CONTIGUOUS(x)
 
 // allow16: the sparse forward also takes float16 / bfloat16 storage (the reference dispatches Half
-// there, cuda/l1attn_sparse_cuda_kernel.cu:405); every other operator is float32 / float64 only
+// there, cuda/l1attn_sparse_cuda_kernel.cu:405), as do masked attention and the cache; every other operator is float32 / float64 only
 inline int l1b_dtype(const torch::Tensor &t, const char *what, bool allow16 = false)
 {
 	if (t.scalar_type() == torch::kFloat32)
