@@ -2,11 +2,12 @@
 //
 // Forward: a CTA of four warps owns 64 query rows of one head, a warp 16 of them, in registers; keys and values stream in tiles of 64 through
 // two stages of asynchronous copies.  Running softmax in registers (a row's scores lie in one quad); weights are rounded to the inputs' type for the value
-// product (11 or 8 bits, as the values have; the normaliser sums them unrounded), everything else is float32.  Rows whose result is not
+// product (11 bits, or 8 and what these leave in a second product; the normaliser sums them unrounded), everything else is float32.  Rows whose result is not
 // finite are done again, exactly, by a warp each: an infinite or NaN operand spoils its neighbours in a product.
 // Bound: instruction issue of few warps.  mma.sync does not overlap float32 instructions (mma alone 8 clocks per scheduler, 13.2 with four
 // additions, 9.7 with four minima), so the softmax costs what it takes; forming the next step's distances beside it brought [2,2048,8,128] from
-// 343 to 293 us, the short copy loop a tenth.  Now 54 terms per clock and SM ([4,2048,8,128], no mask: 1.10 ms) where float32 instructions reach 48 at best.
+// 343 to 293 us, the short copy loop a tenth; the rests of bfloat16 weights cost a tenth of it again and bring the error of dq (by its row's delta) from 1.5 to 1.35 of a
+// float32 form's that rounds at the end.  Now 52 terms per clock and SM in float16 ([4,2048,8,64], no mask: 564 us), 48 in bfloat16 ([4,2048,8,128]: 1.22 ms).
 #include "mma.cuh"
 
 namespace l1b {
@@ -77,7 +78,7 @@ template <typename T> __device__ __noinline__ void exact_row(const MaskedArgs &a
 			vo[row * a.v_width + lane + 32 * i] = from_float<T>(f == 0.f ? 0.f : acc[i] * f);
 }
 
-// W: 32-column groups of the width; V: 16-column groups of the value rows (4 or 8).  CTAs of an SM, two against three (168 registers): [1,4096,8,64]
+// W: 32-column groups of the width; V: 16-column groups of the value rows (4 or 8).  CTAs of an SM, two against three (168 registers; before the rests' products): [1,4096,8,64]
 // with values of 128 339 / 447 us, [2,2048,8,128] 293 / 472, widths of 32 200 / 235; but [1,8192,8,64] 1230 / 1157 and [4,2048,8,128] with values of 64
 // (no mask) 1179 / 1005.
 template <typename T, int W, int V>
@@ -87,6 +88,7 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 	__shared__ float key_sums[KEYS];
 	using H = Half2<T>;
 	constexpr int KP = 4 * W, VP = 2 * V; // 16-byte pieces of a row
+	constexpr bool TWICE = H::ONES == Half2<__nv_bfloat16>::ONES; // what bfloat16 leaves of a weight (8 bits) takes a product of its own
 	const uint32_t base = shared_address(smem16), stage_bytes = KEYS * (KP + VP) * 16;
 	const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4;
 	const int bh = blockIdx.x % (a.bs * a.heads), tile = tiles - 1 - int(blockIdx.x / (a.bs * a.heads)); // the longest rows of a causal mask first
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 	};
 	// weights of 16 keys, and their products with the values
 	auto values = [&](uint32_t vt, int kb, const float(&x)[MB][2][4]) {
-		uint32_t p[MB][4];
+		uint32_t p[MB][4], low[MB][4];
 #pragma unroll
 		for (int i = 0; i < MB; i++)
 #pragma unroll
@@ -187,8 +189,12 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 					e[c] = exp2_fast(x[i][h][c] - ref[2 * i + c / 2]);
 					l[2 * i + c / 2] += e[c];
 				}
-				p[i][2 * h] = H::pack(e[0], e[1]);
-				p[i][2 * h + 1] = H::pack(e[2], e[3]);
+#pragma unroll
+				for (int c = 0; c < 2; c++) {
+					const uint32_t high = p[i][2 * h + c] = H::pack(e[2 * c], e[2 * c + 1]);
+					if (TWICE) // (a bfloat16 is the upper half of its float)
+						low[i][2 * h + c] = H::pack(e[2 * c] - __uint_as_float(high << 16), e[2 * c + 1] - __uint_as_float(high & 0xffff0000u));
+				}
 			}
 #pragma unroll
 		for (int vb = 0; vb < V; vb++) {
@@ -198,6 +204,10 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 			for (int i = 0; i < MB; i++) {
 				H::mma(o[i][2 * vb], p[i][0], p[i][1], p[i][2], p[i][3], y[0], y[1]);
 				H::mma(o[i][2 * vb + 1], p[i][0], p[i][1], p[i][2], p[i][3], y[2], y[3]);
+				if (TWICE) {
+					H::mma(o[i][2 * vb], low[i][0], low[i][1], low[i][2], low[i][3], y[0], y[1]);
+					H::mma(o[i][2 * vb + 1], low[i][0], low[i][1], low[i][2], low[i][3], y[2], y[3]);
+				}
 			}
 		}
 	};
