@@ -144,24 +144,32 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(THREADS) gathe
 		T *const out = (values ? v : k) + row * c.kv_heads * w;
 		const long long head = (long long)c.page * w;
 		if (VEC) {
-			constexpr int N = Vector<T>::N;
-			const int per_head = w / N;
-#pragma unroll 4
-			for (int i = lane; i < c.kv_heads * per_head; i += 32) {
-				const int h = i / per_head;
-				const int8_t *const from = codes + h * head + i % per_head * N;
-				uint32_t x[N / 4];
-				if constexpr (N == 8) {
-					const uint2 y = *reinterpret_cast<const uint2 *>(from);
-					x[0] = y.x, x[N / 4 - 1] = y.y;
-				} else
-					x[0] = *reinterpret_cast<const uint32_t *>(from);
-				const float s = scale[h];
-				uint4 y;
+			constexpr int N = Vector<T>::N, AT_ONCE = 4; // vectors of a lane whose reads do not wait for one another
+			const unsigned per_head = w / N, all = c.kv_heads * per_head;
+			const unsigned over = 0xffffffffu / per_head + 1; // i / per_head = the high half of i * over: exact for i < 2^32 / per_head; 1: itself
+			for (unsigned i0 = lane; i0 < all; i0 += 32 * AT_ONCE) {
+				uint32_t x[AT_ONCE][N / 4];
+				float s[AT_ONCE];
 #pragma unroll
-				for (int e = 0; e < N; e++) // (a page out of range: zeros, whatever has been read)
-					reinterpret_cast<T *>(&y)[e] = from_float<T>(id < 0 ? 0.f : float(int8_t(x[e / 4] >> 8 * (e % 4))) * s);
-				reinterpret_cast<uint4 *>(out)[i] = y;
+				for (int j = 0; j < AT_ONCE; j++) {
+					const unsigned i = min(i0 + 32 * j, all - 1), h = per_head == 1 ? i : __umulhi(i, over);
+					const int8_t *const from = codes + h * head + (i - h * per_head) * N;
+					if constexpr (N == 8) {
+						const uint2 y = *reinterpret_cast<const uint2 *>(from);
+						x[j][0] = y.x, x[j][N / 4 - 1] = y.y;
+					} else
+						x[j][0] = *reinterpret_cast<const uint32_t *>(from);
+					s[j] = scale[h];
+				}
+#pragma unroll
+				for (int j = 0; j < AT_ONCE; j++) {
+					uint4 y;
+#pragma unroll
+					for (int e = 0; e < N; e++) // (a page out of range: zeros, whatever has been read)
+						reinterpret_cast<T *>(&y)[e] = from_float<T>(id < 0 ? 0.f : float(int8_t(x[j][e / 4] >> 8 * (e % 4))) * s[j]);
+					if (i0 + 32 * j < all)
+						reinterpret_cast<uint4 *>(out)[i0 + 32 * j] = y;
+				}
 			}
 		} else
 			for (int i = lane; i < c.kv_heads * w; i += 32)
