@@ -24,16 +24,28 @@ __device__ __noinline__ int quantise_any(float x, float s, float inv)
 		q += copysignf(1.f, r);
 	return int(fminf(fmaxf(q, -127.f), 127.f));
 }
-// The low byte of the same.  1.5 * 2^23 leaves the whole number in the low bits of the sum; where the residual says that it is the nearest for sure
-// (almost always), that is all.
-__device__ __forceinline__ uint32_t quantise(float x, float s, float inv)
+// The same in the low byte, for sure where *near stays true: 1.5 * 2^23 leaves the whole number in the low bits of the sum, and the residual says that it is
+// the nearest (almost always).  half: s / 2, or 0 where that is not exact.
+__device__ __forceinline__ uint32_t quantise_near(float x, float s, float inv, float half, bool *near)
 {
 	const float t = fmaf(x, inv, 12582912.f), r = fmaf(12582912.f - t, s, x);
-	return (fabsf(r + r) < s ? __float_as_uint(t) : uint32_t(quantise_any(x, s, inv))) & 0xffu;
+	*near = *near && fabsf(r) < half;
+	return __float_as_uint(t);
 }
 
 template <typename T> struct Vector { // 16 bytes of tokens
 	static constexpr int N = 16 / sizeof(T);
+};
+// bits of a value without its sign: ordered as the values are, infinities and NaN behind all others
+template <typename T> struct Bits;
+template <> struct Bits<float> {
+	static constexpr uint32_t ALL = 0x7fffffffu, INF = 0x7f800000u;
+};
+template <> struct Bits<__half> {
+	static constexpr uint32_t ALL = 0x7fff7fffu, INF = 0x7c00u;
+};
+template <> struct Bits<__nv_bfloat16> {
+	static constexpr uint32_t ALL = 0x7fff7fffu, INF = 0x7f80u;
 };
 
 // A CTA per (page that new tokens touch, head, keys or values): it alone reads and writes that page's rows and scale of that head.
@@ -70,16 +82,29 @@ __global__ void __launch_bounds__(THREADS) append_kernel(CacheArgs c, const T *k
 				break;
 			held[j] = *reinterpret_cast<const uint4 *>(src + (i / per_row) * src_row + i % per_row * N);
 		}
+		uint32_t top = 0; // the largest bits, two of a word where values are of 16
 #pragma unroll
 		for (int j = 0; j < HELD; j++) {
 			if (tid + j * THREADS >= vectors)
 				break;
-#pragma unroll
-			for (int e = 0; e < N; e++) {
-				const float x = fabsf(to_float(reinterpret_cast<const T *>(&held[j])[e]));
-				most = finite(x) ? fmaxf(most, x) : most;
-			}
+			for (uint32_t word : {held[j].x, held[j].y, held[j].z, held[j].w})
+				top = N == 8 ? __vmaxu2(top, word & Bits<T>::ALL) : max(top, word & Bits<T>::ALL);
 		}
+		if (N == 8)
+			top = max(top >> 16, top & 0xffffu);
+		if (top < Bits<T>::INF)
+			most = to_float(*reinterpret_cast<const T *>(&top));
+		else // what is not finite does not count
+#pragma unroll
+			for (int j = 0; j < HELD; j++) {
+				if (tid + j * THREADS >= vectors)
+					break;
+#pragma unroll
+				for (int e = 0; e < N; e++) {
+					const float x = fabsf(to_float(reinterpret_cast<const T *>(&held[j])[e]));
+					most = finite(x) ? fmaxf(most, x) : most;
+				}
+			}
 	} else
 		for (int i = tid; i < (b - a) * w; i += THREADS) {
 			const float x = fabsf(to_float(src[(i / w) * src_row + i % w]));
@@ -95,7 +120,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(CacheArgs c, const T *k
 #pragma unroll
 	for (int i = 0; i < THREADS / 32; i++)
 		most = fmaxf(most, part[i]);
-	const float now = fmaxf(most / 127.f, old), inv = 1.f / now;
+	const float now = fmaxf(most / 127.f, old), inv = 1.f / now, half = now >= 0x1p-125f ? 0.5f * now : 0.f;
 	if (a > 0 && now > old) // the rows that were there follow the new scale
 		for (int i = tid; i < a * w; i += THREADS)
 			codes[i] = int8_t(rint(double(codes[i]) * double(old) / double(now)));
@@ -105,12 +130,18 @@ __global__ void __launch_bounds__(THREADS) append_kernel(CacheArgs c, const T *k
 			const int i = tid + j * THREADS;
 			if (i >= vectors)
 				break;
-			uint32_t out[N / 4];
+			uint32_t out[N / 4], q[N];
+			bool near = true;
 #pragma unroll
-			for (int e = 0; e < N; e++) {
-				const uint32_t q = quantise(to_float(reinterpret_cast<const T *>(&held[j])[e]), now, inv);
-				out[e / 4] = e % 4 ? out[e / 4] | q << 8 * (e % 4) : q;
-			}
+			for (int e = 0; e < N; e++)
+				q[e] = quantise_near(to_float(reinterpret_cast<const T *>(&held[j])[e]), now, inv, half, &near);
+			if (!near)
+#pragma unroll
+				for (int e = 0; e < N; e++)
+					q[e] = uint32_t(quantise_any(to_float(reinterpret_cast<const T *>(&held[j])[e]), now, inv));
+#pragma unroll
+			for (int i = 0; i < N / 4; i++)
+				out[i] = __byte_perm(__byte_perm(q[4 * i], q[4 * i + 1], 0x0040), __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040), 0x5410);
 			int8_t *const to = codes + (long long)a * w + i * N;
 			if constexpr (N == 8)
 				*reinterpret_cast<uint2 *>(to) = make_uint2(out[0], out[1]);
@@ -119,7 +150,7 @@ __global__ void __launch_bounds__(THREADS) append_kernel(CacheArgs c, const T *k
 		}
 	} else
 		for (int i = tid; i < (b - a) * w; i += THREADS)
-			codes[a * w + i] = int8_t(quantise(to_float(src[(i / w) * src_row + i % w]), now, inv));
+			codes[a * w + i] = int8_t(quantise_any(to_float(src[(i / w) * src_row + i % w]), now, inv));
 	if (tid == 0)
 		*scale = now;
 }
