@@ -3,7 +3,7 @@
 // Forward: a CTA owns 64 query rows of one head; keys and values stream in tiles of 64 (32), all operands as floats in shared memory.  256
 // threads, a 4 x 4 (4 x 2) tile of scores each (rows 4 ty + i, keys tx + 16 j); the 16 lanes of a half-warp own their four rows, so the running maximum
 // and sum (one pass over the keys) and the weights never leave the half-warp.  Bound: FP32 instructions -- two per term of the distance, one per term
-// of a product -- and, at 12 terms per clock and SM ([4,2048,8,128], no mask: 5.05 ms), the loads of the tiles, which nothing hides.
+// of a product -- of which the loads of scores and weights take a quarter of the issue slots: 21 terms per clock and SM ([4,2048,8,128], no mask: 2.75 ms).
 // Backward: two kernels without atomics.  One owns 64 query rows and makes dq, the other 64 key rows of one query head and makes its share of dk and dv;
 // both recompute the weights from the log-normalisers and stream the other side in
 // tiles of 32.  sign(0) = 0.
@@ -26,13 +26,42 @@ __host__ __device__ inline int pitch(int w)
 template <typename T>
 __device__ bool load_rows(float *dst, int pitch_, int cols, const Strided &x, int b, int head, int first, int rows, int n, int width)
 {
+	constexpr int AT_ONCE = 4; // rows of a warp whose reads do not wait for one another
 	const T *src = static_cast<const T *>(x.p) + b * x.batch + head * x.head;
+	const int lane = threadIdx.x % 32;
 	bool odd = false;
-	for (int r = threadIdx.x / 32; r < rows; r += THREADS / 32)
-		for (int c = threadIdx.x % 32; c < cols; c += 32) {
-			const float f = first + r < n && c < width ? to_float(src[(first + r) * x.tok + c]) : 0.f;
-			odd |= !(fabsf(f) < INFINITY);
-			dst[r * pitch_ + c] = f;
+	if (sizeof(T) == 4 && width % 4 == 0 && reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && (x.batch | x.tok | x.head) % 4 == 0) { // 16 bytes a lane
+		for (int r0 = threadIdx.x / 32; r0 < rows; r0 += AT_ONCE * (THREADS / 32))
+			for (int c = 4 * lane; c < cols; c += 128) {
+				float4 f[AT_ONCE];
+#pragma unroll
+				for (int i = 0; i < AT_ONCE; i++) {
+					const int r = r0 + i * (THREADS / 32);
+					f[i] = r < rows && first + r < n && c < width ? *reinterpret_cast<const float4 *>(src + (first + r) * x.tok + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+				}
+#pragma unroll
+				for (int i = 0; i < AT_ONCE; i++)
+					if (const int r = r0 + i * (THREADS / 32); r < rows) {
+						odd |= !(fabsf(f[i].x) + fabsf(f[i].y) + fabsf(f[i].z) + fabsf(f[i].w) < INFINITY);
+						*reinterpret_cast<float4 *>(dst + r * pitch_ + c) = f[i];
+					}
+			}
+		return odd;
+	}
+	for (int r0 = threadIdx.x / 32; r0 < rows; r0 += AT_ONCE * (THREADS / 32))
+		for (int c = lane; c < cols; c += 32) {
+			float f[AT_ONCE];
+#pragma unroll
+			for (int i = 0; i < AT_ONCE; i++) {
+				const int r = r0 + i * (THREADS / 32);
+				f[i] = r < rows && first + r < n && c < width ? to_float(src[(first + r) * x.tok + c]) : 0.f;
+			}
+#pragma unroll
+			for (int i = 0; i < AT_ONCE; i++)
+				if (const int r = r0 + i * (THREADS / 32); r < rows) {
+					odd |= !(fabsf(f[i]) < INFINITY);
+					dst[r * pitch_ + c] = f[i];
+				}
 		}
 	return odd;
 }
@@ -104,8 +133,8 @@ template <typename T, int NV, int KEYS> __global__ void __launch_bounds__(THREAD
 	const int wp = pitch(a.width), vp = 64 * NV, tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
 	float *Q = reinterpret_cast<float *>(smem4), *K = Q + OWN * wp, *V = K + KEYS * wp, *P = V + KEYS * vp;
 	constexpr int PP = KEYS + 4;
-	const int tile = tiles - 1 - int(blockIdx.x % tiles); // the longest rows of a causal mask first
-	const int head = (blockIdx.x / tiles) % a.heads, b = blockIdx.x / tiles / a.heads, kv = head / (a.heads / a.kv_heads);
+	const int bh = blockIdx.x % (a.bs * a.heads), tile = tiles - 1 - int(blockIdx.x / (a.bs * a.heads)); // the longest rows of a causal mask first, of all heads
+	const int head = bh % a.heads, b = bh / a.heads, kv = head / (a.heads / a.kv_heads);
 	const MaskView mask(a, b);
 	const int t0 = tile * OWN, t1 = min(a.n, t0 + OWN);
 	const float slope = a.slopes ? a.slopes[head] : 0.f, inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
@@ -129,6 +158,7 @@ template <typename T, int NV, int KEYS> __global__ void __launch_bounds__(THREAD
 		load_rows<T>(K, wp, wp, a.k, b, kv, s0, KEYS, a.n, a.width);
 		const bool odd = __syncthreads_or(load_rows<T>(V, vp, vp, a.v, b, kv, s0, KEYS, a.n, a.v_width));
 		constexpr int J = KEYS / 16;
+		const bool whole = s1 == s0 + KEYS && t1 == t0 + OWN && mask.all(t0, t1, s0, s1);
 		float x[4][J];
 		distances<J>(Q, K, wp, a.width, ty, tx, x);
 #pragma unroll
@@ -142,7 +172,7 @@ template <typename T, int NV, int KEYS> __global__ void __launch_bounds__(THREAD
 				if (a.cap > 0.f)
 					y = a.cap * tanhf(y * inv_cap);
 				y -= slope * fabsf(float(t - s));
-				x[i][j] = mask.sees(t, s, doc_t[i], mask.doc && s < a.n ? mask.doc[s] : 0) ? y : -INFINITY;
+				x[i][j] = whole || mask.sees(t, s, doc_t[i], mask.doc && s < a.n ? mask.doc[s] : 0) ? y : -INFINITY;
 				top = fmaxf(top, x[i][j]);
 			}
 			top = half_warp_max(top);
@@ -161,17 +191,13 @@ template <typename T, int NV, int KEYS> __global__ void __launch_bounds__(THREAD
 				acc[i][c] *= keep;
 		}
 		__syncwarp();
-		for (int s = 0; s < s1 - s0; s++) {
-			float p[4];
-#pragma unroll
-			for (int i = 0; i < 4; i++)
-				p[i] = P[(4 * ty + i) * PP + s];
+		auto add = [&](const float (&p)[4], int s, bool skip) {
 #pragma unroll
 			for (int u = 0; u < NV; u++) {
 				const float4 v = *reinterpret_cast<const float4 *>(V + s * vp + 64 * u + 4 * tx);
 #pragma unroll
 				for (int i = 0; i < 4; i++) {
-					if (odd && p[i] == 0.f)
+					if (skip && p[i] == 0.f)
 						continue;
 					acc[i][4 * u] = fmaf(p[i], v.x, acc[i][4 * u]);
 					acc[i][4 * u + 1] = fmaf(p[i], v.y, acc[i][4 * u + 1]);
@@ -179,7 +205,26 @@ template <typename T, int NV, int KEYS> __global__ void __launch_bounds__(THREAD
 					acc[i][4 * u + 3] = fmaf(p[i], v.w, acc[i][4 * u + 3]);
 				}
 			}
-		}
+		};
+		if (odd) // a value that is not finite: what has no weight must not be multiplied
+			for (int s = 0; s < s1 - s0; s++) {
+				float p[4];
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					p[i] = P[(4 * ty + i) * PP + s];
+				add(p, s, true);
+			}
+		else // four keys at a time (past the last one: weights and values of zero)
+			for (int s = 0; s < s1 - s0; s += 4) {
+				float4 p[4];
+#pragma unroll
+				for (int i = 0; i < 4; i++)
+					p[i] = *reinterpret_cast<const float4 *>(P + (4 * ty + i) * PP + s);
+				add({p[0].x, p[1].x, p[2].x, p[3].x}, s, false);
+				add({p[0].y, p[1].y, p[2].y, p[3].y}, s + 1, false);
+				add({p[0].z, p[1].z, p[2].z, p[3].z}, s + 2, false);
+				add({p[0].w, p[1].w, p[2].w, p[3].w}, s + 3, false);
+			}
 	}
 #pragma unroll
 	for (int i = 0; i < 4; i++) {
@@ -224,8 +269,8 @@ __global__ void __launch_bounds__(THREADS, NW >= 6 ? 1 : 0) masked_bwd_simple_ke
 	constexpr int GP = OWN + 4;
 	// (columns past a row's pitch read the next row, the last ones' G: what they come to is not stored)
 	float *A = reinterpret_cast<float *>(smem4), *B = A + OWN * wp, *C = B + OWN * vp, *D = C + STREAM * wp, *G = D + STREAM * vp, *P = G + STREAM * GP;
-	const int tile = OWN_KEYS ? int(blockIdx.x % tiles) : tiles - 1 - int(blockIdx.x % tiles);
-	const int head = (blockIdx.x / tiles) % a.heads, b = blockIdx.x / tiles / a.heads, kv = head / (a.heads / a.kv_heads);
+	const int bh = blockIdx.x % (a.bs * a.heads), rank = blockIdx.x / (a.bs * a.heads), tile = OWN_KEYS ? rank : tiles - 1 - rank; // what a causal mask leaves most work first
+	const int head = bh % a.heads, b = bh / a.heads, kv = head / (a.heads / a.kv_heads);
 	const MaskView mask(a, b);
 	const int o0 = tile * OWN, o1 = min(a.n, o0 + OWN);
 	const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f, slope = a.slopes ? a.slopes[head] : 0.f;
@@ -253,6 +298,7 @@ __global__ void __launch_bounds__(THREADS, NW >= 6 ? 1 : 0) masked_bwd_simple_ke
 		load_rows<T>(C, wp, wp, OWN_KEYS ? a.q : a.k, b, OWN_KEYS ? head : kv, r0, STREAM, a.n, a.width);
 		const bool odd = __syncthreads_or(load_rows<T>(D, vp, vp, OWN_KEYS ? go : a.v, b, OWN_KEYS ? head : kv, r0, STREAM, a.n, a.v_width));
 		constexpr int J = STREAM / 16;
+		const bool whole = r1 == r0 + STREAM && o1 == o0 + OWN && (OWN_KEYS ? mask.all(r0, r1, o0, o1) : mask.all(o0, o1, r0, r1));
 		float x[4][J], dp[4][J];
 		distances<J>(A, C, wp, a.width, ty, tx, x);
 		products<J>(B, D, vp, a.v_width, ty, tx, dp);
@@ -263,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, NW >= 6 ? 1 : 0) masked_bwd_simple_ke
 			for (int i = 0; i < 4; i++) {
 				const int o = o0 + 4 * ty + i, r = r0 + tx + 16 * j, t = OWN_KEYS ? r : o, s = OWN_KEYS ? o : r;
 				p[i] = e[i] = 0.f;
-				if (t < a.n && s < a.n && mask.sees(t, s, mask.doc ? mask.doc[t] : 0, mask.doc ? mask.doc[s] : 0)) {
+				if (whole || (t < a.n && s < a.n && mask.sees(t, s, mask.doc ? mask.doc[t] : 0, mask.doc ? mask.doc[s] : 0))) {
 					const long long row = ((long long)b * a.n + t) * a.heads + head;
 					float y = -a.scale * x[i][j], slant = 1.f;
 					if (a.cap > 0.f) {
@@ -345,11 +391,11 @@ template <typename T, int NV, int KEYS> int fwd_tiles(const MaskedArgs &a, void 
 	return L1ATTN_OK;
 }
 
-// Tiles of 64 keys where two CTAs of them fit an SM, else of 32: [4,2048,8,128], no mask, 5.05 against 7.66 ms; but [2,2048,8,64], causal, 0.99 / 0.84, and
-// [3,501,6,65] with values of 40 169 / 143 us.
+// Tiles of 32 keys where two CTAs of them fit an SM and two of 64 keys do not, else of 64.  64 against 32: [2,2048,8,64], causal, 402 / 474 us,
+// [3,501,6,65] with values of 40 94 / 117, [1,1000,8,200] 378 / 440 (one CTA either way); but [2,2048,8,128] 865 / 725.
 template <typename T, int NV> int fwd(const MaskedArgs &a, void *vo, float *lse, cudaStream_t st)
 {
-	return fwd_bytes(a.width, NV, 64) <= 113 * 1024 ? fwd_tiles<T, NV, 64>(a, vo, lse, st) : fwd_tiles<T, NV, 32>(a, vo, lse, st);
+	return fwd_bytes(a.width, NV, 64) > 113 * 1024 && fwd_bytes(a.width, NV, 32) <= 113 * 1024 ? fwd_tiles<T, NV, 32>(a, vo, lse, st) : fwd_tiles<T, NV, 64>(a, vo, lse, st);
 }
 
 template <typename T, typename OUT, bool OWN_KEYS, int NW, int NV>
