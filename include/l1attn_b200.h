@@ -200,17 +200,18 @@ typedef struct l1attn_mask {
  * vo[b][t][h][:] = sum_s weight * v[b][s][h / (n_heads / n_kv_heads)][:], and the gradients.  q: [bs][n_tok][n_heads][width], k, v:
  * [bs][n_tok][n_kv_heads][width / v_width] with n_heads a multiple of n_kv_heads; widths 1 .. 256; dtype L1ATTN_F32, L1ATTN_F16 or L1ATTN_BF16.
  * strides: nine element strides (batch, token, head of q, then of k, then of v), in host memory; the width is contiguous, 0 repeats
- * a tensor.  vo, dvo and the gradients are contiguous.  lse: float [bs][n_tok][n_heads], the rows' log-normalisers (NULL in the forward: not
+ * a tensor.  vo, dvo and the gradients are contiguous.  rest: like vo, what its rounding to 16 bits left (NULL: not kept, and dq a little less exact;
+ * not used in float32).  lse: float [bs][n_tok][n_heads], the rows' log-normalisers (NULL in the forward: not
  * kept).  work: device memory of l1attn_masked_work_bytes() bytes, 256-byte aligned (the forward uses it only with documents and takes NULL
  * without); nothing in it needs to be initialised or outlives the call, and calls that share it must not overlap on the GPU.
  * The backward in 16 bits with widths up to 128 keeps gradients of the distances there, up to a gigabyte at once (a float per pair and query head of a
  * batch item; none beyond 16384 tokens).  Sums and normalisers are float32 in every case.  The backward is deterministic.  n_tok: up to 2^30.
  */
 size_t l1attn_masked_work_bytes(int bs, int n_tok, int n_heads, int n_kv_heads, int width, int v_width, int dtype, int backward);
-int l1attn_masked_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *vo, float *lse, void *work,
+int l1attn_masked_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *vo, void *rest, float *lse, void *work,
 		      int bs, int n_tok, int n_heads, int n_kv_heads, int width, int v_width,
 		      const l1attn_mask *mask, int dtype, void *stream);
-int l1attn_masked_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *vo, const void *dvo, const float *lse,
+int l1attn_masked_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *vo, const void *rest, const void *dvo, const float *lse,
 		      void *dq, void *dk, void *dv, void *work,
 		      int bs, int n_tok, int n_heads, int n_kv_heads, int width, int v_width,
 		      const l1attn_mask *mask, int dtype, void *stream);

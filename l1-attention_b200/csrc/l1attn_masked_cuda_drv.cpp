@@ -73,7 +73,7 @@ struct Call {
 
 void *ptr(const torch::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// -> [vo, lse] (lse undefined unless keep), and what the backward takes: q, k, v, slopes, doc, prefix as they were used
+// -> [vo], or (keep) [vo, rest, lse] -- rest: what rounding to 16 bits left of vo, undefined in float32 -- and what the backward takes: q, k, v, slopes, doc, prefix as they were used
 std::vector<torch::Tensor> forward(torch::Tensor q, torch::Tensor k, torch::Tensor v, Maybe slopes, Maybe doc, Maybe prefix, int mode, bool causal, int64_t window,
 				   double softcap, bool keep)
 {
@@ -82,17 +82,18 @@ std::vector<torch::Tensor> forward(torch::Tensor q, torch::Tensor k, torch::Tens
 	const auto options = c.q.options().requires_grad(false);
 	auto vo = torch::empty({c.bs, c.n, c.h, c.wv}, options);
 	torch::Tensor lse = keep ? torch::empty({c.bs, c.n, c.h}, options.dtype(torch::kFloat32)) : torch::Tensor();
+	torch::Tensor rest = keep && c.type != L1ATTN_F32 ? torch::empty_like(vo) : torch::Tensor();
 	const auto work = c.work(0);
-	l1b_status(l1attn_masked_fwd(ptr(c.q), ptr(c.k), ptr(c.v), c.strides, ptr(vo), static_cast<float *>(ptr(lse)), ptr(work), c.bs, c.n, c.h, c.hk, c.w, c.wv, &c.mask, c.type,
+	l1b_status(l1attn_masked_fwd(ptr(c.q), ptr(c.k), ptr(c.v), c.strides, ptr(vo), ptr(rest), static_cast<float *>(ptr(lse)), ptr(work), c.bs, c.n, c.h, c.hk, c.w, c.wv, &c.mask, c.type,
 				     l1b_stream()),
 		   "l1attn_masked_fwd");
 	if (!keep)
 		return {vo};
-	return {vo, lse, c.q, c.k, c.v, c.slopes, c.doc, c.prefix};
+	return {vo, rest, lse, c.q, c.k, c.v, c.slopes, c.doc, c.prefix};
 }
 
 std::vector<torch::Tensor> backward(torch::Tensor q, torch::Tensor k, torch::Tensor v, Maybe slopes, Maybe doc, Maybe prefix, int mode, bool causal, int64_t window,
-				    double softcap, torch::Tensor vo, torch::Tensor lse, torch::Tensor dvo)
+				    double softcap, torch::Tensor vo, Maybe rest, torch::Tensor lse, torch::Tensor dvo)
 {
 	const Call c(q, k, v, slopes, doc, prefix, mode, causal, window, softcap);
 	TORCH_CHECK(dvo.sizes() == vo.sizes() && dvo.scalar_type() == vo.scalar_type() && dvo.device() == vo.device(), "the gradient must be like the output");
@@ -101,7 +102,7 @@ std::vector<torch::Tensor> backward(torch::Tensor q, torch::Tensor k, torch::Ten
 	const auto options = c.q.options().requires_grad(false);
 	auto dq = torch::empty(c.q.sizes(), options), dk = torch::empty(c.k.sizes(), options), dv = torch::empty(c.v.sizes(), options);
 	const auto work = c.work(1);
-	l1b_status(l1attn_masked_bwd(ptr(c.q), ptr(c.k), ptr(c.v), c.strides, ptr(vo), ptr(dvo), lse.data_ptr<float>(), ptr(dq), ptr(dk), ptr(dv), ptr(work), c.bs, c.n, c.h, c.hk,
+	l1b_status(l1attn_masked_bwd(ptr(c.q), ptr(c.k), ptr(c.v), c.strides, ptr(vo), rest.has_value() ? ptr(*rest) : nullptr, ptr(dvo), lse.data_ptr<float>(), ptr(dq), ptr(dk), ptr(dv), ptr(work), c.bs, c.n, c.h, c.hk,
 				     c.w, c.wv, &c.mask, c.type, l1b_stream()),
 		   "l1attn_masked_bwd");
 	return {dq, dk, dv};

@@ -95,6 +95,13 @@ template <> __device__ __forceinline__ float from_float(float x) { return x; }
 template <> __device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
 
+// what rounding to T leaves of a value (0 where that is not finite)
+template <typename T> __device__ __forceinline__ T rest_of(float x)
+{
+	const float rest = x - to_float(from_float<T>(x));
+	return from_float<T>(fabsf(rest) < INFINITY ? rest : 0.f);
+}
+
 // weight of a score under a row's log-normaliser; a row without any weight has -inf there
 __device__ __forceinline__ float weight_of(float x, float lse) { return lse == -INFINITY ? 0.f : expf(x - lse); }
 
@@ -114,13 +121,13 @@ __device__ __forceinline__ float finish_row(int mode, float m, float l, float *l
 
 // 16-bit types, widths up to 128: distances and products on the tensor cores
 bool masked_mma_fits(int width, int v_width, int dtype);
-int masked_mma_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st);
+int masked_mma_fwd_launch(const MaskedArgs &a, void *vo, void *rest, float *lse, int dtype, cudaStream_t st);
 // shares: [bs][n][heads][width + v_width] floats where heads are shared; e: masked_units_at_once() * masked_unit_floats() floats, or null
 long long masked_unit_floats(int n);
 long long masked_units_at_once(int bs, int n, int heads);
 int masked_mma_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, float *e, int dtype,
 			  cudaStream_t st);
-int masked_simple_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st);
+int masked_simple_fwd_launch(const MaskedArgs &a, void *vo, void *rest, float *lse, int dtype, cudaStream_t st);
 int masked_simple_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, int dtype,
 			     cudaStream_t st);
 

@@ -36,8 +36,9 @@ __global__ void doc_ranges_kernel(const int32_t *doc, DocRange *out, int n, long
 		out[tile] = {lo, hi, others, 0};
 }
 
-// delta[row] = <dvo[row], vo[row]> = sum_s p <v_s, dvo>, a warp per row; the exp form has no normaliser to differentiate
-template <typename T> __global__ void delta_kernel(const T *dvo, const T *vo, float *delta, long long rows, int width, int zero)
+// delta[row] = <dvo[row], vo[row]> = sum_s p <v_s, dvo>, a warp per row; the exp form has no normaliser to differentiate.  rest: what rounding left of vo, or
+// null (without it a row's score gradients are off by what half a step of vo makes, all alike, which shows in dq)
+template <typename T> __global__ void delta_kernel(const T *dvo, const T *vo, const T *rest, float *delta, long long rows, int width, int zero)
 {
 	const long long row = blockIdx.x * (long long)(blockDim.x / 32) + threadIdx.x / 32;
 	if (row >= rows)
@@ -45,7 +46,7 @@ template <typename T> __global__ void delta_kernel(const T *dvo, const T *vo, fl
 	float sum = 0.f;
 	if (!zero)
 		for (int w = threadIdx.x % 32; w < width; w += 32)
-			sum = fmaf(to_float(dvo[row * width + w]), to_float(vo[row * width + w]), sum);
+			sum = fmaf(to_float(dvo[row * width + w]), to_float(vo[row * width + w]) + (rest ? to_float(rest[row * width + w]) : 0.f), sum);
 #pragma unroll
 	for (int o = 16; o; o >>= 1)
 		sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -134,9 +135,9 @@ int launch_ranges(const MaskedArgs &a, void *work, cudaStream_t st)
 	return L1ATTN_OK;
 }
 
-template <typename T> void launch_delta(const MaskedArgs &a, const void *dvo, const void *vo, float *delta, long long rows, cudaStream_t st)
+template <typename T> void launch_delta(const MaskedArgs &a, const void *dvo, const void *vo, const void *rest, float *delta, long long rows, cudaStream_t st)
 {
-	delta_kernel<T><<<unsigned((rows + 7) / 8), 256, 0, st>>>(static_cast<const T *>(dvo), static_cast<const T *>(vo), delta, rows, a.v_width,
+	delta_kernel<T><<<unsigned((rows + 7) / 8), 256, 0, st>>>(static_cast<const T *>(dvo), static_cast<const T *>(vo), static_cast<const T *>(rest), delta, rows, a.v_width,
 								  a.mode == L1ATTN_SV_EXP);
 }
 
@@ -171,7 +172,7 @@ extern "C" size_t l1attn_masked_work_bytes(int bs, int n_tok, int n_heads, int n
 	return backward ? BackwardWork(bs, n_tok, n_heads, n_kv_heads, width, v_width, dtype).bytes : ranges_bytes(bs, n_tok);
 }
 
-extern "C" int l1attn_masked_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *vo, float *lse, void *work, int bs, int n_tok,
+extern "C" int l1attn_masked_fwd(const void *q, const void *k, const void *v, const int64_t *strides, void *vo, void *rest, float *lse, void *work, int bs, int n_tok,
 				 int n_heads, int n_kv_heads, int width, int v_width, const l1attn_mask *mask, int dtype, void *stream)
 {
 	MaskedArgs a;
@@ -179,15 +180,17 @@ extern "C" int l1attn_masked_fwd(const void *q, const void *k, const void *v, co
 	int rc = check(q, k, v, strides, others, 1, bs, n_tok, n_heads, n_kv_heads, width, v_width, mask, dtype, work, &a);
 	if (rc)
 		return rc > 0 ? L1ATTN_OK : rc;
-	if (!aligned(lse, 4))
+	if (!aligned(lse, 4) || !aligned(rest, dtype == L1ATTN_F32 ? 4 : 2))
 		return L1ATTN_ERR_ALIGN;
+	if (dtype == L1ATTN_F32)
+		rest = nullptr;
 	const cudaStream_t st = static_cast<cudaStream_t>(stream);
 	if ((rc = launch_ranges(a, work, st)))
 		return rc;
-	return masked_mma_fits(width, v_width, dtype) ? masked_mma_fwd_launch(a, vo, lse, dtype, st) : masked_simple_fwd_launch(a, vo, lse, dtype, st);
+	return masked_mma_fits(width, v_width, dtype) ? masked_mma_fwd_launch(a, vo, rest, lse, dtype, st) : masked_simple_fwd_launch(a, vo, rest, lse, dtype, st);
 }
 
-extern "C" int l1attn_masked_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *vo, const void *dvo, const float *lse, void *dq,
+extern "C" int l1attn_masked_bwd(const void *q, const void *k, const void *v, const int64_t *strides, const void *vo, const void *rest, const void *dvo, const float *lse, void *dq,
 				 void *dk, void *dv, void *work, int bs, int n_tok, int n_heads, int n_kv_heads, int width, int v_width, const l1attn_mask *mask,
 				 int dtype, void *stream)
 {
@@ -198,7 +201,7 @@ extern "C" int l1attn_masked_bwd(const void *q, const void *k, const void *v, co
 		return rc > 0 ? L1ATTN_OK : rc;
 	if (!lse || !work)
 		return L1ATTN_ERR_ARG;
-	if (!aligned(lse, 4))
+	if (!aligned(lse, 4) || !aligned(rest, dtype == L1ATTN_F32 ? 4 : 2))
 		return L1ATTN_ERR_ALIGN;
 	const cudaStream_t st = static_cast<cudaStream_t>(stream);
 	const long long rows = (long long)bs * n_tok * n_heads;
@@ -211,11 +214,11 @@ extern "C" int l1attn_masked_bwd(const void *q, const void *k, const void *v, co
 	if ((rc = launch_ranges(a, work, st)))
 		return rc;
 	if (dtype == L1ATTN_F32)
-		launch_delta<float>(a, dvo, vo, delta, rows, st);
+		launch_delta<float>(a, dvo, vo, nullptr, delta, rows, st);
 	else if (dtype == L1ATTN_F16)
-		launch_delta<__half>(a, dvo, vo, delta, rows, st);
+		launch_delta<__half>(a, dvo, vo, rest, delta, rows, st);
 	else
-		launch_delta<__nv_bfloat16>(a, dvo, vo, delta, rows, st);
+		launch_delta<__nv_bfloat16>(a, dvo, vo, rest, delta, rows, st);
 	L1B_LAUNCH_CHECK();
 	rc = masked_mma_fits(width, v_width, dtype) ? masked_mma_bwd_launch(a, dvo, lse, delta, dq, dk, dv, shares, e, dtype, st) :
 						      masked_simple_bwd_launch(a, dvo, lse, delta, dq, dk, dv, shares, dtype, st);

@@ -2,12 +2,13 @@
 //
 // Forward: a CTA of four warps owns 64 query rows of one head, a warp 16 of them, in registers; keys and values stream in tiles of 64 through
 // two stages of asynchronous copies.  Running softmax in registers (a row's scores lie in one quad); weights are rounded to the inputs' type for the value
-// product (11 bits, or 8 and what these leave in a second product; the normaliser sums them unrounded), everything else is float32.  Rows whose result is not
+// product, and what that leaves takes a second one (22 bits, or 16; the normaliser sums them unrounded), everything else is float32.  Rows whose result is not
 // finite are done again, exactly, by a warp each: an infinite or NaN operand spoils its neighbours in a product.
 // Bound: instruction issue of few warps.  mma.sync does not overlap float32 instructions (mma alone 8 clocks per scheduler, 13.2 with four
 // additions, 9.7 with four minima), so the softmax costs what it takes; forming the next step's distances beside it brought [2,2048,8,128] from
-// 343 to 293 us, the short copy loop a tenth; the rests of bfloat16 weights cost a tenth of it again and bring the error of dq (by its row's delta) from 1.5 to 1.35 of a
-// float32 form's that rounds at the end.  Now 52 terms per clock and SM in float16 ([4,2048,8,64], no mask: 564 us), 48 in bfloat16 ([4,2048,8,128]: 1.22 ms).
+// 343 to 293 us, the short copy loop a tenth; the weights' rests cost a tenth of it again: with
+// them, and with what rounding leaves of vo kept for delta (masked.cu), dq is as exact as a float32 form's that rounds at the end in bfloat16 (1.38 of its
+// error without).  Now 47 terms per clock and SM at widths of 64 ([4,2048,8,64], no mask: 622 us), 49 at 128 (1.20 ms).
 #include "mma.cuh"
 
 namespace l1b {
@@ -20,7 +21,7 @@ constexpr float LOG2E = 1.4426950408889634f, LAG = 8.f;
 template <typename T> constexpr float LIFT = Half2<T>::ONES == Half2<__half>::ONES ? 6.f : 0.f;
 
 // One query row, by the definition: a warp, 32 keys at a time.  Rare, so simple.
-template <typename T> __device__ __noinline__ void exact_row(const MaskedArgs &a, const MaskView &mask, int b, int head, int t, T *vo, float *lse)
+template <typename T> __device__ __noinline__ void exact_row(const MaskedArgs &a, const MaskView &mask, int b, int head, int t, T *vo, T *rest, float *lse)
 {
 	const int lane = threadIdx.x % 32, kv = head / (a.heads / a.kv_heads);
 	const T *q = static_cast<const T *>(a.q.p) + b * a.q.batch + t * a.q.tok + head * a.q.head;
@@ -74,21 +75,24 @@ template <typename T> __device__ __noinline__ void exact_row(const MaskedArgs &a
 		lse[row] = ls;
 #pragma unroll
 	for (int i = 0; i < 4; i++)
-		if (lane + 32 * i < a.v_width)
-			vo[row * a.v_width + lane + 32 * i] = from_float<T>(f == 0.f ? 0.f : acc[i] * f);
+		if (lane + 32 * i < a.v_width) {
+			const float y = f == 0.f ? 0.f : acc[i] * f;
+			vo[row * a.v_width + lane + 32 * i] = from_float<T>(y);
+			if (rest)
+				rest[row * a.v_width + lane + 32 * i] = rest_of<T>(y);
+		}
 }
 
 // W: 32-column groups of the width; V: 16-column groups of the value rows (4 or 8).  CTAs of an SM, two against three (168 registers; before the rests' products): [1,4096,8,64]
 // with values of 128 339 / 447 us, [2,2048,8,128] 293 / 472, widths of 32 200 / 235; but [1,8192,8,64] 1230 / 1157 and [4,2048,8,128] with values of 64
 // (no mask) 1179 / 1005.
 template <typename T, int W, int V>
-__global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_mma_kernel(MaskedArgs a, T *vo, float *lse, int tiles, int vec)
+__global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_mma_kernel(MaskedArgs a, T *vo, T *rest, float *lse, int tiles, int vec)
 {
 	extern __shared__ uint4 smem16[];
 	__shared__ float key_sums[KEYS];
 	using H = Half2<T>;
 	constexpr int KP = 4 * W, VP = 2 * V; // 16-byte pieces of a row
-	constexpr bool TWICE = H::ONES == Half2<__nv_bfloat16>::ONES; // what bfloat16 leaves of a weight (8 bits) takes a product of its own
 	const uint32_t base = shared_address(smem16), stage_bytes = KEYS * (KP + VP) * 16;
 	const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4;
 	const int bh = blockIdx.x % (a.bs * a.heads), tile = tiles - 1 - int(blockIdx.x / (a.bs * a.heads)); // the longest rows of a causal mask first
@@ -192,8 +196,8 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 #pragma unroll
 				for (int c = 0; c < 2; c++) {
 					const uint32_t high = p[i][2 * h + c] = H::pack(e[2 * c], e[2 * c + 1]);
-					if (TWICE) // (a bfloat16 is the upper half of its float)
-						low[i][2 * h + c] = H::pack(e[2 * c] - __uint_as_float(high << 16), e[2 * c + 1] - __uint_as_float(high & 0xffff0000u));
+					const float2 f = H::unpack(high);
+					low[i][2 * h + c] = H::pack(e[2 * c] - f.x, e[2 * c + 1] - f.y);
 				}
 			}
 #pragma unroll
@@ -204,10 +208,8 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 			for (int i = 0; i < MB; i++) {
 				H::mma(o[i][2 * vb], p[i][0], p[i][1], p[i][2], p[i][3], y[0], y[1]);
 				H::mma(o[i][2 * vb + 1], p[i][0], p[i][1], p[i][2], p[i][3], y[2], y[3]);
-				if (TWICE) {
-					H::mma(o[i][2 * vb], low[i][0], low[i][1], low[i][2], low[i][3], y[0], y[1]);
-					H::mma(o[i][2 * vb + 1], low[i][0], low[i][1], low[i][2], low[i][3], y[2], y[3]);
-				}
+				H::mma(o[i][2 * vb], low[i][0], low[i][1], low[i][2], low[i][3], y[0], y[1]);
+				H::mma(o[i][2 * vb + 1], low[i][0], low[i][1], low[i][2], low[i][3], y[2], y[3]);
 			}
 		}
 	};
@@ -365,12 +367,18 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 			const float y0 = f == 0.f ? 0.f : o[r / 2][i][2 * (r % 2)] * exp2f(-LIFT<T>) * f, y1 = f == 0.f ? 0.f : o[r / 2][i][2 * (r % 2) + 1] * exp2f(-LIFT<T>) * f;
 			odd |= !(fabsf(y0) < INFINITY) || !(fabsf(y1) < INFINITY);
 			if (t < a.n && w < a.v_width) {
+				const long long at = row * a.v_width + w;
 				if (vec & 8)
-					*reinterpret_cast<uint32_t *>(vo + row * a.v_width + w) = H::pack(y0, y1);
+					*reinterpret_cast<uint32_t *>(vo + at) = H::pack(y0, y1);
 				else {
-					vo[row * a.v_width + w] = from_float<T>(y0);
+					vo[at] = from_float<T>(y0);
 					if (w + 1 < a.v_width)
-						vo[row * a.v_width + w + 1] = from_float<T>(y1);
+						vo[at + 1] = from_float<T>(y1);
+				}
+				if (rest) {
+					rest[at] = rest_of<T>(y0);
+					if (w + 1 < a.v_width)
+						rest[at + 1] = rest_of<T>(y1);
 				}
 			}
 		}
@@ -385,7 +393,7 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 	for (int r = 0; r < 16 * MB; r++) {
 		const int t = t0 + 16 * MB * warp + r;
 		if (t < a.n && (again >> r & 1u))
-			exact_row<T>(a, mask, b, head, t, vo, lse);
+			exact_row<T>(a, mask, b, head, t, vo, rest, lse);
 	}
 }
 
@@ -492,8 +500,9 @@ template <int W, int KP> __device__ __forceinline__ void encode_tile(unsigned ch
 
 // acc[column block][own rows 0-7, 8-15] += signs(own - streamed) e of 16 own rows and 16 streamed ones (rows `first` of the tile at xs); the products' rows
 // are columns w, their columns own rows.  coded: both sides are codes, and signs one too large; else streamed values, and own ones of `plain` for bfloat16.
-template <typename T, int W>
-__device__ __forceinline__ void add_signed(float (&acc)[2 * W][2][4], const uint32_t (&eb)[2][2], bool coded, uint32_t xs, int first, const unsigned char *table,
+// TWICE: what rounding left of e (el) takes a product of its own, with the same signs; not for codes.
+template <typename T, int W, bool TWICE>
+__device__ __forceinline__ void add_signed(float (&acc)[2 * W][2][4], const uint32_t (&eb)[2][2], const uint32_t (&el)[2][2], bool coded, uint32_t xs, int first, const unsigned char *table,
 					   const uint16_t *plain, int warp, int lane)
 {
 	using H = Half2<T>;
@@ -527,6 +536,7 @@ __device__ __forceinline__ void add_signed(float (&acc)[2 * W][2][4], const uint
 #pragma unroll
 		for (int half = 0; half < 2; half++) {
 			const uint32_t b0 = g == r ? eb[half][0] : 0u, b1 = g == r ? eb[half][1] : 0u;
+			const uint32_t l0 = TWICE && g == r ? el[half][0] : 0u, l1 = TWICE && g == r ? el[half][1] : 0u;
 			const uint16_t *row = plain + (16 * warp + r + 8 * half) * 32 * W + g;
 #pragma unroll
 			for (int wb = 0; wb < WB; wb += 2) {
@@ -535,9 +545,14 @@ __device__ __forceinline__ void add_signed(float (&acc)[2 * W][2][4], const uint
 					w = make_uint4(row[16 * wb] * 0x10001u, row[16 * wb + 8] * 0x10001u, row[16 * wb + 16] * 0x10001u, row[16 * wb + 24] * 0x10001u);
 				else
 					w = *reinterpret_cast<const uint4 *>(twice + own_word<W>(16 * warp + r + 8 * half, g, 2 * wb));
-				Half2<__half>::mma(acc[wb][half], H::sign(w.x, x[wb][0]), H::sign(w.y, x[wb][1]), H::sign(w.x, x[wb][2]), H::sign(w.y, x[wb][3]), b0, b1);
-				Half2<__half>::mma(acc[wb + 1][half], H::sign(w.z, x[wb + 1][0]), H::sign(w.w, x[wb + 1][1]), H::sign(w.z, x[wb + 1][2]),
-						   H::sign(w.w, x[wb + 1][3]), b0, b1);
+				const uint32_t s0[4] = {H::sign(w.x, x[wb][0]), H::sign(w.y, x[wb][1]), H::sign(w.x, x[wb][2]), H::sign(w.y, x[wb][3])};
+				const uint32_t s1[4] = {H::sign(w.z, x[wb + 1][0]), H::sign(w.w, x[wb + 1][1]), H::sign(w.z, x[wb + 1][2]), H::sign(w.w, x[wb + 1][3])};
+				Half2<__half>::mma(acc[wb][half], s0[0], s0[1], s0[2], s0[3], b0, b1);
+				Half2<__half>::mma(acc[wb + 1][half], s1[0], s1[1], s1[2], s1[3], b0, b1);
+				if (TWICE) {
+					Half2<__half>::mma(acc[wb][half], s0[0], s0[1], s0[2], s0[3], l0, l1);
+					Half2<__half>::mma(acc[wb + 1][half], s1[0], s1[1], s1[2], s1[3], l0, l1);
+				}
 			}
 		}
 }
@@ -627,7 +642,7 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 	__shared__ float sums[STREAM], stats[2][2][STREAM]; // [stage][log-normaliser, delta] of streamed queries
 	using H = Half2<T>;
 	constexpr int KP = W == 3 ? 16 : 4 * W, VP = 2 * V, WB = 2 * W; // 16-byte pieces of a row; 16-column blocks
-	constexpr bool CODES = H::ONES == Half2<__nv_bfloat16>::ONES;
+	constexpr bool CODES = H::ONES == Half2<__nv_bfloat16>::ONES, TWICE = !CODES && !OWN_KEYS;
 	constexpr uint32_t OWN_Y = ROWS * 64 * W * 2, STAGES = OWN_Y + ROWS * VP * 16, STAGE = STREAM * (KP + VP) * 16, OWN_X = STAGES + 2 * STAGE, CODED = OWN_X + ROWS * 64 * W;
 	unsigned char *const smem = reinterpret_cast<unsigned char *>(smem16);
 	const uint32_t base = shared_address(smem16);
@@ -829,10 +844,16 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 				}
 			if (__any_sync(0xffffffffu, grew))
 				follow_largest<W>(e, unit, limit, e_sum, acc, j);
-			uint32_t eb[2][2]; // [own row g, g + 8][streamed 0-7, 8-15]
+			uint32_t eb[2][2], el[2][2] = {}; // [own row g, g + 8][streamed 0-7, 8-15]; el: what rounding left
 #pragma unroll
-			for (int i = 0; i < 4; i++)
-				eb[i / 2][i % 2] = Half2<__half>::pack(e[i % 2][i / 2 * 2] * unit[i / 2], e[i % 2][i / 2 * 2 + 1] * unit[i / 2]);
+			for (int i = 0; i < 4; i++) {
+				const float e0 = e[i % 2][i / 2 * 2] * unit[i / 2], e1 = e[i % 2][i / 2 * 2 + 1] * unit[i / 2];
+				eb[i / 2][i % 2] = Half2<__half>::pack(e0, e1);
+				if (TWICE) {
+					const float2 f = Half2<__half>::unpack(eb[i / 2][i % 2]);
+					el[i / 2][i % 2] = Half2<__half>::pack(e0 - f.x, e1 - f.y);
+				}
+			}
 			if (OWN_KEYS && parts.e) { // for the queries' kernel: [unit][t][s]
 				float *const to = parts.e + unit_bh * parts.unit_floats + (long long)(r0 + 16 * kb + 2 * j) * parts.pitch + oa;
 #pragma unroll
@@ -859,7 +880,7 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 			const bool coded = CODES && !off;
 			if (coded) // (one product: e as A, ones as B)
 				Half2<__half>::mma(e_sum, eb[0][0], eb[1][0], eb[0][1], eb[1][1], Half2<__half>::ONES, Half2<__half>::ONES);
-			add_signed<T, W>(acc, eb, coded, coded ? base + CODED : xs, 16 * kb, smem, reinterpret_cast<const uint16_t *>(smem + OWN_X), warp, lane);
+			add_signed<T, W, TWICE>(acc, eb, el, coded, coded ? base + CODED : xs, 16 * kb, smem, reinterpret_cast<const uint16_t *>(smem + OWN_X), warp, lane);
 		}
 		it = following;
 		stage ^= 1;
@@ -905,7 +926,7 @@ __global__ void __launch_bounds__(THREADS, 3) masked_dq_mma_kernel(MaskedArgs a,
 {
 	extern __shared__ uint4 smem16[];
 	constexpr int KP = W == 3 ? 16 : 4 * W, WB = 2 * W;
-	constexpr bool CODES = Half2<T>::ONES == Half2<__nv_bfloat16>::ONES;
+	constexpr bool CODES = Half2<T>::ONES == Half2<__nv_bfloat16>::ONES, TWICE = !CODES; // (float16: dq to 22 bits of e, else 1.55 of the error of a float32 form rounded at the end)
 	constexpr uint32_t STAGES = ROWS * 128 * W, STAGE = STREAM * KP * 16, OWN_X = STAGES + 2 * STAGE, CODED = OWN_X + ROWS * 64 * W, FROM = CODES ? OWN_X : STAGES;
 	unsigned char *const smem = reinterpret_cast<unsigned char *>(smem16);
 	const uint32_t base = shared_address(smem16);
@@ -975,14 +996,20 @@ __global__ void __launch_bounds__(THREADS, 3) masked_dq_mma_kernel(MaskedArgs a,
 				}
 				if (__any_sync(0xffffffffu, grew))
 					follow_largest<W>(e, unit, limit, e_sum, acc, j);
-				uint32_t eb[2][2];
+				uint32_t eb[2][2], el[2][2] = {};
 #pragma unroll
-				for (int i = 0; i < 4; i++)
-					eb[i / 2][i % 2] = Half2<__half>::pack(e[i % 2][i / 2 * 2] * unit[i / 2], e[i % 2][i / 2 * 2 + 1] * unit[i / 2]);
+				for (int i = 0; i < 4; i++) {
+					const float e0 = e[i % 2][i / 2 * 2] * unit[i / 2], e1 = e[i % 2][i / 2 * 2 + 1] * unit[i / 2];
+					eb[i / 2][i % 2] = Half2<__half>::pack(e0, e1);
+					if (TWICE) {
+						const float2 f = Half2<__half>::unpack(eb[i / 2][i % 2]);
+						el[i / 2][i % 2] = Half2<__half>::pack(e0 - f.x, e1 - f.y);
+					}
+				}
 				const bool coded = CODES && !off;
 				if (coded)
 					Half2<__half>::mma(e_sum, eb[0][0], eb[1][0], eb[0][1], eb[1][1], Half2<__half>::ONES, Half2<__half>::ONES);
-				add_signed<T, W>(acc, eb, coded, coded ? base + CODED : base + STAGES + stage * STAGE, 16 * kb, smem, reinterpret_cast<const uint16_t *>(smem + OWN_X), warp, lane);
+				add_signed<T, W, TWICE>(acc, eb, el, coded, coded ? base + CODED : base + STAGES + stage * STAGE, 16 * kb, smem, reinterpret_cast<const uint16_t *>(smem + OWN_X), warp, lane);
 			}
 		it = following;
 		stage ^= 1;
@@ -1031,7 +1058,7 @@ int bwd(const MaskedArgs &a, const void *dvo_, const float *lse, const float *de
 	return L1ATTN_OK;
 }
 
-template <typename T, int W, int V> int fwd(const MaskedArgs &a, void *vo, float *lse, int vec, cudaStream_t st)
+template <typename T, int W, int V> int fwd(const MaskedArgs &a, void *vo, void *rest, float *lse, int vec, cudaStream_t st)
 {
 	constexpr int bytes = 2 * KEYS * (4 * W + 2 * V) * 16;
 	static_assert(bytes >= ROWS * 4 * W * 16 && MB * 16 <= 32, "the query rows pass through the stages");
@@ -1040,7 +1067,7 @@ template <typename T, int W, int V> int fwd(const MaskedArgs &a, void *vo, float
 	if (grid > 0x7fffffffll)
 		return L1ATTN_ERR_SHAPE;
 	L1B_SHARED_MEMORY((masked_fwd_mma_kernel<T, W, V>), bytes);
-	masked_fwd_mma_kernel<T, W, V><<<unsigned(grid), THREADS, bytes, st>>>(a, static_cast<T *>(vo), lse, tiles, vec);
+	masked_fwd_mma_kernel<T, W, V><<<unsigned(grid), THREADS, bytes, st>>>(a, static_cast<T *>(vo), static_cast<T *>(rest), lse, tiles, vec);
 	L1B_LAUNCH_CHECK();
 	return L1ATTN_OK;
 }
@@ -1048,12 +1075,12 @@ template <typename T, int W, int V> int fwd(const MaskedArgs &a, void *vo, float
 // rows of 16-byte vectors: what asynchronous copies need
 bool vectors(const Strided &x) { return aligned(x.p, 16) && x.batch % 8 == 0 && x.tok % 8 == 0 && x.head % 8 == 0; }
 
-template <typename T> int fwd_type(const MaskedArgs &a, void *vo, float *lse, cudaStream_t st)
+template <typename T> int fwd_type(const MaskedArgs &a, void *vo, void *rest, float *lse, cudaStream_t st)
 {
 	const int vec = vectors(a.q) | vectors(a.k) << 1 | vectors(a.v) << 2 | (aligned(vo, 4) && a.v_width % 2 == 0) << 3, w = (a.width + 31) / 32;
 	if (a.v_width <= 64)
-		return w == 1 ? fwd<T, 1, 4>(a, vo, lse, vec, st) : w == 2 ? fwd<T, 2, 4>(a, vo, lse, vec, st) : w == 3 ? fwd<T, 3, 4>(a, vo, lse, vec, st) : fwd<T, 4, 4>(a, vo, lse, vec, st);
-	return w == 1 ? fwd<T, 1, 8>(a, vo, lse, vec, st) : w == 2 ? fwd<T, 2, 8>(a, vo, lse, vec, st) : w == 3 ? fwd<T, 3, 8>(a, vo, lse, vec, st) : fwd<T, 4, 8>(a, vo, lse, vec, st);
+		return w == 1 ? fwd<T, 1, 4>(a, vo, rest, lse, vec, st) : w == 2 ? fwd<T, 2, 4>(a, vo, rest, lse, vec, st) : w == 3 ? fwd<T, 3, 4>(a, vo, rest, lse, vec, st) : fwd<T, 4, 4>(a, vo, rest, lse, vec, st);
+	return w == 1 ? fwd<T, 1, 8>(a, vo, rest, lse, vec, st) : w == 2 ? fwd<T, 2, 8>(a, vo, rest, lse, vec, st) : w == 3 ? fwd<T, 3, 8>(a, vo, rest, lse, vec, st) : fwd<T, 4, 8>(a, vo, rest, lse, vec, st);
 }
 
 template <typename T>
@@ -1071,9 +1098,9 @@ int bwd_type(const MaskedArgs &a, const void *dvo, const float *lse, const float
 
 bool masked_mma_fits(int width, int v_width, int dtype) { return dtype != L1ATTN_F32 && width <= 128 && v_width <= 128; }
 
-int masked_mma_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st)
+int masked_mma_fwd_launch(const MaskedArgs &a, void *vo, void *rest, float *lse, int dtype, cudaStream_t st)
 {
-	return dtype == L1ATTN_F16 ? fwd_type<__half>(a, vo, lse, st) : fwd_type<__nv_bfloat16>(a, vo, lse, st);
+	return dtype == L1ATTN_F16 ? fwd_type<__half>(a, vo, rest, lse, st) : fwd_type<__nv_bfloat16>(a, vo, rest, lse, st);
 }
 
 

@@ -127,7 +127,7 @@ template <int J> __device__ __forceinline__ void products(const float *A, const 
 	}
 }
 
-template <typename T, int NV, int KEYS> __global__ void __launch_bounds__(THREADS) masked_fwd_simple_kernel(MaskedArgs a, T *vo, float *lse, int tiles)
+template <typename T, int NV, int KEYS> __global__ void __launch_bounds__(THREADS) masked_fwd_simple_kernel(MaskedArgs a, T *vo, T *rest, float *lse, int tiles)
 {
 	extern __shared__ float4 smem4[];
 	const int wp = pitch(a.width), vp = 64 * NV, tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
@@ -239,8 +239,12 @@ template <typename T, int NV, int KEYS> __global__ void __launch_bounds__(THREAD
 #pragma unroll
 		for (int c = 0; c < 4 * NV; c++) {
 			const int w = 64 * (c / 4) + 4 * tx + c % 4;
-			if (w < a.v_width)
-				vo[row * a.v_width + w] = from_float<T>(f == 0.f ? 0.f : acc[i][c] * f);
+			if (w < a.v_width) {
+				const float y = f == 0.f ? 0.f : acc[i][c] * f;
+				vo[row * a.v_width + w] = from_float<T>(y);
+				if (rest)
+					rest[row * a.v_width + w] = rest_of<T>(y);
+			}
 		}
 	}
 }
@@ -379,23 +383,23 @@ int grid_of(long long n, unsigned *out)
 
 inline int fwd_bytes(int width, int nv, int keys) { return 4 * ((OWN + keys) * pitch(width) + keys * 64 * nv + OWN * (keys + 4)); }
 
-template <typename T, int NV, int KEYS> int fwd_tiles(const MaskedArgs &a, void *vo, float *lse, cudaStream_t st)
+template <typename T, int NV, int KEYS> int fwd_tiles(const MaskedArgs &a, void *vo, void *rest, float *lse, cudaStream_t st)
 {
 	const int tiles = (a.n + OWN - 1) / OWN, bytes = fwd_bytes(a.width, NV, KEYS);
 	unsigned grid = 0;
 	if (int rc = grid_of((long long)tiles * a.heads * a.bs, &grid))
 		return rc;
 	L1B_SHARED_MEMORY((masked_fwd_simple_kernel<T, NV, KEYS>), bytes);
-	masked_fwd_simple_kernel<T, NV, KEYS><<<grid, THREADS, bytes, st>>>(a, static_cast<T *>(vo), lse, tiles);
+	masked_fwd_simple_kernel<T, NV, KEYS><<<grid, THREADS, bytes, st>>>(a, static_cast<T *>(vo), static_cast<T *>(rest), lse, tiles);
 	L1B_LAUNCH_CHECK();
 	return L1ATTN_OK;
 }
 
 // Tiles of 32 keys where two CTAs of them fit an SM and two of 64 keys do not, else of 64.  64 against 32: [2,2048,8,64], causal, 402 / 474 us,
 // [3,501,6,65] with values of 40 94 / 117, [1,1000,8,200] 378 / 440 (one CTA either way); but [2,2048,8,128] 865 / 725.
-template <typename T, int NV> int fwd(const MaskedArgs &a, void *vo, float *lse, cudaStream_t st)
+template <typename T, int NV> int fwd(const MaskedArgs &a, void *vo, void *rest, float *lse, cudaStream_t st)
 {
-	return fwd_bytes(a.width, NV, 64) > 113 * 1024 && fwd_bytes(a.width, NV, 32) <= 113 * 1024 ? fwd_tiles<T, NV, 32>(a, vo, lse, st) : fwd_tiles<T, NV, 64>(a, vo, lse, st);
+	return fwd_bytes(a.width, NV, 64) > 113 * 1024 && fwd_bytes(a.width, NV, 32) <= 113 * 1024 ? fwd_tiles<T, NV, 32>(a, vo, rest, lse, st) : fwd_tiles<T, NV, 64>(a, vo, rest, lse, st);
 }
 
 template <typename T, typename OUT, bool OWN_KEYS, int NW, int NV>
@@ -422,12 +426,12 @@ int bwd(const MaskedArgs &a, const void *dvo, const float *lse, const float *del
 	return bwd_one<T, T, true, NW, NV>(a, dvo, lse, delta, static_cast<T *>(dk), static_cast<T *>(dv), st);
 }
 
-template <typename T> int fwd_type(const MaskedArgs &a, void *vo, float *lse, cudaStream_t st)
+template <typename T> int fwd_type(const MaskedArgs &a, void *vo, void *rest, float *lse, cudaStream_t st)
 {
 	if constexpr (sizeof(T) == 2) // (smaller ones of 16 bits are done on the tensor cores)
-		return fwd<T, 4>(a, vo, lse, st);
+		return fwd<T, 4>(a, vo, rest, lse, st);
 	else
-	return a.v_width <= 64 ? fwd<T, 1>(a, vo, lse, st) : a.v_width <= 128 ? fwd<T, 2>(a, vo, lse, st) : fwd<T, 4>(a, vo, lse, st);
+	return a.v_width <= 64 ? fwd<T, 1>(a, vo, rest, lse, st) : a.v_width <= 128 ? fwd<T, 2>(a, vo, rest, lse, st) : fwd<T, 4>(a, vo, rest, lse, st);
 }
 // columns a thread, for the width and for the values: 32, 64, 96, 128, 256 columns in all
 template <typename T, int NW>
@@ -449,10 +453,10 @@ int bwd_type(const MaskedArgs &a, const void *dvo, const float *lse, const float
 
 } // namespace
 
-int masked_simple_fwd_launch(const MaskedArgs &a, void *vo, float *lse, int dtype, cudaStream_t st)
+int masked_simple_fwd_launch(const MaskedArgs &a, void *vo, void *rest, float *lse, int dtype, cudaStream_t st)
 {
-	return dtype == L1ATTN_F32 ? fwd_type<float>(a, vo, lse, st) : dtype == L1ATTN_F16 ? fwd_type<__half>(a, vo, lse, st) :
-											     fwd_type<__nv_bfloat16>(a, vo, lse, st);
+	return dtype == L1ATTN_F32 ? fwd_type<float>(a, vo, rest, lse, st) : dtype == L1ATTN_F16 ? fwd_type<__half>(a, vo, rest, lse, st) :
+											     fwd_type<__nv_bfloat16>(a, vo, rest, lse, st);
 }
 
 int masked_simple_bwd_launch(const MaskedArgs &a, const void *dvo, const float *lse, const float *delta, void *dq, void *dk, void *dv, float *shares, int dtype,

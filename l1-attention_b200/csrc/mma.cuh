@@ -23,6 +23,7 @@ template <> struct Half2<__half> {
 		asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
 		return d;
 	}
+	static __device__ __forceinline__ float2 unpack(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2 *>(&x)); }
 	static __device__ __forceinline__ uint32_t pack(float lo, float hi)
 	{
 		uint32_t d;
@@ -57,6 +58,7 @@ template <> struct Half2<__nv_bfloat16> {
 		asm("min.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
 		return d;
 	}
+	static __device__ __forceinline__ float2 unpack(uint32_t x) { return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)); }
 	static __device__ __forceinline__ uint32_t pack(float lo, float hi)
 	{
 		uint32_t d;

@@ -38,8 +38,8 @@ SIGNATURES = {
     "l1attn_dense_bwd_scratch_bytes": (_sz, [_i] * 5),
     "l1attn_dense_bwd": (_i, [_vp] * 6 + [_i] * 5 + [_vp]),
     "l1attn_masked_work_bytes": (_sz, [_i] * 8),
-    "l1attn_masked_fwd": (_i, [_vp] * 7 + [_i] * 6 + [_vp, _i, _vp]),
-    "l1attn_masked_bwd": (_i, [_vp] * 11 + [_i] * 6 + [_vp, _i, _vp]),
+    "l1attn_masked_fwd": (_i, [_vp] * 8 + [_i] * 6 + [_vp, _i, _vp]),
+    "l1attn_masked_bwd": (_i, [_vp] * 12 + [_i] * 6 + [_vp, _i, _vp]),
     "l1attn_cache_append": (_i, [_vp] * 4 + [_i] * 2 + [_vp]),
     "l1attn_cache_gather": (_i, [_vp] * 3 + [_i] * 2 + [_vp]),
     "l1attn_cache_copy_pages": (_i, [_vp, _i, _vp, _vp, _i, _vp]),

@@ -16,10 +16,10 @@ zeros, and gradients of zero.  A key whose weight is zero contributes nothing, w
 
 Heads of queries may share heads of keys and values (h a multiple of hk).  float32, float16 and bfloat16; widths up to 256.  q, k, v may
 be strided views (of one projection, say) with contiguous rows; others are copied.  The output and the gradients are contiguous.
-Differentiable in q, k and v (sign(0) = 0); the backward is deterministic and keeps one float per query and head beside its inputs; while it
-runs it takes up to a gigabyte in 16 bits (a float per pair), and a float per query head and element of k and v where heads are shared.
-In 16 bits, weights are rounded for the value products (to 11 bits, or 2^-31 of the row's largest, in float16; to 16 in bfloat16, 8 for dv) and score gradients to 11 bits or
-2^-25 of their row's largest; scores, normalisers and all sums are float32.
+Differentiable in q, k and v (sign(0) = 0); the backward is deterministic and keeps one float per query and head beside its inputs, and in 16 bits what rounding
+left of the output; while it runs it takes up to a gigabyte in 16 bits (a float per pair), and a float per query head and element of k and v where heads are shared.
+In 16 bits, weights are rounded for the value products (to 22 bits, or 2^-31 of the row's largest, in float16; to 16 in bfloat16; to 11 and 8 for dv)
+and score gradients to 11 bits or 2^-25 of their row's largest (dq in float16: 22); scores, normalisers and all sums are float32.
 Everything runs on the tensors' device and the current stream.  No CPU path.  A backward that is captured into a CUDA graph must not share its leaves with an
 eager graph that is still alive: autograd ties a leaf to the stream of its first use (detach or drop the eager outputs before the capture).
 """
@@ -53,15 +53,15 @@ class L1AttnMaskedFn(torch.autograd.Function):
     def forward(ctx, q, k, v, slopes=None, doc=None, prefix=None, mode="softmax", causal=True, window=0, softcap=0.0):
         ctx.options = _options(mode, causal, window, softcap)
         _tensors(q=q, k=k, v=v, slopes=slopes, doc=doc, prefix=prefix)
-        vo, lse, *used = l1attn_masked_cuda_drv.forward(q, k, v, slopes, doc, prefix, *ctx.options, True)
-        ctx.save_for_backward(*used, vo, lse)
+        vo, rest, lse, *used = l1attn_masked_cuda_drv.forward(q, k, v, slopes, doc, prefix, *ctx.options, True)
+        ctx.save_for_backward(*used, vo, rest, lse)
         return vo
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dvo):
-        *used, vo, lse = ctx.saved_tensors
-        return (*l1attn_masked_cuda_drv.backward(*used, *ctx.options, vo, lse, dvo),) + (None,) * 7
+        *used, vo, rest, lse = ctx.saved_tensors
+        return (*l1attn_masked_cuda_drv.backward(*used, *ctx.options, vo, rest, lse, dvo),) + (None,) * 7
 
 
 class L1AttnMasked(torch.nn.Module):

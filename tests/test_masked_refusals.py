@@ -12,7 +12,7 @@ def _call(back=False, **change):
     lib = l1attn_cabi.lib()
     buf = (ctypes.c_double * 64)()
     p = ctypes.addressof(buf)
-    a = dict(q=p, k=p, v=p, strides=(ctypes.c_int64 * 9)(*[8] * 9), vo=p, dvo=p, lse=p, dq=p, dk=p, dv=p, work=p, bs=1, n=2, h=2, hk=1, w=4, wv=4, dtype=l1attn_cabi.BF16)
+    a = dict(q=p, k=p, v=p, strides=(ctypes.c_int64 * 9)(*[8] * 9), vo=p, rest=p, dvo=p, lse=p, dq=p, dk=p, dv=p, work=p, bs=1, n=2, h=2, hk=1, w=4, wv=4, dtype=l1attn_cabi.BF16)
     m = dict(mode="softmax", causal=True, window=0, softcap=0.0)
     m.update({x: change.pop(x) for x in list(change) if x in m})
     mask = l1attn_cabi.Mask(**m)
@@ -23,8 +23,8 @@ def _call(back=False, **change):
     sizes = [a[x] for x in ("bs", "n", "h", "hk", "w", "wv")]
     tail = sizes + [None if a.get("no_mask") else ctypes.byref(mask), a["dtype"], None]
     if back:
-        return lib.l1attn_masked_bwd(a["q"], a["k"], a["v"], a["strides"], a["vo"], a["dvo"], a["lse"], a["dq"], a["dk"], a["dv"], a["work"], *tail)
-    return lib.l1attn_masked_fwd(a["q"], a["k"], a["v"], a["strides"], a["vo"], a["lse"], a["work"], *tail)
+        return lib.l1attn_masked_bwd(a["q"], a["k"], a["v"], a["strides"], a["vo"], a["rest"], a["dvo"], a["lse"], a["dq"], a["dk"], a["dv"], a["work"], *tail)
+    return lib.l1attn_masked_fwd(a["q"], a["k"], a["v"], a["strides"], a["vo"], a["rest"], a["lse"], a["work"], *tail)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -40,7 +40,7 @@ def test_abi_refusals(change, code):
 def test_abi_alignment_and_empty():
     buf = (ctypes.c_double * 8)()
     p = ctypes.addressof(buf)
-    assert _call(q=p + 1) == -6 and _call(vo=p + 1) == -6 and _call(lse=p + 2) == -6 and _call(back=True, dk=p + 1) == -6
+    assert _call(rest=p + 1) == -6 and _call(back=True, rest=p + 1) == -6 and _call(q=p + 1) == -6 and _call(vo=p + 1) == -6 and _call(lse=p + 2) == -6 and _call(back=True, dk=p + 1) == -6
     assert _call(dtype=l1attn_cabi.F32, k=p + 2) == -6
     assert _call(back=True, work=None) == -1 and _call(back=True, lse=None) == -1
     assert _call(bs=0) == 0 and _call(n=0) == 0 and _call(back=True, bs=0) == 0
