@@ -11,6 +11,9 @@
 // take runs of its chunks and join at the end.  The chunks of all units -- a tile of query rows and a head of keys and values -- lie behind one
 // another, and every CTA of one wave takes an equal share, whatever the lengths (known on the device alone): a unit may end in a later CTA's share, and
 // is joined by join_splits_kernel.
+// Bound: instruction issue, 55 % of the slots with 12 warps an SM (168 registers); what every chunk costs (copies, unpacking, weights) is half of it, a query
+// row a tenth or so.  Widths of 128: 37 sequences of 16384 tokens, one query head 269 us (72 % of the rate of a copy), four 406 (47 %); 64 ragged
+// ones of up to 8192, one 138 us, four 202, eight 289.
 #include "cache.cuh"
 #include "mma.cuh"
 

