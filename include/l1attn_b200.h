@@ -190,7 +190,7 @@ typedef struct l1attn_mask {
 	int causal;            /* 0 or 1 */
 	int window;            /* 0: none */
 	int mode;              /* L1ATTN_SV_* */
-	float softcap;         /* 0: none */
+	float softcap;         /* 0: none; else 1e-30 to 1e30 */
 	const float *slopes;   /* device, [n_heads], or NULL: no bias */
 	const int32_t *doc;    /* device, [bs][n_tok] document of each token, negative: padding; or NULL: one document */
 	const int32_t *prefix; /* device, [bs] length of the prefix that every query sees, or NULL: none */

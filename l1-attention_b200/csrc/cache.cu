@@ -132,8 +132,8 @@ extern "C" int l1attn_cache_attend(const l1attn_cache *cache, const void *q, con
 	const int rc = check(cache, rows, dtype, true, &a.c);
 	if (rc < 0)
 		return rc;
-	if (!mask || !strides || n_heads < 1 || n_heads % cache->n_kv_heads || mask->mode < 0 || mask->mode > 2 || mask->window < 0 || !(mask->softcap >= 0.f) ||
-	    std::isinf(mask->softcap) || !mask->causal || mask->doc || mask->prefix || strides[0] < 0 || strides[1] < 0)
+	if (!mask || !strides || n_heads < 1 || n_heads % cache->n_kv_heads || mask->mode < 0 || mask->mode > 2 || mask->window < 0 || !cap_fits(mask->softcap) ||
+	    !mask->causal || mask->doc || mask->prefix || strides[0] < 0 || strides[1] < 0)
 		return L1ATTN_ERR_ARG;
 	if (rc > 0)
 		return L1ATTN_OK;

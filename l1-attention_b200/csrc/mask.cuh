@@ -36,6 +36,9 @@ struct MaskedArgs {
 	const DocRange *ranges;
 };
 
+// (a cap whose reciprocal is no float32 would give NaN, or no cap at all)
+inline bool cap_fits(float cap) { return cap == 0.f || (cap >= 1e-30f && cap <= 1e30f); }
+
 // What one batch item's masks say.
 struct MaskView {
 	int n, causal, window, prefix;

@@ -92,7 +92,7 @@ int check(const void *q, const void *k, const void *v, const int64_t *strides, c
 		return L1ATTN_ERR_ARG;
 	if (dtype != L1ATTN_F32 && dtype != L1ATTN_F16 && dtype != L1ATTN_BF16)
 		return L1ATTN_ERR_ARG;
-	if (mask->mode < 0 || mask->mode > 2 || mask->window < 0 || !(mask->softcap >= 0.f) || std::isinf(mask->softcap))
+	if (mask->mode < 0 || mask->mode > 2 || mask->window < 0 || !cap_fits(mask->softcap))
 		return L1ATTN_ERR_ARG;
 	if (width > 256 || v_width > 256 || n_tok > 1 << 30) // (ends of tiles stay within int)
 		return L1ATTN_ERR_SHAPE;

@@ -37,8 +37,8 @@ def _options(mode, causal, window, softcap):
         raise ValueError("mode must be one of %s" % (MODES,))
     if isinstance(window, bool) or int(window) != window or not 0 <= window < 1 << 31:
         raise ValueError("window must be a whole number, 0 for none")
-    if not 0.0 <= float(softcap) < float("inf"):
-        raise ValueError("softcap must be finite and not negative, 0 for none")
+    if float(softcap) != 0.0 and not 1e-30 <= float(softcap) <= 1e30:
+        raise ValueError("softcap must be 0 (none) or from 1e-30 to 1e30")
     return SV_MODES[mode], bool(causal), int(window), float(softcap)
 
 

@@ -74,6 +74,18 @@ def test_abi_refuses_what_no_kernel_covers():
     for back in (False, True):
         assert _call(back=back, h=0) == -1 and _call(back=back, h=0, hk=0) == 0
         assert _call(back=back, n=(1 << 30) + 1) == -2
+        assert _call(back=back, softcap=1e-40) == _call(back=back, softcap=1e31) == -1  # (a reciprocal that is no float32)
+
+
+def test_caps_without_a_reciprocal_are_refused():
+    from l1attn_cache_cuda import attend
+    from l1attn_masked_cuda import L1AttnMasked
+    x = torch.zeros(1)
+    for cap in (1e-50, 1e-40, 1e31, 1e300):
+        with pytest.raises(ValueError):
+            L1AttnMasked(softcap=cap)
+        with pytest.raises(ValueError):
+            attend(x, x, x, x, x, x, x, x, softcap=cap)
 
 
 @pytest.mark.gpu
