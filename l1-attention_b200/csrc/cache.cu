@@ -45,14 +45,15 @@ int plan(AttendArgs *a, int rows, int heads, int max_len, int dtype, size_t *byt
 	if ((long long)rows * heads > 0x7fffffffll)
 		return L1ATTN_ERR_SHAPE;
 	const size_t part = (a->c.v_width + 2) * sizeof(float);
-	if (attend_mma_fits(a->c.width, a->c.v_width, dtype)) { // one wave of CTAs that share the chunks; at least 16 chunks each
+	if (attend_mma_fits(a->c.width, a->c.v_width, dtype)) { // one wave of CTAs that share the chunks; a unit's costs count as some (cache_attend_mma.cu)
 		// eight rows cost half of sixteen; sequences of one token have as many rows as a group has heads
 		a->tile_rows = (long long)rows * a->group / a->c.n_seqs <= 8 ? 8 : 16;
 		int sms = 0;
 		if (int rc = multiprocessors(&sms))
 			return rc;
 		a->ctas = attend_mma_ctas(a->tile_rows, sms);
-		a->least = 16;
+		// fewest chunks of a CTA, 6 against 16 and 44: 4 sequences of 1000 tokens 22.8 / 26.4 / 40.6 us, 16 of up to 300 23.5 / 26.8 / 44.4; 3 is no better
+		a->least = 6;
 		a->splits = 1;
 		*bytes = (2ull * a->ctas * a->tile_rows * part + 255) / 256 * 256 + a->ctas * sizeof(AttendSplit);
 		return L1ATTN_OK;
