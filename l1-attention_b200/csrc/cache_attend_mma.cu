@@ -80,7 +80,7 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 	const CacheArgs &c = a.c;
 	unsigned char *const smem = reinterpret_cast<unsigned char *>(smem16);
 	const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4;
-	const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
+	const float inv_cap = a.cap > 0.f ? 2.f * LOG2E / a.cap : 0.f; // as tanh_of_exponent takes it
 
 	// all sequences' chunks, and this CTA's share of them
 	auto weigh = [&](int i, SeqView *view) {
@@ -390,7 +390,7 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 							const int s = s0 + 16 * n + g + 8 * (e / 2), t = t_of[i][e & 1];
 							float y = x[n][i][e];
 							if (a.cap > 0.f)
-								y = a.cap * tanhf(y * inv_cap);
+								y = a.cap * tanh_of_exponent(y * inv_cap);
 							if (a.cap > 0.f || a.slopes)
 								y = (y - slope[i][e & 1] * float(t - s)) * LOG2E;
 							if (id < 0 || s < lo || s >= hi || s > t || (a.window && t - s >= a.window))

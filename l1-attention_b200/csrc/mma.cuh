@@ -110,6 +110,14 @@ __device__ __forceinline__ float exp2_fast(float x)
 	asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
 	return y;
 }
+// tanh of x = y / (2 log2 e), for x that is not above 0 by more than a rounding: (t - 1) / (t + 1) with t = e^2x.  Off by 2^-22 at most, absolutely: what a
+// score has of it times its cap is small beside the weights' rounding.  ([2,2048,8,128], causal, bfloat16: 378 us, not capped 329, with
+// tanhf, which is exact near 0 too, 396.)
+__device__ __forceinline__ float tanh_of_exponent(float y)
+{
+	const float t = exp2_fast(y);
+	return __fdividef(t - 1.f, t + 1.f);
+}
 
 // bfloat16 values as codes of 15 bits in their order: signs of differences then take one instruction for two (signs_of_codes).  A code is the value's
 // magnitude, less CODE_BASE and not below 0, with its sign: exact from 2^-63 to 2^64, and for zero.
