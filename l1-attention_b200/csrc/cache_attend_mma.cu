@@ -80,7 +80,6 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 	const CacheArgs &c = a.c;
 	unsigned char *const smem = reinterpret_cast<unsigned char *>(smem16);
 	const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, j = lane % 4;
-	const float inv_cap = a.cap > 0.f ? 2.f * LOG2E / a.cap : 0.f; // as tanh_of_exponent takes it
 
 	// all sequences' chunks, and this CTA's share of them
 	auto weigh = [&](int i, SeqView *view) {
@@ -381,6 +380,8 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 					for (int e = 0; e < 4; e++)
 						x[n][i][e] = fmaf(k_unit, x[n][i][e], q_part[i][e & 1]);
 			if (!whole || a.cap > 0.f || a.slopes) {
+				if (a.cap > 0.f)
+					cap_scores<NG * TILES * 4, false>(&x[0][0][0], nullptr, a.cap);
 #pragma unroll
 				for (int n = 0; n < NG; n++)
 #pragma unroll
@@ -389,8 +390,6 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 						for (int e = 0; e < 4; e++) {
 							const int s = s0 + 16 * n + g + 8 * (e / 2), t = t_of[i][e & 1];
 							float y = x[n][i][e];
-							if (a.cap > 0.f)
-								y = a.cap * tanh_of_exponent(y * inv_cap);
 							if (a.cap > 0.f || a.slopes)
 								y = (y - slope[i][e & 1] * float(t - s)) * LOG2E;
 							if (id < 0 || s < lo || s >= hi || s > t || (a.window && t - s >= a.window))

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 	const int head = bh % a.heads, b = bh / a.heads, kv = head / (a.heads / a.kv_heads);
 	const MaskView mask(a, b);
 	const int t0 = tile * ROWS, t1 = min(a.n, t0 + ROWS), ta = t0 + 16 * MB * warp + g; // this lane's rows: ta + 8 r
-	const float slope = a.slopes ? a.slopes[head] : 0.f, inv_cap = a.cap > 0.f ? 2.f * LOG2E / a.cap : 0.f; // as tanh_of_exponent takes it
+	const float slope = a.slopes ? a.slopes[head] : 0.f;
 
 	// the warp's query rows, in registers for good, and their sums
 	load_tile16<T, false, KP, ROWS, THREADS>(base, a.q, b, head, t0, a.n, a.width, nullptr, vec & 1, tid);
@@ -226,14 +226,14 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 					x[i][h][c] = unit * (fmaf(2.f, x[i][h][c], -qs[2 * i + c / 2]) - (c & 1 ? ks.y : ks.x));
 		}
 		if (special) {
+			if (a.cap > 0.f)
+				cap_scores<MB * 8, false>(&x[0][0][0], nullptr, a.cap);
 #pragma unroll
 			for (int i = 0; i < MB; i++)
 #pragma unroll
 				for (int c = 0; c < 8; c++) {
 					const int s = s0 + 8 * (c / 4) + 2 * j + (c & 1), t = ta + 16 * i + 8 * (c / 2 % 2);
 					float y = x[i][c / 4][c % 4];
-					if (a.cap > 0.f)
-						y = a.cap * tanh_of_exponent(y * inv_cap);
 					if (a.slopes)
 						y -= slope * fabsf(float(t - s));
 					if (!whole && !(t < a.n && s < a.n && mask.sees(t, s, mask.doc ? mask.doc[t] : 0, mask.doc ? mask.doc[s] : 0)))
@@ -654,7 +654,6 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 	const int head = bh % a.heads, b = bh / a.heads, kv = head / (a.heads / a.kv_heads);
 	const MaskView mask(a, b);
 	const int o0 = tile * ROWS, o1 = min(a.n, o0 + ROWS), oa = o0 + 16 * warp + g; // this lane's rows: oa, oa + 8
-	const float inv_cap = a.cap > 0.f ? 2.f * LOG2E / a.cap : 0.f;
 	const Strided go = {dvo, (long long)a.n * a.heads * a.v_width, (long long)a.heads * a.v_width, a.v_width};
 
 	// own rows stay in shared memory: as they are for the scores (registers that held them were missing beside the sums), as a table for the signs
@@ -813,18 +812,15 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 					slant[h][c] = -a.scale;
 				}
 			}
-			if (!whole || a.cap > 0.f || a.slopes) {
+			if (a.cap > 0.f)
+				cap_scores<8, true>(&x[0][0], &slant[0][0], a.cap);
+			if (!whole || a.slopes) {
 #pragma unroll
 				for (int h = 0; h < 2; h++)
 #pragma unroll
 					for (int c = 0; c < 4; c++) {
 						const int r = r0 + 16 * kb + 8 * h + 2 * j + (c & 1), o = oa + 8 * (c / 2), t = OWN_KEYS ? r : o, s = OWN_KEYS ? o : r;
 						float y = x[h][c];
-						if (a.cap > 0.f) {
-							const float th = tanh_of_exponent(y * inv_cap);
-							slant[h][c] *= 1.f - th * th;
-							y = a.cap * th;
-						}
 						if (a.slopes)
 							y -= slope * fabsf(float(t - s));
 						if (!whole && !(t < a.n && s < a.n && mask.sees(t, s, mask.doc ? mask.doc[t] : 0, mask.doc ? mask.doc[s] : 0)))
