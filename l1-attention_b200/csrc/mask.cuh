@@ -122,6 +122,16 @@ __device__ __forceinline__ float finish_row(int mode, float m, float l, float *l
 	return l == 0.f ? 0.f : 1.f / l;
 }
 
+// The same for rows that begin with nothing (m = -inf, l = 0) in every mode, so that m is the largest score of a key: the +1 form's key of score 0 joins here.
+__device__ __forceinline__ float finish_row_of_keys(int mode, float m, float l, float *lse)
+{
+	if (mode != L1ATTN_SV_SOFTMAX_PLUS_ONE)
+		return finish_row(mode, m, l, lse);
+	const float top = fmaxf(m, 0.f), keep = expf(m - top), sum = l * keep + expf(-top);
+	*lse = top + logf(sum);
+	return keep / sum;
+}
+
 // 16-bit types, widths up to 128: distances and products on the tensor cores
 bool masked_mma_fits(int width, int v_width, int dtype);
 int masked_mma_fwd_launch(const MaskedArgs &a, void *vo, void *rest, float *lse, int dtype, cudaStream_t st);

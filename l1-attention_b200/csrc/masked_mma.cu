@@ -149,9 +149,8 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 	float o[MB][2 * V][4];
 #pragma unroll
 	for (int r = 0; r < 2 * MB; r++) {
-		m[r] = start_max(a.mode);
-		ref[r] = m[r] == -INFINITY ? 0.f : m[r] - LIFT<T>;
-		l[r] = 0.f;
+		m[r] = -INFINITY; // (in every mode: weights are rounded relative to the row's largest)
+		ref[r] = l[r] = 0.f;
 	}
 #pragma unroll
 	for (int i = 0; i < MB * 2 * V * 4; i++)
@@ -352,10 +351,8 @@ __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_m
 		l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
 		l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
 		l[r] *= exp2f(-LIFT<T>);
-		if (a.mode == L1ATTN_SV_SOFTMAX_PLUS_ONE)
-			l[r] += exp2_fast(-m[r]);
 		float ls;
-		const float f = finish_row(a.mode, m[r] / LOG2E, l[r], &ls);
+		const float f = finish_row_of_keys(a.mode, m[r] / LOG2E, l[r], &ls);
 		bool odd = !(fabsf(l[r]) < INFINITY) || !(fabsf(f) < INFINITY);
 		const int t = ta + 8 * r;
 		const long long row = ((long long)b * a.n + t) * a.heads + head;
