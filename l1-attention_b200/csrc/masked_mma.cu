@@ -586,6 +586,31 @@ template <int W> __device__ __forceinline__ void follow_largest(const float (&e)
 	}
 }
 
+// The same for weights on their way to dv in float16, relative to their own row's (key's) largest so far: without a normaliser, or for a key that nobody
+// weighs much, they are as small as exp(score).
+template <int N> __device__ __forceinline__ void follow_largest_weight(const float (&p)[2][4], float (&unit)[2], float (&limit)[2], float (&acc)[N][4])
+{
+#pragma unroll
+	for (int r = 0; r < 2; r++) {
+		float most = fmaxf(fmaxf(p[0][2 * r], p[0][2 * r + 1]), fmaxf(p[1][2 * r], p[1][2 * r + 1]));
+		most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+		most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+		float keep = 1.f;
+		if (most > limit[r]) {
+			const int top = min(max(int(__float_as_uint(most) >> 23), 13), 242);
+			const float now = __uint_as_float(uint32_t(254 + 11 - top) << 23);
+			keep = limit[r] == 0.f ? 1.f : now / unit[r];
+			unit[r] = now;
+			limit[r] = __uint_as_float(uint32_t(top + 4) << 23);
+		}
+#pragma unroll
+		for (int i = 0; i < N; i++) {
+			acc[i][2 * r] *= keep;
+			acc[i][2 * r + 1] *= keep;
+		}
+	}
+}
+
 // Signs were 2^-24 (and one too large where e_sum counts them), e times unit: a warp's 16 rows of the gradient, to `part` or `dx`.  Returns the rows whose
 // values are not finite, by this lane.
 template <typename T, int W>
@@ -630,7 +655,7 @@ __device__ __forceinline__ unsigned store_signed(const float (&acc)[2 * W][2][4]
 //                     B = e in the column of that row: 16 own rows fill two 16 x 8 tiles per 16 columns.  Signs take two instructions for two values
 //                     (a subtraction, which mma.sync does not overlap, and a minimum), or one for bfloat16 as codes of 15 bits; a tile with values
 //                     that these do not hold takes the two
-//   dv                p^T dvo, weights rounded to the type (float16: times 2^12, so that small ones keep their bits)
+//   dv                p^T dvo, weights rounded to the type (float16: relative to their row's largest so far, as e)
 // No atomics, and the same sums in the same order every time.
 // Bound: the tensor pipe and the instructions that feed it, of 8 warps an SM (registers: two CTAs).  [2,2048,8,128], causal, two heads of keys, bfloat16:
 // 1.26 ms; [1,8192,8,64], float16: 5.67 ms; [4,2048,8,128], no mask, bfloat16: 4.38 ms (in float32 arithmetic, masked_simple.cu: 15.6).
@@ -679,7 +704,7 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 		accv[i / 4][i % 4] = 0.f;
 	float e_sum[4] = {0.f, 0.f, 0.f, 0.f}; // CODES: of the rounded e, by own row: signs there are one too large
 	float unit[2] = {1.f, 1.f}, limit[2] = {0.f, 0.f}; // per row: a power of two times e is rounded to float16; e may come this far
-	const float p_unit = OWN_KEYS && sizeof(T) == 2 && H::ONES == Half2<__half>::ONES && a.mode != L1ATTN_SV_EXP ? 4096.f : 1.f;
+	float p_unit[2] = {1.f, 1.f}, p_limit[2] = {0.f, 0.f}; // the same for weights, in float16
 
 	// tiles of the other side
 	const int first_tile = [&] {
@@ -835,10 +860,13 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 					const float p = exp2_fast(fmaf(x[h][c], LOG2E, -ls));
 					e[h][c] = p == 0.f ? 0.f : p * slant[h][c] * (dp[h][c] - de);
 					x[h][c] = p;
-					grew |= fabsf(e[h][c]) > limit[c / 2];
+					grew |= fabsf(e[h][c]) > limit[c / 2] || (OWN_KEYS && !CODES && p > p_limit[c / 2]);
 				}
-			if (__any_sync(0xffffffffu, grew))
+			if (__any_sync(0xffffffffu, grew)) {
 				follow_largest<W>(e, unit, limit, e_sum, acc, j);
+				if constexpr (OWN_KEYS && !CODES)
+					follow_largest_weight(x, p_unit, p_limit, accv);
+			}
 			uint32_t eb[2][2], el[2][2] = {}; // [own row g, g + 8][streamed 0-7, 8-15]; el: what rounding left
 #pragma unroll
 			for (int i = 0; i < 4; i++) {
@@ -861,8 +889,8 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 				uint32_t p[4];
 #pragma unroll
 				for (int h = 0; h < 2; h++) {
-					p[2 * h] = H::pack(x[h][0] * p_unit, x[h][1] * p_unit);
-					p[2 * h + 1] = H::pack(x[h][2] * p_unit, x[h][3] * p_unit);
+					p[2 * h] = H::pack(x[h][0] * p_unit[0], x[h][1] * p_unit[0]);
+					p[2 * h + 1] = H::pack(x[h][2] * p_unit[1], x[h][3] * p_unit[1]);
 				}
 #pragma unroll
 				for (int vb = 0; vb < V; vb++) {
@@ -892,7 +920,7 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 #pragma unroll
 				for (int c = 0; c < 2; c++) {
 					const int w = 8 * i + 2 * j + c;
-					const float y = accv[i % (OWN_KEYS ? 2 * V : 1)][2 * r + c] * (1.f / p_unit);
+					const float y = accv[i % (OWN_KEYS ? 2 * V : 1)][2 * r + c] * (1.f / p_unit[r]);
 					odd |= !(fabsf(y) < INFINITY);
 					if (o < a.n && w < a.v_width) {
 						const long long at = (((long long)b * a.n + o) * a.heads + head) * a.v_width + w;
