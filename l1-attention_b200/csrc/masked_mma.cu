@@ -655,7 +655,8 @@ __device__ __forceinline__ unsigned store_signed(const float (&acc)[2 * W][2][4]
 //                     B = e in the column of that row: 16 own rows fill two 16 x 8 tiles per 16 columns.  Signs take two instructions for two values
 //                     (a subtraction, which mma.sync does not overlap, and a minimum), or one for bfloat16 as codes of 15 bits; a tile with values
 //                     that these do not hold takes the two
-//   dv                p^T dvo, weights rounded to the type (float16: relative to their row's largest so far, as e)
+//   dv                p^T dvo, weights rounded to the type (float16: relative to their row's largest so far, as e) and what that leaves in a second product
+//                     (without it dv is 1.4 times as far from 64 bits as when rounded once; 1.5 % of the time)
 // No atomics, and the same sums in the same order every time.
 // Bound: the tensor pipe and the instructions that feed it, of 8 warps an SM (registers: two CTAs).  [2,2048,8,128], causal, two heads of keys, bfloat16:
 // 1.26 ms; [1,8192,8,64], float16: 5.67 ms; [4,2048,8,128], no mask, bfloat16: 4.38 ms (in float32 arithmetic, masked_simple.cu: 15.6).
@@ -886,18 +887,23 @@ __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a
 						to[(8 * h + (c & 1)) * parts.pitch + 8 * (c / 2)] = e[h][c];
 			}
 			if (OWN_KEYS) {
-				uint32_t p[4];
+				uint32_t p[4], low[4]; // low: what rounding left
 #pragma unroll
-				for (int h = 0; h < 2; h++) {
-					p[2 * h] = H::pack(x[h][0] * p_unit[0], x[h][1] * p_unit[0]);
-					p[2 * h + 1] = H::pack(x[h][2] * p_unit[1], x[h][3] * p_unit[1]);
+				for (int i = 0; i < 4; i++) {
+					const float p0 = x[i / 2][i % 2 * 2] * p_unit[i % 2], p1 = x[i / 2][i % 2 * 2 + 1] * p_unit[i % 2];
+					p[i] = H::pack(p0, p1);
+					const float2 f = H::unpack(p[i]);
+					low[i] = H::pack(p0 - f.x, p1 - f.y);
 				}
 #pragma unroll
 				for (int vb = 0; vb < V; vb++) {
 					uint32_t y[4];
 					ldmatrix4_trans(y, ys + tile_offset<true>(VP, 16 * kb + lane % 16, 2 * vb + lane / 16));
-					H::mma(accv[(2 * vb) % (OWN_KEYS ? 2 * V : 1)], p[0], p[1], p[2], p[3], y[0], y[1]);
-					H::mma(accv[(2 * vb + 1) % (OWN_KEYS ? 2 * V : 1)], p[0], p[1], p[2], p[3], y[2], y[3]);
+					float(&a0)[4] = accv[(2 * vb) % (OWN_KEYS ? 2 * V : 1)], (&a1)[4] = accv[(2 * vb + 1) % (OWN_KEYS ? 2 * V : 1)];
+					H::mma(a0, p[0], p[1], p[2], p[3], y[0], y[1]);
+					H::mma(a1, p[0], p[1], p[2], p[3], y[2], y[3]);
+					H::mma(a0, low[0], low[1], low[2], low[3], y[0], y[1]);
+					H::mma(a1, low[0], low[1], low[2], low[3], y[2], y[3]);
 				}
 			}
 			const bool coded = CODES && !off;
