@@ -32,3 +32,11 @@ SIZES = [(1024, 1, 1, 64, 64), (600, 2, 2, 128, 128), (500, 4, 2, 96, 40)]
 @pytest.mark.parametrize("size", SIZES)
 def test_values(size, mode, dt):
     assert _ratios(dt, mode, *size)["dv"] <= 1.1
+
+
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("mode", ["softmax", "exp"])
+@pytest.mark.parametrize("size", SIZES)
+def test_all(size, mode, dt):
+    ratios = _ratios(dt, mode, *size)
+    assert max(ratios.values()) <= 1.1, ratios
