@@ -24,9 +24,10 @@ L1B_BOTH void cache_fault(const CacheArgs &c)
 		*reinterpret_cast<volatile int *>(c.status) = L1ATTN_ERR_INDEX;
 }
 
-// One sequence's part of a call: rows [row, row + count) of the token tensors are its positions [start, start + count).
+// One sequence's part of a call: rows [row, row + count) of the token tensors are its positions [start, start + count); the `lost` rows behind them are its
+// too, but have no place (the offsets or the start are out of range, or the table ends): what is read at them is zeros.
 struct SeqView {
-	int row, count, start;
+	int row, count, start, lost;
 };
 
 L1B_BOTH int cache_row(const CacheArgs &c, int seq)
@@ -38,9 +39,11 @@ L1B_BOTH int cache_row(const CacheArgs &c, int seq)
 L1B_BOTH SeqView cache_seq(const CacheArgs &c, int seq)
 {
 	const int a = c.cu[seq], b = c.cu[seq + 1], s = c.start[seq];
-	SeqView v = {cache_row(c, seq), 0, s};
+	SeqView v = {cache_row(c, seq), 0, s, 0};
 	if (a < 0 || b < a || b > c.rows || s < 0) {
 		cache_fault(c);
+		const int own = cache_row(c, seq + 1) - v.row;
+		v.lost = own > 0 ? own : 0;
 		v.start = 0;
 		return v;
 	}
@@ -49,6 +52,7 @@ L1B_BOTH SeqView cache_seq(const CacheArgs &c, int seq)
 	if (v.count > room) {
 		cache_fault(c);
 		v.count = room > 0 ? int(room) : 0;
+		v.lost = b - a - v.count;
 	}
 	return v;
 }

@@ -41,7 +41,14 @@ template <typename T, int NV> __global__ void __launch_bounds__(THREADS) attend_
 	const int seq = cache_find_warp(c, blockIdx.x, a.group, a.tile_rows, 1);
 	const SeqView sv = cache_seq(c, seq);
 	const long long first = (blockIdx.x - cache_first_unit(c, seq, a.group, a.tile_rows, 1)) * ROWS, all = (long long)sv.count * a.group;
-	if (first < 0 || first >= all)
+	const long long ends = min(first + ROWS, all + (long long)sv.lost * a.group);
+	if (first < 0 || first >= ends)
+		return;
+	if (!a.part) // rows without a place (else attend_merge_kernel's)
+		for (long long lr = max(first, all); lr < ends; lr++)
+			for (int w = tid; w < c.v_width; w += THREADS)
+				static_cast<T *>(a.vo)[((sv.row + lr / a.group) * a.heads + kv * a.group + lr % a.group) * c.v_width + w] = from_float<T>(0.f);
+	if (first >= all)
 		return;
 	const long long last = min(first + ROWS, all) - 1;
 	const int t_lo = sv.start + int(first / a.group), t_hi = sv.start + int(last / a.group);
@@ -150,8 +157,13 @@ template <typename T> __global__ void __launch_bounds__(128) attend_merge_kernel
 		return;
 	const int seq = cache_find_row(c, row);
 	const SeqView sv = cache_seq(c, seq);
-	if (row < sv.row || row - sv.row >= sv.count)
+	if (row < sv.row || row - sv.row >= (long long)sv.count + sv.lost)
 		return;
+	if (row - sv.row >= sv.count) { // a row without a place
+		for (int w = lane; w < c.v_width; w += 32)
+			static_cast<T *>(a.vo)[unit * c.v_width + w] = from_float<T>(0.f);
+		return;
+	}
 	const int t = sv.start + int(row - sv.row);
 	const int parts = min(a.splits, t / a.split_keys + 1);
 	const float *part = a.part + unit * (c.v_width + 2);

@@ -104,6 +104,12 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 	long long at = blockIdx.x * share, before = 0; // before: chunks of the sequences before seq
 	if (a.splits_of && tid == 0)
 		a.splits_of[blockIdx.x].kv = -1;
+	for (int i = blockIdx.x; i < c.n_seqs; i += gridDim.x) { // queries without a place: zeros, a sequence a CTA
+		const SeqView v = cache_seq(c, i);
+		const long long size = (long long)a.heads * c.v_width, begin = (v.row + v.count) * size, end = begin + v.lost * size;
+		for (long long w = begin + tid; w < end; w += THREADS)
+			static_cast<T *>(a.vo)[w] = from_float<T>(0.f);
+	}
 	if (at >= to)
 		return;
 	int seq = 0;

@@ -27,7 +27,7 @@ The functions take them with the places of this call's tokens, all on the device
     t = cache.fork(s); cache.truncate(s, 10); cache.close(t); cache.compact()
 
 Rows behind cu[n_seqs] (a padded batch) are neither read nor written.  Page ids, starts and offsets out of range are never followed: their
-tokens are left out, and `status` (int32 [1], optional; `L1Cache.check()`) becomes non-zero.  float32, float16 and bfloat16 tokens, float32 sums.
+tokens are left out (keys are not seen, gathered rows and the outputs of queries without a place are zeros), and `status` (int32 [1], optional; `L1Cache.check()`) becomes non-zero.  float32, float16 and bfloat16 tokens, float32 sums.
 No gradients (a cache answers, it does not train) and no CPU path.
 """
 import torch
