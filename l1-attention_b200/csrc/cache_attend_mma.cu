@@ -36,6 +36,14 @@ __device__ __forceinline__ uint32_t permute(uint32_t a, uint32_t b, uint32_t how
 __device__ __forceinline__ uint32_t half_codes(uint32_t u, uint32_t how) { return H::sub(permute(u, 0x64646464u, how), 0x64806480u); }
 constexpr uint32_t LOW = 0x4140, HIGH = 0x4342;
 
+__device__ __forceinline__ float warp_max(float x)
+{
+#pragma unroll
+	for (int s = 16; s; s >>= 1)
+		x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, s));
+	return x;
+}
+
 template <typename T> __device__ __forceinline__ T half_of(uint32_t x, int which)
 {
 	const uint16_t bits = uint16_t(x >> 16 * which);
@@ -61,7 +69,7 @@ template <int VG> __device__ __forceinline__ uint32_t value_place(int row, int g
 // are of 16 tokens, so that a chunk has one scale)
 template <typename T, int WG, int VG, int TILES, int NG> struct Layout {
 	static constexpr int CHUNK = 16 * NG, KEY_BYTES = CHUNK * 64 * WG, STAGE = CHUNK * (64 * WG + 32 * VG), STAGES = 2;
-	static constexpr int Q_TABLE = 8 * TILES * 64 * WG * 2, WARP = Q_TABLE + STAGES * STAGE + 64 * TILES; // q' | stages | clipped rests
+	static constexpr int Q_TABLE = 8 * TILES * 64 * WG * 2, WARP = Q_TABLE + STAGES * STAGE + 64 * TILES; // q' | stages | clipped rests, lowest unit
 	static constexpr int Q_ROWS = 8 * TILES * 64 * WG * 2, JOIN = WARPS * 8 * TILES * (32 * VG + 2) * 4;
 	static constexpr int BYTES = Q_ROWS + (WARPS * WARP > JOIN ? WARPS * WARP : JOIN);
 };
@@ -184,9 +192,7 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 			const float x = fabsf(to_float(q_rows[i]));
 			q_max = fmaxf(q_max, x == x ? x : INFINITY);
 		}
-#pragma unroll
-		for (int s = 16; s; s >>= 1)
-			q_max = fmaxf(q_max, __shfl_xor_sync(0xffffffffu, q_max, s));
+		q_max = warp_max(q_max);
 
 		// The range's chunks are dealt out to the warps in runs (a run has each page's q' formed once); this warp's number k begins at position
 		// (chunk0 + k) CHUNK.  Pages are looked up for 32 chunks at a time, one a lane, two such sets.
@@ -257,7 +263,11 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 			fetch(k);
 
 		int page_before = -2;
-		float k_unit = 0.f, v_unit = 0.f, q_part[TILES][2]; // k_unit: 2 scale s (log2 e); v_unit: power of two that value scales are taken relative to (2^6 more, so that weights far below the largest keep bits; at most 2^15 then); q_part: of the score
+		// k_unit: 2 scale s (log2 e); q_part: of the score.  v_unit: power of two that the page's value scale is taken relative to: 2^4 to 2^7 times it, so that weights far
+		// below the largest keep bits (at most 2^15 then).  It follows smaller scales too, since any page may hold a row's weight, but never more than 2^58 times above
+		// its lowest: 2^30 keys of 2^22, codes and all, then stay within 2^110.
+		int *const lowest = reinterpret_cast<int *>(rest + ROWS);
+		float k_unit = 0.f, v_unit = 0.f, q_part[TILES][2];
 		for (int k = 0; k < chunks; k++) {
 			if (k && k % 32 == 0)
 				look_up(k / 32 + 1);
@@ -315,10 +325,18 @@ template <typename T, int WG, int VG, int TILES, int NG> __global__ void __launc
 					for (int b = 0; b < 2; b++)
 						q_part[i][b] = -0.5f * k_unit * sum[b] - a.scale * (straight ? LOG2E : 1.f) * (clips ? rest[8 * i + 2 * j + b] : 0.f);
 				}
-				if (vs * v_unit > 128.f || v_unit == 0.f) { // (a power of two from the first scale that is not zero; larger ones take it along)
-					const int e = min(max(int(__float_as_uint(vs) >> 23), 7), 253);
-					const float now = vs > 0.f ? __uint_as_float(uint32_t(260 - e) << 23) : 0.f, keep = v_unit == 0.f ? 0.f : now / v_unit;
-					v_unit = now;
+				if (__float_as_uint(vs * v_unit) - 0x41800000u > 0x01800000u && vs > 0.f) { // not from 16 to 128; what has been added up follows
+					const int was = __float_as_uint(v_unit) >> 23; // exponents; 0: no scale yet
+					int to = 260 - min(max(int(__float_as_uint(vs) >> 23), 7), 253), low = to;
+					if (was) {
+						low = *lowest;
+						to = min(to, low + 58);
+						low = min(low, to);
+					}
+					__syncwarp();
+					*lowest = low;
+					v_unit = __uint_as_float(uint32_t(to) << 23);
+					const float keep = !was ? 1.f : to - was < -126 ? 0.f : __uint_as_float(uint32_t(127 + to - was) << 23);
 #pragma unroll
 					for (int i = 0; i < TILES * 2 * VG * 4; i++)
 						o[i / (8 * VG)][i / 4 % (2 * VG)][i % 4] *= keep;

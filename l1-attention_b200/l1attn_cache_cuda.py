@@ -61,7 +61,8 @@ def attend(q, k_codes, v_codes, k_scale, v_scale, table, start, cu, mode="softma
     max_len: the longest start + count, where the program knows it (default: what the table has room for); it shapes the launch alone.
     out: a contiguous tensor to write, not q itself; rows behind cu[-1] are left as they were in it, and undefined without it.
 
-    16-bit q: query / scale is rounded to float16 next to codes that it holds exactly, weights to 11 bits (float16: 22) or 2^-31 of the row's largest; float32 q: float32 throughout."""
+    16-bit q: query / scale is rounded to float16 next to codes that it holds exactly, weights to 11 bits (float16: 22) or 2^-29 of the
+    row's largest, whatever the scales of its pages' values, up to 2^58 times one another; float32 q: float32 throughout."""
     mode, _, window, softcap = _options(mode, True, window, softcap)
     return l1attn_cache_cuda_drv.attend(q, (k_codes, v_codes, k_scale, v_scale), table, start, cu, mode, window, softcap, slopes, -1 if max_len is None else max(0, int(max_len)),
                                         out, status)
