@@ -38,6 +38,7 @@ template <typename T, int NV> __global__ void __launch_bounds__(THREADS) attend_
 	const int wp = pitch(c.width), vp = 64 * NV, tid = threadIdx.x, tx = tid % 16, ty = tid / 16, kv = blockIdx.y;
 	constexpr int PP = KEYS + 4;
 	float *Q = reinterpret_cast<float *>(smem4), *K = Q + ROWS * wp, *V = K + KEYS * wp, *P = V + KEYS * vp;
+	int *there = reinterpret_cast<int *>(P + ROWS * PP); // keys whose page is in range
 	const int seq = cache_find_warp(c, blockIdx.x, a.group, a.tile_rows, 1);
 	const SeqView sv = cache_seq(c, seq);
 	const long long first = (blockIdx.x - cache_first_unit(c, seq, a.group, a.tile_rows, 1)) * ROWS, all = (long long)sv.count * a.group;
@@ -73,9 +74,10 @@ template <typename T, int NV> __global__ void __launch_bounds__(THREADS) attend_
 		for (int s = tid / 32; s < KEYS; s += THREADS / 32) {
 			const int pos = s0 + s, id = pos < hi ? cache_page(c, seq, pos / c.page) : -1;
 			const long long at = (long long)max(id, 0) * c.kv_heads + kv, r = at * c.page + pos % c.page;
-			// a page that is out of range: keys infinitely far
+			if (tid % 32 == 0)
+				there[s] = id >= 0;
 			for (int w = tid % 32; w < wp; w += 32)
-				K[s * wp + w] = id < 0 ? INFINITY : w < c.width ? c.k_codes[r * c.width + w] * c.k_scale[at] : 0.f;
+				K[s * wp + w] = id >= 0 && w < c.width ? c.k_codes[r * c.width + w] * c.k_scale[at] : 0.f;
 			for (int w = tid % 32; w < vp; w += 32)
 				V[s * vp + w] = id >= 0 && w < c.v_width ? c.v_codes[r * c.v_width + w] * c.v_scale[at] : 0.f;
 		}
@@ -94,7 +96,7 @@ template <typename T, int NV> __global__ void __launch_bounds__(THREADS) attend_
 			if (a.cap > 0.f)
 				y = y == -INFINITY ? y : a.cap * tanhf(y * inv_cap);
 			y -= slope * float(t - s);
-			x[j] = mine && s >= lo && s < hi && s <= t && (a.window == 0 || t - s < a.window) ? y : -INFINITY;
+			x[j] = mine && there[tx + 16 * j] && s >= lo && s < hi && s <= t && (a.window == 0 || t - s < a.window) ? y : -INFINITY;
 			top = fmaxf(top, x[j]);
 		}
 		top = half_warp_max(top);
@@ -193,7 +195,7 @@ template <typename T> __global__ void __launch_bounds__(128) attend_merge_kernel
 
 template <typename T, int NV> int simple(const AttendArgs &a, cudaStream_t st)
 {
-	const int wp = pitch(a.c.width), bytes = 4 * (ROWS * wp + KEYS * wp + KEYS * 64 * NV + ROWS * (KEYS + 4));
+	const int wp = pitch(a.c.width), bytes = 4 * (ROWS * wp + KEYS * wp + KEYS * 64 * NV + ROWS * (KEYS + 4) + KEYS);
 	const long long tiles = (long long)a.c.rows * a.group / ROWS + a.c.n_seqs;
 	if (tiles > 0x7fffffffll || a.c.kv_heads > 65535 || a.splits > 65535)
 		return L1ATTN_ERR_SHAPE;
