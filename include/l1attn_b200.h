@@ -184,7 +184,7 @@ int l1attn_test_softmax_v_form(int bs, int n_tok, int n_heads, int width, int v_
  *   x[t][s] = (-1/sqrt(width)) * sum_w |q[t][w] - k[s][w]|;  x = softcap * tanh(x / softcap) where softcap > 0;  x -= slopes[head] * |t - s|
  *   t sees s when (no doc, or doc[t] == doc[s] >= 0) and (s < prefix, or (s <= t where causal) and (|t - s| < window where window > 0))
  * Weights as in l1attn_dense_softmax_v_fwd, over the keys that a query sees.  A query that sees none gets an output of zeros and no gradient;
- * so does one whose keys are all infinitely far.  A key whose weight is zero contributes nothing, whatever its value row holds.
+ * so does one whose keys are all infinitely far, where no cap bounds that.  A key whose weight is zero contributes nothing, whatever its value row holds.
  */
 typedef struct l1attn_mask {
 	int causal;            /* 0 or 1 */

@@ -94,7 +94,7 @@ template <typename T, int NV> __global__ void __launch_bounds__(THREADS) attend_
 			const int s = s0 + tx + 16 * j;
 			float y = -a.scale * d;
 			if (a.cap > 0.f)
-				y = y == -INFINITY ? y : a.cap * tanhf(y * inv_cap);
+				y = a.cap * tanhf(y * inv_cap);
 			y -= slope * float(t - s);
 			x[j] = mine && there[tx + 16 * j] && s >= lo && s < hi && s <= t && (a.window == 0 || t - s < a.window) ? y : -INFINITY;
 			top = fmaxf(top, x[j]);

@@ -26,3 +26,18 @@ def test_bad_pages(w, wv, dt):
     for table in ((3, 1, 0), (3, 99, 0), (-1, 1, 0)):
         _, vo = _call(dt, w, wv, table)
         assert torch.isfinite(vo).all() and not vo[1, 2].any() and vo[1, 3].any() and vo[0, 2].any()
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("w,wv", SIZES)
+def test_caps(w, wv, dt):
+    """A cap bounds infinite distances too: every key scores -cap, so the row is the mean of the values -- of those that it sees."""
+    table = (3, 99, 0)
+    for cap in (1e-3, 5.0, 1000.0):
+        cache, vo = _call(dt, w, wv, table, softcap=cap)
+        v = (cache[1].double() * cache[3].double()[..., None, None])[[3, 0], 1]
+        mean = torch.cat([v[0], v[1, :10]]).mean(0)  # positions 0 to 15 and 32 to 41; the page between is out of range
+        step = torch.finfo(dt).eps / 2
+        # weights are alike, rounded to 11 bits in 16 bits; the sum of 26 in float32; the output once
+        tol = (2.0 ** -11 if dt != F32 else 0.0) * v.abs().amax() + 32 * 2.0 ** -24 * v.abs().amax() + step * mean.abs()
+        assert torch.isfinite(vo).all() and ((vo[1, 2].double() - mean).abs() <= tol).all()
