@@ -72,7 +72,7 @@ template <typename T, int NV> __global__ void __launch_bounds__(THREADS) attend_
 	for (int s0 = lo / KEYS * KEYS; s0 < hi; s0 += KEYS) {
 		__syncthreads();
 		for (int s = tid / 32; s < KEYS; s += THREADS / 32) {
-			const int pos = s0 + s, id = pos < hi ? cache_page(c, seq, pos / c.page) : -1;
+			const int pos = s0 + s, id = pos >= lo && pos < hi ? cache_page(c, seq, pos / c.page) : -1; // (pages before a window may have gone)
 			const long long at = (long long)max(id, 0) * c.kv_heads + kv, r = at * c.page + pos % c.page;
 			if (tid % 32 == 0)
 				there[s] = id >= 0;
