@@ -38,6 +38,12 @@ inline void l1b_same(const torch::Tensor &a, const torch::Tensor &b, const char 
 		TORCH_CHECK(a.sizes() == b.sizes(), an, " and ", bn, " must have the same shape");
 }
 
+// Calls that autograd does not see would lose a tensor's forward-mode tangent; those that it sees refuse it themselves.
+inline void l1b_no_tangent(const torch::Tensor &t, const char *name)
+{
+	TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name, " carries a forward-mode tangent: there is no forward-mode derivative");
+}
+
 // Numbers of a message as text.  (They are not streamed: a driver may carry its own copy of the C++ library, whose streams then look for
 // number formats in the locale of the process's other copy.)
 inline std::string l1b_shape(at::IntArrayRef sizes)

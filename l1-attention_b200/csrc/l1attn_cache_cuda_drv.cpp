@@ -80,6 +80,7 @@ torch::Tensor tokens(const torch::Tensor &t, const char *name, const torch::Tens
 	TORCH_CHECK(type == torch::kFloat32 || type == torch::kFloat16 || type == torch::kBFloat16, name, " must be float32, float16 or bfloat16");
 	TORCH_CHECK(t.dim() == 3 && t.size(2) == width && (heads < 0 || t.size(1) == heads) && t.size(0) <= INT32_MAX, name, " must be [rows, ", heads < 0 ? "heads" : std::to_string(heads),
 		    ", ", std::to_string(width), "]");
+	l1b_no_tangent(t, name);
 	return t.stride(2) == 1 || width == 1 ? t : t.contiguous();
 }
 
@@ -129,6 +130,7 @@ torch::Tensor attend(torch::Tensor q, std::vector<torch::Tensor> cache, torch::T
 		TORCH_CHECK(slopes->scalar_type() == torch::kFloat32 && slopes->dim() == 1 && slopes->size(0) == h && slopes->device() == q.device(),
 			    "slopes must be a float32 tensor of shape ", l1b_shape({h}), " on the device of q");
 		TORCH_CHECK(!slopes->requires_grad(), "slopes is a constant: it must not require a gradient");
+		l1b_no_tangent(*slopes, "slopes");
 		sl = slopes->contiguous();
 	}
 	const c10::cuda::CUDAGuard guard(q.device());

@@ -9,7 +9,7 @@ using Maybe = c10::optional<torch::Tensor>;
 
 const char *const SHAPES = "q must be [bs, n, h, w], k [bs, n, hk, w], v [bs, n, hk, wv]";
 
-// a small tensor beside q, k, v: its shape, type and device; contiguous
+// a small tensor beside q, k, v: its shape, type and device; contiguous.
 torch::Tensor side(const Maybe &t, const char *name, at::IntArrayRef shape, torch::ScalarType type, const torch::Tensor &like)
 {
 	if (!t.has_value() || !t->defined())
@@ -17,6 +17,7 @@ torch::Tensor side(const Maybe &t, const char *name, at::IntArrayRef shape, torc
 	TORCH_CHECK(t->scalar_type() == type && t->sizes() == shape && t->device() == like.device(), name, " must be a ", type, " tensor of shape ", l1b_shape(shape),
 		    " on the device of q");
 	TORCH_CHECK(!t->requires_grad(), name, " is a constant: it must not require a gradient");
+	l1b_no_tangent(*t, name);
 	return t->contiguous();
 }
 
@@ -44,6 +45,9 @@ struct Call {
 		TORCH_CHECK(q_.size(3) >= 1 && q_.size(3) <= 256 && v_.size(3) >= 1 && v_.size(3) <= 256, "widths must be 1 to 256");
 		for (int64_t s : {q_.size(0), q_.size(1), q_.size(2)})
 			TORCH_CHECK(s <= 1 << 30, "sizes must be 2^30 at most");
+		l1b_no_tangent(q_, "q");
+		l1b_no_tangent(k_, "k");
+		l1b_no_tangent(v_, "v");
 		q = rows(q_);
 		k = rows(k_);
 		v = rows(v_);

@@ -16,7 +16,7 @@ zeros, and gradients of zero.  A key whose weight is zero contributes nothing, w
 
 Heads of queries may share heads of keys and values (h a multiple of hk).  float32, float16 and bfloat16; widths up to 256.  q, k, v may
 be strided views (of one projection, say) with contiguous rows; others are copied.  The output and the gradients are contiguous.
-Differentiable in q, k and v (sign(0) = 0); the backward is deterministic and keeps one float per query and head beside its inputs, and in 16 bits what rounding
+Differentiable in q, k and v (sign(0) = 0; backward mode, forward-mode tangents are refused); the backward is deterministic and keeps one float per query and head beside its inputs, and in 16 bits what rounding
 left of the output; while it runs it takes up to a gigabyte in 16 bits (a float per pair), and a float per query head and element of k and v where heads are shared.
 In 16 bits, weights are rounded for the value products and for dv (to 22 bits, or 2^-31 of the row's largest, in float16; to 16 in bfloat16)
 and score gradients to 11 bits or 2^-25 of their row's largest (float16: 22, 2^-35); scores, normalisers and all sums are float32.
