@@ -129,7 +129,7 @@ torch::Tensor attend(torch::Tensor q, std::vector<torch::Tensor> cache, torch::T
 	if (slopes.has_value() && slopes->defined()) {
 		TORCH_CHECK(slopes->scalar_type() == torch::kFloat32 && slopes->dim() == 1 && slopes->size(0) == h && slopes->device() == q.device(),
 			    "slopes must be a float32 tensor of shape ", l1b_shape({h}), " on the device of q");
-		TORCH_CHECK(!slopes->requires_grad(), "slopes is a constant: it must not require a gradient");
+		TORCH_CHECK(!(at::GradMode::is_enabled() && slopes->requires_grad()), "slopes is a constant: it must not require a gradient");
 		l1b_no_tangent(*slopes, "slopes");
 		sl = slopes->contiguous();
 	}

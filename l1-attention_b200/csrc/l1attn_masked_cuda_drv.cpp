@@ -9,14 +9,14 @@ using Maybe = c10::optional<torch::Tensor>;
 
 const char *const SHAPES = "q must be [bs, n, h, w], k [bs, n, hk, w], v [bs, n, hk, wv]";
 
-// a small tensor beside q, k, v: its shape, type and device; contiguous.
-torch::Tensor side(const Maybe &t, const char *name, at::IntArrayRef shape, torch::ScalarType type, const torch::Tensor &like)
+// a small tensor beside q, k, v: its shape, type and device; contiguous.  record: gradients are wanted
+torch::Tensor side(const Maybe &t, const char *name, at::IntArrayRef shape, torch::ScalarType type, const torch::Tensor &like, bool record)
 {
 	if (!t.has_value() || !t->defined())
 		return {};
 	TORCH_CHECK(t->scalar_type() == type && t->sizes() == shape && t->device() == like.device(), name, " must be a ", type, " tensor of shape ", l1b_shape(shape),
 		    " on the device of q");
-	TORCH_CHECK(!t->requires_grad(), name, " is a constant: it must not require a gradient");
+	TORCH_CHECK(!(record && t->requires_grad()), name, " is a constant: it must not require a gradient");
 	l1b_no_tangent(*t, name);
 	return t->contiguous();
 }
@@ -30,7 +30,7 @@ struct Call {
 	int bs, n, h, hk, w, wv, type;
 
 	Call(const torch::Tensor &q_, const torch::Tensor &k_, const torch::Tensor &v_, const Maybe &slopes_, const Maybe &doc_, const Maybe &prefix_, int mode, bool causal,
-	     int64_t window, double softcap)
+	     int64_t window, double softcap, bool record)
 	{
 		CHECK_CUDA(q_);
 		CHECK_CUDA(k_);
@@ -51,9 +51,9 @@ struct Call {
 		q = rows(q_);
 		k = rows(k_);
 		v = rows(v_);
-		slopes = side(slopes_, "slopes", {q.size(2)}, torch::kFloat32, q);
-		doc = side(doc_, "doc", {q.size(0), q.size(1)}, torch::kInt32, q);
-		prefix = side(prefix_, "prefix", {q.size(0)}, torch::kInt32, q);
+		slopes = side(slopes_, "slopes", {q.size(2)}, torch::kFloat32, q, record);
+		doc = side(doc_, "doc", {q.size(0), q.size(1)}, torch::kInt32, q, record);
+		prefix = side(prefix_, "prefix", {q.size(0)}, torch::kInt32, q, record);
 		const torch::Tensor *const all[] = {&q, &k, &v};
 		for (int i = 0; i < 9; i++)
 			strides[i] = all[i / 3]->stride(i % 3);
@@ -81,7 +81,7 @@ void *ptr(const torch::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr;
 std::vector<torch::Tensor> forward(torch::Tensor q, torch::Tensor k, torch::Tensor v, Maybe slopes, Maybe doc, Maybe prefix, int mode, bool causal, int64_t window,
 				   double softcap, bool keep)
 {
-	const Call c(q, k, v, slopes, doc, prefix, mode, causal, window, softcap);
+	const Call c(q, k, v, slopes, doc, prefix, mode, causal, window, softcap, keep || at::GradMode::is_enabled());
 	const c10::cuda::CUDAGuard guard(c.q.device());
 	const auto options = c.q.options().requires_grad(false);
 	auto vo = torch::empty({c.bs, c.n, c.h, c.wv}, options);
@@ -99,7 +99,7 @@ std::vector<torch::Tensor> forward(torch::Tensor q, torch::Tensor k, torch::Tens
 std::vector<torch::Tensor> backward(torch::Tensor q, torch::Tensor k, torch::Tensor v, Maybe slopes, Maybe doc, Maybe prefix, int mode, bool causal, int64_t window,
 				    double softcap, torch::Tensor vo, Maybe rest, torch::Tensor lse, torch::Tensor dvo)
 {
-	const Call c(q, k, v, slopes, doc, prefix, mode, causal, window, softcap);
+	const Call c(q, k, v, slopes, doc, prefix, mode, causal, window, softcap, false);
 	TORCH_CHECK(dvo.sizes() == vo.sizes() && dvo.scalar_type() == vo.scalar_type() && dvo.device() == vo.device(), "the gradient must be like the output");
 	const c10::cuda::CUDAGuard guard(c.q.device());
 	dvo = dvo.contiguous();

@@ -6,7 +6,8 @@
 Scores are the framework's: x[t, s] = -(1/sqrt(w)) * sum_w |q_t - k_s|.  Then, each where it is asked for,
 
     x = softcap * tanh(x / softcap)                           a bound on the scores (they lie in (-softcap, 0])
-    x = x - slopes[h] * |t - s|                               a bias that grows with the distance; slopes float32 [h], constants
+    x = x - slopes[h] * |t - s|                               a bias that grows with the distance; slopes float32 [h], constants: refused with
+                                                              a gradient of their own unless gradients are off
     causal, window                                            t sees s <= t; |t - s| < window
     prefix   int32 [bs]                                       keys s < prefix[b] are seen by every query of the item
     doc      int32 [bs, n]                                    t sees s of its own document only; negative: padding, sees nothing, unseen

@@ -1,4 +1,4 @@
-"""What masked attention and the cache make of tensors that carry forward-mode tangents."""
+"""What masked attention and the cache make of tensors that carry forward-mode tangents, and of slopes that are a model's parameters."""
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -39,3 +39,25 @@ def test_tangents_are_refused_by_the_cache():
             with pytest.raises(NotImplementedError):
                 call()
     assert torch.isfinite(m.attend(q, *cache, *places, slopes=slopes)).all()
+
+
+def test_slopes_of_a_model():
+    """Parameters: refused where their gradient would be wanted, taken where none is."""
+    q, k, v, dvo = _inputs(1, 40, 2, 1, 16, 16, F32)
+    slopes = torch.nn.Parameter(torch.tensor([0.1, 0.2], device="cuda"))
+    want = _op()(q, k, v, slopes=slopes.detach()).detach()
+    for x in ((q, k, v), (q.detach(), k.detach(), v.detach())):
+        with pytest.raises(RuntimeError, match="constant"):
+            _op()(*x, slopes=slopes)
+        with torch.no_grad():
+            assert torch.equal(_op()(*x, slopes=slopes), want)
+        with torch.inference_mode():
+            assert torch.equal(_op()(*x, slopes=slopes), want)
+    vo = _op()(q, k, v, slopes=slopes.detach())
+    assert all(torch.isfinite(x).all() for x in torch.autograd.grad(vo, (q, k, v), dvo))
+    m = _mod()
+    cache, places = _random_cache(4, 1, 16, 16, 16), _places([(20, 2)], 16, 4)
+    with pytest.raises(RuntimeError, match="constant"):
+        m.attend(q[0, :2].detach(), *cache, *places, slopes=slopes)
+    with torch.no_grad():
+        assert torch.equal(m.attend(q[0, :2], *cache, *places, slopes=slopes), m.attend(q[0, :2].detach(), *cache, *places, slopes=slopes.detach()))
