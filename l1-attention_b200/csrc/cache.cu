@@ -58,10 +58,13 @@ int plan(AttendArgs *a, int rows, int heads, int max_len, int dtype, size_t *byt
 		*bytes = (2ull * a->ctas * a->tile_rows * part + 255) / 256 * 256 + a->ctas * sizeof(AttendSplit);
 		return L1ATTN_OK;
 	}
-	// splits of the keys: enough CTAs for the GPU, at least 256 keys each
+	// splits of the keys: eight CTAs a multiprocessor (several waves of them even out unequal lengths), at least 256 keys each
+	int sms = 0;
+	if (int rc = multiprocessors(&sms))
+		return rc;
 	a->tile_rows = 16;
 	const long long tiles = (long long)rows * a->group / a->tile_rows + a->c.n_seqs, len = max_len < 1 ? 1 : max_len;
-	long long want = (1184 + tiles * a->c.kv_heads - 1) / (tiles * a->c.kv_heads), most = (len + 255) / 256;
+	long long want = (8 * sms + tiles * a->c.kv_heads - 1) / (tiles * a->c.kv_heads), most = (len + 255) / 256;
 	want = want < most ? want : most;
 	a->split_keys = int(((len + want - 1) / want + 63) / 64 * 64);
 	a->splits = int((len + a->split_keys - 1) / a->split_keys);
