@@ -140,6 +140,10 @@ torch::Tensor attend(torch::Tensor q, std::vector<torch::Tensor> cache, torch::T
 		TORCH_CHECK(vo.dim() == 3 && vo.size(0) == q.size(0) && vo.size(1) == h && vo.size(2) == c.v_width && vo.scalar_type() == q.scalar_type() && vo.device() == q.device() &&
 				    vo.is_contiguous(),
 			    "out must be a contiguous tensor [rows, heads, v_width] of the type of q on its device");
+		// (rows of q are read while others are written)
+		const char *const q0 = static_cast<const char *>(q.data_ptr()), *const v0 = static_cast<const char *>(vo.data_ptr());
+		const int64_t q_span = q.numel() ? ((q.size(0) - 1) * q.stride(0) + (h - 1) * q.stride(1) + c.width) * q.element_size() : 0;
+		TORCH_CHECK(v0 + vo.nbytes() <= q0 || q0 + q_span <= v0 || !vo.numel() || !q_span, "out must not overlap q");
 	} else
 		vo = torch::empty({q.size(0), h, c.v_width}, q.options().requires_grad(false));
 	const int rows = int(q.size(0)), type = l1b_dtype(q, "attend", true);
