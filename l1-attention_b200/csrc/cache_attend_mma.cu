@@ -12,8 +12,8 @@
 // another, and every CTA of one wave takes an equal share, whatever the lengths (known on the device alone): a unit may end in a later CTA's share, and
 // is joined by join_splits_kernel.
 // Bound: instruction issue, 55 % of the slots with 12 warps an SM (168 registers); what every chunk costs (copies, unpacking, weights) is half of it, a query
-// row a tenth or so.  Widths of 128: 37 sequences of 16384 tokens, one query head 269 us (72 % of the rate of a copy), four 406 (47 %); 64 ragged
-// ones of up to 8192, one 138 us, four 202, eight 289.
+// row a tenth or so.  Widths of 128: 37 sequences of 16384 tokens, one query head 266 us (72 % of the rate of a copy), four 415 (46 %); 64 ragged
+// ones of up to 8192, one 138 us, four 203, eight 297.
 #include "cache.cuh"
 #include "mma.cuh"
 
@@ -23,7 +23,9 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr float LOG2E = 1.4426950408889634f, LAG = 8.f;
-constexpr int ENTRY = 11; // chunks that a unit costs beside its own (query rows, lookups, the join; 64 ragged sequences: 5: 231 us, 8: 213, 11: 202, 15: 204)
+// Chunks that a unit costs beside its own (query rows, lookups, the join).  5 / 8 / 11 / 15, ragged sequences, four query heads a group: 64 of up to 8192 tokens
+// 222 / 207 / 203 / 206 us, 256 of 2048 256 / 249 / 231 / 238, 1024 of 500 411 / 401 / 395 / 393; pieces of 256 tokens on 3001, which share units less, 217 / 219 / 223 / 226.
+constexpr int ENTRY = 11;
 using H = Half2<__half>;
 
 __device__ __forceinline__ uint32_t permute(uint32_t a, uint32_t b, uint32_t how)

@@ -8,7 +8,7 @@
 // additions, 9.7 with four minima), so the softmax costs what it takes; forming the next step's distances beside it brought [2,2048,8,128] from
 // 343 to 293 us, the short copy loop a tenth; the weights' rests cost a tenth of it again: with
 // them, and with what rounding leaves of vo kept for delta (masked.cu), dq is as exact as a float32 form's that rounds at the end in bfloat16 (1.38 of its
-// error without).  Now 47 terms per clock and SM at widths of 64 ([4,2048,8,64], no mask: 622 us), 49 at 128 (1.20 ms).
+// error without).  Now 48 terms per clock and SM at widths of 64 ([4,2048,8,64], no mask: 615 us), 49 at 128 (1.20 ms).
 #include "mma.cuh"
 
 namespace l1b {
@@ -83,9 +83,9 @@ template <typename T> __device__ __noinline__ void exact_row(const MaskedArgs &a
 		}
 }
 
-// W: 32-column groups of the width; V: 16-column groups of the value rows (4 or 8).  CTAs of an SM, two against three (168 registers; before the rests' products): [1,4096,8,64]
-// with values of 128 339 / 447 us, [2,2048,8,128] 293 / 472, widths of 32 200 / 235; but [1,8192,8,64] 1230 / 1157 and [4,2048,8,128] with values of 64
-// (no mask) 1179 / 1005.
+// W: 32-column groups of the width; V: 16-column groups of the value rows (4 or 8).  CTAs of an SM, two against three (168 registers), bfloat16: [1,4096,8,64]
+// with values of 128 374 / 509 us, [2,2048,8,128] 327 / 457, widths of 32 227 / 257; but without a mask [4,2048,8,64] 695 / 615, widths of 128 and 96 with values of
+// 64 1168 / 1055 and 863 / 837 (causal [1,8192,8,64] 1264 either way).
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(THREADS, V == 4 && W > 1 ? 3 : 2) masked_fwd_mma_kernel(MaskedArgs a, T *vo, T *rest, float *lse, int tiles, int vec)
 {
@@ -660,7 +660,7 @@ __device__ __forceinline__ unsigned store_signed(const float (&acc)[2 * W][2][4]
 //                     (without it dv is 1.4 times as far from 64 bits as when rounded once; 1.5 % of the time)
 // No atomics, and the same sums in the same order every time.
 // Bound: the tensor pipe and the instructions that feed it, of 8 warps an SM (registers: two CTAs).  [2,2048,8,128], causal, two heads of keys, bfloat16:
-// 1.26 ms; [1,8192,8,64], float16: 5.67 ms; [4,2048,8,128], no mask, bfloat16: 4.38 ms (in float32 arithmetic, masked_simple.cu: 15.6).
+// 1.30 ms; [1,8192,8,64], float16: 6.08 ms; [4,2048,8,128], no mask, bfloat16: 4.49 ms (in float32 arithmetic, masked_simple.cu: 15.6).
 template <typename T, bool OWN_KEYS, int W, int V>
 __global__ void __launch_bounds__(THREADS, 2) masked_bwd_mma_kernel(MaskedArgs a, const T *dvo, const float *lse, const float *delta, T *dx, T *dv, BackwardParts parts, int tiles, int vec)
 {

@@ -21,6 +21,8 @@ Differentiable in q, k and v (sign(0) = 0; backward mode, forward-mode tangents 
 left of the output; while it runs it takes up to a gigabyte in 16 bits (a float per pair), and a float per query head and element of k and v where heads are shared.
 In 16 bits, weights are rounded for the value products and for dv (to 22 bits, or 2^-31 of the row's largest, in float16; to 16 in bfloat16)
 and score gradients to 11 bits or 2^-25 of their row's largest (float16: 22, 2^-35); scores, normalisers and all sums are float32.
+The 16-bit distance (widths to 128) is sum q + sum k - 2 sum min(q, k): exact minima, but its error goes with |q| + |k|, not with |q - k| (up to 3e-5 in
+a score of width 128 where q and k share a channel at 1000, 7e-4 at 10000).
 Everything runs on the tensors' device and the current stream.  No CPU path.  A backward that is captured into a CUDA graph must not share its leaves with an
 eager graph that is still alive: autograd ties a leaf to the stream of its first use (detach or drop the eager outputs before the capture).
 """
