@@ -227,7 +227,8 @@ int l1attn_masked_bwd(const void *q, const void *k, const void *v, const int64_t
  * start[i] + 1, ...; its position p is in page table[i][p / page].  Rows behind cu[n_seqs] belong to no sequence: nothing reads or writes them.
  * table, start and cu are device memory and may change between replays of a captured call.  Entries of table past a sequence's last page
  * are not looked at, nor, by attention, those of pages that lie before the window of its first row.  A page id, a start or an offset out of range is never followed: its tokens are left out (keys: not seen; gathered rows and the outputs of
- * queries without a place: zeros) and *status, where given, is set to L1ATTN_ERR_INDEX.
+ * queries without a place: zeros) and *status, where given, is set to L1ATTN_ERR_INDEX.  (Offsets that do not ascend: outputs of attention at the rows between them
+ * are undefined.)
  */
 typedef struct l1attn_cache {
 	int8_t *k_codes, *v_codes;

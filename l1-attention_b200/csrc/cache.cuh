@@ -42,7 +42,8 @@ L1B_BOTH SeqView cache_seq(const CacheArgs &c, int seq)
 	SeqView v = {cache_row(c, seq), 0, s, 0};
 	if (a < 0 || b < a || b > c.rows || s < 0) {
 		cache_fault(c);
-		const int own = cache_row(c, seq + 1) - v.row;
+		// (an end that is out of order: up to where the next one ends, so that rows of sequences in order stay theirs)
+		const int own = (b < a || b > c.rows ? seq + 2 <= c.n_seqs ? cache_row(c, seq + 2) : c.rows : b) - v.row;
 		v.lost = own > 0 ? own : 0;
 		v.start = 0;
 		return v;

@@ -166,9 +166,9 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(THREADS) gathe
 		return;
 	const int seq = cache_find_warp(c, row, 1, 1, 0);
 	const SeqView sv = cache_seq(c, seq);
-	if (row < sv.row || row - sv.row >= (long long)sv.count + sv.lost)
+	const bool placed = row >= sv.row && row - sv.row < sv.count; // (else zeros, for all that offsets out of order leave to nobody, but behind the last sequence)
+	if (!placed && !(row >= sv.row && row - sv.row < (long long)sv.count + sv.lost) && (row < cache_row(c, 0) || row >= cache_row(c, c.n_seqs)))
 		return;
-	const bool placed = row - sv.row < sv.count; // (else zeros)
 	const int pos = placed ? sv.start + int(row - sv.row) : 0, id = placed ? cache_page(c, seq, pos / c.page) : -1;
 	const long long at = (long long)max(id, 0) * c.kv_heads;
 	for (int values = 0; values < 2; values++) {

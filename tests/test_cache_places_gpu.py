@@ -57,3 +57,28 @@ def test_many_sequences_some_without_a_place():
         rows = bad.repeat_interleave(3)
         assert not out[rows].any()
         assert torch.equal(out[~rows], want[~rows]) or float((out[~rows].double() - want[~rows].double()).abs().max()) <= torch.finfo(dt).eps * float(want.abs().max())
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("cu,zero", [([0, 9, 3, 7], [0, 1, 2]), ([0, 3, 3, 9], [3, 4, 5, 6]), ([0, 2, -1, 7], [2, 3, 4, 5, 6]), ([0, 3, 9, 7], [3, 4, 5, 6])])
+def test_offsets_out_of_range(cu, zero, dt):
+    """One offset beyond the rows or below zero: the sequences that it is no end of stay right, gathered rows hold values or zeros."""
+    m = _mod()
+    cache = _random_cache(8, 2, 16, 32, 32, seed=1)
+    table, start = _at(3, 1, 0, 2, 7, 5).view(3, 2), _at(1, 5, 2)
+    good = [i for i in range(3) if 0 <= cu[i] <= cu[i + 1] <= 7]
+    q = torch.randn(7, 4, 32, generator=torch.Generator().manual_seed(2)).to(dt).cuda()
+    status = _at(0)
+    out = torch.full((7, 4, 32), math.nan, dtype=dt, device="cuda")
+    m.attend(q, *cache, table, start, _at(*cu), out=out, status=status)
+    assert int(status) != 0
+    kv = tuple(torch.full((7, 2, 32), math.nan, dtype=dt, device="cuda") for _ in range(2))
+    status.zero_()
+    m.gather(*cache, table, start, _at(*cu), 7, dtype=dt, out=kv, status=status)
+    assert int(status) != 0 and not any(x.isnan().any() for x in kv)
+    if dt != F32:  # (the 16-bit kernel looks at every sequence for itself)
+        assert not out[zero].any()
+        for i in good:
+            rows = slice(cu[i], cu[i + 1])
+            alone = m.attend(q[rows].contiguous(), *cache, table[i:i + 1], start[i:i + 1], _at(0, cu[i + 1] - cu[i]))
+            assert ((out[rows].double() - alone.double()).abs() <= 2 * torch.finfo(dt).eps * (1 + alone.double().abs())).all()
