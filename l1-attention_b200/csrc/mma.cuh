@@ -5,7 +5,7 @@
 // The minimum of two 16-bit values is exact, two at a time in one instruction; the sum over w is a product with ones: mma.m16n8k16, float32 accumulators.  What the three sums
 // are off by goes with |q| + |k|, not with the distance: for a channel that q and k share at 1e3, 1e4, 1e5, 1e6 a score (128 wide) was off by 3e-5, 7e-4, 6e-3, 0.1 at most
 // (next to a step of the channel itself of 4, 64, 512, 4096 in bfloat16).
-//  A's 16 rows are 16 (query, key) pairs; which of
+// A's 16 rows are 16 (query, key) pairs; which of
 // the eight columns gets their sums is chosen by B, ones in that column and zeros elsewhere, so that eight such products fill a 16 x 8
 // tile of scores in the layout that the value product reads.  256 terms per mma, which issues every 8 clocks per scheduler: 128 terms per clock and
 // SM at most, where float32 subtraction and addition of |.| reach 64.  Measured for the loop alone: 90 terms per clock and SM with 16 warps, 86 with 8.
